@@ -45,7 +45,7 @@ def build_cpu() -> Path:
 
 
 def build_ref(cuda: bool = True) -> bool:
-    if not REF.exists():
+    if not (REF / "engines").exists():        # no checkout, or an empty directory in its place
         return False
     OUT.mkdir(exist_ok=True)
     glm = REF / "engines/hayate/crates/kernels/cu/glm53"
