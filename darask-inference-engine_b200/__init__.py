@@ -13,6 +13,7 @@ from .tsumuji import TsumujiMoeLayer  # noqa: F401
 from .hayate import HayateMoeLayer  # noqa: F401
 from .fp8 import Fp8MoeLayer  # noqa: F401
 from . import fp8  # noqa: F401
+from . import kogarashi  # noqa: F401
 from . import ep  # noqa: F401
 from . import gguf  # noqa: F401
 from . import tsumuji_loader  # noqa: F401

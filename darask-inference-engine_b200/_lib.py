@@ -64,7 +64,34 @@ class DaraskFp8Moe(ctypes.Structure):
     ]
 
 
+class DaraskFp8Linear(ctypes.Structure):
+    """Mirror of `DaraskFp8Linear` in include/darask_moe_b200.h."""
+    _fields_ = [
+        ("m", c_int), ("n", c_int), ("k", c_int),
+        ("x", c_void_p), ("x_ty", c_int), ("ldx", c_longlong), ("x_scales", c_void_p), ("ld_xs", c_longlong), ("swiglu", c_int),
+        ("w", c_void_p), ("ldw", c_longlong), ("w_scales", c_void_p), ("ld_ws", c_longlong),
+        ("out", c_void_p), ("out_ty", c_int), ("ldo", c_longlong), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class DaraskGgmlGrouped(ctypes.Structure):
+    """Mirror of `DaraskGgmlGrouped` in include/darask_moe_b200.h."""
+    _fields_ = [
+        ("groups", c_int), ("n", c_int), ("k", c_int), ("rows", c_longlong), ("ranges", c_void_p),
+        ("x", c_void_p), ("x_ty", c_int), ("ldx", c_longlong), ("x_rows", c_longlong),
+        ("assignments", c_void_p), ("topk", c_int), ("swiglu", c_int),
+        ("w", c_void_p), ("w_up", c_void_p), ("w_ty", c_int),
+        ("out", c_void_p), ("out_ty", c_int), ("ldo", c_longlong), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 _SIGNATURES = {
+    "darask_fp8_linear_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "darask_fp8_linear": (c_int, [ctypes.POINTER(DaraskFp8Linear), c_void_p]),
+    "darask_fp8_linear_status": (c_int, [ctypes.POINTER(c_uint), c_void_p]),
+    "darask_ggml_grouped_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int]),
+    "darask_ggml_grouped_gemm": (c_int, [ctypes.POINTER(DaraskGgmlGrouped), c_void_p]),
+    "darask_ggml_grouped_status": (c_int, [ctypes.POINTER(c_uint), c_void_p]),
     "darask_route_topk": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_float, c_void_p, c_void_p,
                                   c_void_p, c_void_p]),
     "darask_route_topk_hayate": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_float, c_void_p, c_void_p,
@@ -169,6 +196,18 @@ def lib() -> ctypes.CDLL:
 
 class CudaError(RuntimeError):
     pass
+
+
+# float types as the C ABI names them (GGML ids); filled on first use so that importing this module does not import torch
+_FLOAT_TYPES: dict = {}
+
+
+def float_type(dtype) -> int | None:
+    """GGML id of a torch float type the kernels read and write, or None."""
+    if not _FLOAT_TYPES:
+        import torch
+        _FLOAT_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+    return _FLOAT_TYPES.get(dtype)
 
 
 def check(code: int, what: str) -> None:

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .formats import GGML_Q6_K, ggml_tensor_bytes
+from .formats import GGML_Q4_K, GGML_Q6_K, ggml_tensor_bytes, q6k_r16_row_bytes
 
 TENSORS = ("ffn_gate_inp.weight", "ffn_gate_exps.weight", "ffn_up_exps.weight", "ffn_down_exps.weight",
            "ffn_gate_shexp.weight", "ffn_up_shexp.weight", "ffn_down_shexp.weight", "ffn_gate_inp_shexp.weight")
@@ -26,6 +26,72 @@ class Weight:
     k: int
     rows: int
     ne: tuple
+
+
+def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=False, out_dtype=None, out=None):
+    """Product grouped by expert over GGUF weights: out[i] = x[row(i)] . W_g^T for the rows i of every group g.
+    weight: a Q4_K or Q6_K `Weight` of GGML order [k, n, groups] as ``KogarashiMoeLayer.load`` keeps it (Q6_K regrouped);
+    with `up`, a second one of the same shape, out holds both products side by side ([rows, 2n]).  ranges int32 [groups, 2] =
+    {rows, offset}.  x float32, float16 or bfloat16 [*, k]; dispatch row i reads x row assignments[i] // topk (int32, on the
+    device), or row i without assignments.  With `swiglu` the rows of x hold gate | up ([*, 2k]) and silu(gate) * up is multiplied.
+    Sums are float32; `out_dtype` defaults to x's type.  Rows outside every range are left as they were (uninitialised when
+    `out` is not given).  Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
+    k, n, groups = weight.k, weight.rows, weight.ne[2] if len(weight.ne) > 2 else 1
+    if weight.ty not in (GGML_Q4_K, GGML_Q6_K) or k < 256 or k % 256 or n < 1 or not 1 <= groups <= 1024:
+        raise ValueError("weight must be Q4_K or Q6_K [k % 256 == 0, n, groups <= 1024]")
+    if up is not None and (up.ty, up.k, up.rows, tuple(up.ne)) != (weight.ty, k, n, tuple(weight.ne)):
+        raise ValueError("up must have the type and shape of weight")
+    row_bytes = k // 256 * 144 if weight.ty == GGML_Q4_K else q6k_r16_row_bytes(k)
+    data = [w.data for w in (weight, up) if w is not None]
+    if any(t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != groups * n * row_bytes or t.data_ptr() % 16 for t in data):
+        raise ValueError(f"weight data must be {groups * n * row_bytes} contiguous bytes on a 16-byte boundary")
+    ty = _lib.float_type(x.dtype)
+    if ty is None or x.dim() != 2 or x.shape[1] != (2 * k if swiglu else k):
+        raise ValueError(f"x must be float32, float16 or bfloat16 rows of {2 * k if swiglu else k} columns")
+    if ranges.dtype != torch.int32 or tuple(ranges.shape) != (groups, 2) or not ranges.is_contiguous():
+        raise ValueError(f"ranges must be contiguous int32 [{groups}, 2]")
+    rows = x.shape[0]
+    if assignments is not None:
+        if assignments.dtype != torch.int32 or assignments.dim() != 1 or not assignments.is_contiguous() or topk < 1:
+            raise ValueError("assignments must be contiguous int32 [rows], topk at least 1")
+        rows = assignments.numel()
+    width = n * len(data)
+    if out is None:
+        out = torch.empty((rows, width), dtype=out_dtype or x.dtype, device=x.device)
+    elif tuple(out.shape) != (rows, width) or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out must be [{rows}, {width}]")
+    out_ty = _lib.float_type(out.dtype)
+    tensors = [x, ranges, out] + data + ([assignments] if assignments is not None else [])
+    if out_ty is None or not x.is_cuda or any(t.device != x.device for t in tensors):
+        raise ValueError("tensors must share one CUDA device, out must be float32, float16 or bfloat16")
+    if any(t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]) for t in (x, out)):
+        raise ValueError("x and out must have unit column stride and rows that do not overlap")
+    if rows == 0:
+        return out
+    lib = _lib.lib()
+    d = _lib.DaraskGgmlGrouped()
+    d.groups, d.n, d.k, d.rows, d.ranges = groups, n, k, rows, ranges.data_ptr()
+    d.x, d.x_ty, d.ldx, d.x_rows = x.data_ptr(), ty, max(x.stride(0), x.shape[1]), x.shape[0]
+    if assignments is not None:
+        d.assignments = assignments.data_ptr()
+    d.topk, d.swiglu = topk, int(swiglu)
+    d.w, d.w_up, d.w_ty = data[0].data_ptr(), data[1].data_ptr() if up is not None else None, weight.ty
+    d.out, d.out_ty, d.ldo = out.data_ptr(), out_ty, max(out.stride(0), width)
+    with torch.cuda.device(x.device):
+        nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        d.workspace, d.workspace_bytes = scratch.data_ptr(), nbytes
+        _lib.check(lib.darask_ggml_grouped_gemm(ctypes.byref(d), torch.cuda.current_stream(x.device).cuda_stream), "darask_ggml_grouped_gemm")
+    return out
+
+
+def grouped_status(device="cuda") -> int:
+    """Status bits that `grouped_gemm` calls on this device have set since the last look; clears them and synchronizes the current stream."""
+    s = ctypes.c_uint(0)
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().darask_ggml_grouped_status(ctypes.byref(s), torch.cuda.current_stream(device).cuda_stream), "darask_ggml_grouped_status")
+    return s.value
 
 
 class KogarashiMoeLayer:

@@ -381,6 +381,63 @@ int darask_fp8_ep_reduce(const float* y, const unsigned* ranges, int local_exper
                          unsigned* status, darask_stream_t stream);
 int darask_fp8_ep_sum(float* out, const float* zr, int ranks, int tokens, int tcap, int hidden, darask_stream_t stream);
 
+/* ---- dense product in block-scaled FP8 ---------------------------------------------------------------------------
+ * out[i][j] = sum over 128-column blocks b of (code(x)[i][b] . w[j][b]) * sx[i][b] * w_scales[j / 128][b], sums in float32,
+ * rounded once to out's type: the dense counterpart of darask_fp8_grouped_gemm (projections, shared experts of an
+ * `Fp8Block` checkpoint), for any m >= 0 (0: nothing is enqueued), n >= 1, k >= 1.
+ *   x        float rows (DARASK_GGML_F32 / F16 / BF16): quantized by the call as darask_quantize_fp8_act does, a last block
+ *            of fewer than 128 columns on its own; a block with an infinity or a NaN makes its row NaN.
+ *            DARASK_E4M3: e4m3 codes with x_scales [m][ld_xs] (16-byte aligned rows).
+ *   swiglu   float x only: rows hold gate | up (2k columns) and silu(gate) * up, in float32, is quantized.
+ *   w        e4m3 [n][ldw], 16-byte aligned rows; w_scales float32 [ceil(n/128)][ld_ws], ld_ws >= ceil(k/128).
+ *   ld*      row strides in elements.  out must not overlap an input.
+ *   workspace  darask_fp8_linear_workspace_bytes(m, n, k, x_ty) bytes, 256-byte aligned (0 bytes: may be NULL), not shared by
+ *            calls that can overlap; nothing has to be initialised and nothing is kept between calls.
+ * darask_fp8_linear_status copies the device's status word (DARASK_STATUS_WAIT_TIMEOUT) to *host_status and clears it; it
+ * synchronizes the stream. */
+enum { DARASK_E4M3 = 100 };
+typedef struct {
+  int m, n, k;
+  const void* x; int x_ty; long long ldx;
+  const float* x_scales; long long ld_xs;
+  int swiglu;
+  const void* w; long long ldw;
+  const float* w_scales; long long ld_ws;
+  void* out; int out_ty; long long ldo;
+  void* workspace; size_t workspace_bytes;
+} DaraskFp8Linear;
+size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_ty);
+int darask_fp8_linear(const DaraskFp8Linear* desc /* host */, darask_stream_t stream);
+int darask_fp8_linear_status(unsigned* host_status /* host */, darask_stream_t stream);
+
+/* ---- product grouped by expert over GGUF weights ------------------------------------------------------------------
+ * out[i][j] = x[row(i)] . w_g[j] for the dispatch rows i in [offset, offset + rows) of every group g (ranges as from
+ * darask_moe_permute), the prefill counterpart of the Kogarashi layer's expert products.
+ *   w, w_up  Q4_K (GGUF bytes) or Q6_K (after darask_q6k_repack) tensors in GGML order [k, n, groups], 16-byte aligned;
+ *            with w_up, out rows hold x . w | x . w_up (2n columns).  k % 256 == 0, k <= 65536, groups <= 1024.
+ *   x        float32 / f16 / bf16 rows, x_rows of them; row(i) = assignments[i] / topk, or i without assignments.
+ *   swiglu   rows of x hold gate | up (2k columns) and silu(gate) * up is multiplied (the down product).
+ *   out      [rows][ldo]; rows outside every range are left as they were.
+ * Sums in float32; weights enter as exact integers (Q4_K, Q6_K: block scale times an integer), float32 rows as two f16
+ * parts (22 bits), f16 and bf16 rows as they are, with one power of two per row taken out first.  An infinity or a NaN in a row
+ * makes the row's outputs NaN.  A range that leaves [0, rows) is cut and a row(i) >= x_rows reads as zeros; both set
+ * DARASK_STATUS_BAD_ROUTE in the device's status word (darask_ggml_grouped_status, as darask_fp8_linear_status).
+ * workspace: darask_ggml_grouped_workspace_bytes(rows, k, x_ty) bytes, 256-byte aligned, as for darask_fp8_linear. */
+typedef struct {
+  int groups, n, k;
+  long long rows;
+  const unsigned* ranges;               /* [groups][2] {rows, offset} */
+  const void* x; int x_ty; long long ldx; long long x_rows;
+  const unsigned* assignments; int topk;
+  int swiglu;
+  const void* w; const void* w_up; int w_ty;
+  void* out; int out_ty; long long ldo;
+  void* workspace; size_t workspace_bytes;
+} DaraskGgmlGrouped;
+size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int x_ty);
+int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* desc /* host */, darask_stream_t stream);
+int darask_ggml_grouped_status(unsigned* host_status /* host */, darask_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
