@@ -4,27 +4,11 @@
 // e4m3 with one float32 scale per row and 128 columns (as darask_quantize_fp8_act), or codes and scales as they are.
 #include "../../include/darask_moe_b200.h"
 #include <cuda_fp8.h>
-#include "row_source.cuh"
-#include "stream_launch.cuh"
+#include "fp8_linear_stream.cuh"
 
 namespace dmoe {
 
 static __device__ unsigned g_fp8_linear_status;
-
-struct Fp8LinearArgs {
-  int m, n, k;
-  const uint8_t* codes;  // e4m3 rows
-  long long ldx;
-  const float* xs;
-  long long ld_xs;
-  const uint8_t* w;
-  long long ldw;
-  const float* ws;
-  long long ld_ws;
-  void* out;
-  int out_ty;
-  long long ldo;
-};
 
 // One warp per row and 128 columns, four columns per lane: scale = absmax / 448 (1 for zeros), code = e4m3(x * (1 / scale)),
 // every step rounded to float32. A group with an infinity or a NaN gets the scale NaN, so that the row's products say so.
@@ -36,58 +20,38 @@ __global__ void __launch_bounds__(256) fp8_linear_quant_kernel(const RowSource s
   const int lane = threadIdx.x & 31, b = int(w % kb);
   float v[4];
   row_source_load4(src, w / kb, b * 128 + lane * 4, v);
-  // the bits of |v| grow with |v|, infinity and NaN on top
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  top = __reduce_max_sync(0xffffffffu, top);
-  const float scale = top == 0u ? 1.f : top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(top) / 448.f;
-  const float inv = 1.f / scale;
-  uint32_t out = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float y = v[i] * inv;            // 0 times the infinite reciprocal of a subnormal scale stays 0
-    out |= uint32_t(__nv_cvt_float_to_fp8(y == y ? fminf(fmaxf(y, -448.f), 448.f) : 0.f, __NV_SATFINITE, __NV_E4M3)) << (8 * i);
-  }
+  uint32_t out;
+  const float scale = fp8_group(v, &out);
   if (lane == 0) scales[w] = scale;
   reinterpret_cast<uint32_t*>(codes)[w * 32 + lane] = out;
 }
 
-// 32 x 32 outputs per block, operands of one 128-column block in shared memory as float32.
-__global__ void __launch_bounds__(256) fp8_linear_kernel(const Fp8LinearArgs a) {
-  __shared__ float xt[32][129], wt[32][129];
-  pdl_wait();
-  pdl_launch();
-  const int j0 = blockIdx.x * 32;
-  for (int i0 = blockIdx.y * 32; i0 < a.m; i0 += gridDim.y * 32) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int tj = threadIdx.x & 31, ti = threadIdx.x >> 5;
-    for (int b = 0; b * 128 < a.k; ++b) {
-      __syncthreads();
-      for (int e = threadIdx.x; e < 32 * 128; e += 256) {
-        const int r = e >> 7, c = b * 128 + (e & 127);
-        const bool xin = i0 + r < a.m && c < a.k, win = j0 + r < a.n && c < a.k;
-        const uint8_t xc = xin ? a.codes[size_t(i0 + r) * size_t(a.ldx) + c] : 0, wc = win ? a.w[size_t(j0 + r) * size_t(a.ldw) + c] : 0;
-        xt[r][e & 127] = __half2float(__half(__nv_cvt_fp8_to_halfraw(xc, __NV_E4M3)));
-        wt[r][e & 127] = __half2float(__half(__nv_cvt_fp8_to_halfraw(wc, __NV_E4M3)));
-      }
-      __syncthreads();
-      if (j0 + tj < a.n) {
-        const float sw = a.ws[size_t((j0 + tj) / 128) * size_t(a.ld_ws) + b];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int i = ti + 8 * q;
-          if (i0 + i >= a.m) continue;
-          float p = 0.f;
-          for (int c = 0; c < 128; ++c) p = fmaf(xt[i][c], wt[tj][c], p);
-          acc[q] = fmaf(p, a.xs[size_t(i0 + i) * size_t(a.ld_xs) + b] * sw, acc[q]);
-        }
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (i0 + ti + 8 * q < a.m && j0 + tj < a.n) store_elem(a.out, a.out_ty, size_t(i0 + ti + 8 * q) * size_t(a.ldo) + j0 + tj, acc[q]);
+// What a call runs: rows of x per tile, blocks per cluster, whether the rows are quantized inside the product's launch.
+struct LinearPlan { int nt, splits; bool fused; };
+static LinearPlan linear_plan(int m, int n, int kb, bool codes) {
+  LinearPlan p;
+  p.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  const long long tiles = (long long)((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
+  p.splits = 1;
+  while (p.splits < 8 && tiles * p.splits * 2 <= sm_count() && p.splits * 2 <= kb) p.splits *= 2;
+  p.fused = !codes && m <= 16 && (kb + p.splits - 1) / p.splits <= kFsResident;
+  return p;
+}
+
+template <int NT, bool FUSED>
+static cudaError_t launch_stream(const CUtensorMap& mw, const CUtensorMap& mx, const FsArgs& a, int tiles, int splits, cudaStream_t st) {
+  static bool configured[64] = {};      // the opt-in is per device and per kernel
+  const int dev = current_device_slot();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  auto kernel = fp8_linear_stream_kernel<NT, FUSED>;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               FUSED ? kFsFusedSmem + kFsResident * (2048 + 64) : FsShape<NT>::kSmem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
   }
+  const size_t smem = FUSED ? size_t(kFsFusedSmem) + size_t((a.kb + splits - 1) / splits) * (2048 + 64) : size_t(FsShape<NT>::kSmem);
+  return launch_cluster(kernel, dim3(unsigned(tiles) * unsigned(splits)), dim3(kFsThreads), smem, unsigned(splits), st, mw, mx, a);
 }
 
 static size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -121,22 +85,41 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
   if (!linear_ok(d)) return cudaErrorInvalidValue;
   if (d->m == 0) return cudaSuccess;
   const int kb = (d->k + 127) / 128;
-  Fp8LinearArgs a = {};
-  a.m = d->m; a.n = d->n; a.k = d->k;
-  a.w = static_cast<const uint8_t*>(d->w); a.ldw = d->ldw; a.ws = d->w_scales; a.ld_ws = d->ld_ws;
+  void* status = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&status, g_fp8_linear_status);
+  if (e != cudaSuccess) return e;
+  const bool codes = d->x_ty == DARASK_E4M3;
+  const LinearPlan p = linear_plan(d->m, d->n, kb, codes);
+  FsArgs a = {};
+  a.m = d->m; a.n = d->n; a.kb = kb;
+  a.ws = d->w_scales; a.ld_ws = d->ld_ws;
   a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo;
-  if (d->x_ty == DARASK_E4M3) {
-    a.codes = static_cast<const uint8_t*>(d->x); a.ldx = d->ldx; a.xs = d->x_scales; a.ld_xs = d->ld_xs;
-  } else {
-    uint8_t* codes = static_cast<uint8_t*>(d->workspace);
-    float* scales = reinterpret_cast<float*>(codes + round_up(size_t(d->m) * kb * 128, 256));
-    const RowSource src{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
+  a.tiles_n = (d->n + 127) / 128;
+  a.status = static_cast<unsigned*>(status);
+  a.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, codes ? 0 : row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
+  const uint8_t* xc = static_cast<const uint8_t*>(d->x);
+  unsigned long long pitch = d->ldx, cols = d->k;
+  a.xs = d->x_scales; a.ld_xs = d->ld_xs;
+  if (!codes && !p.fused) {
+    uint8_t* q = static_cast<uint8_t*>(d->workspace);
+    float* scales = reinterpret_cast<float*>(q + round_up(size_t(d->m) * kb * 128, 256));
     const long long groups = (long long)d->m * kb;
-    const cudaError_t e = launch_pdl(fp8_linear_quant_kernel, dim3(unsigned((groups + 7) / 8)), dim3(256), 0, st, src, groups, kb, codes, scales);
-    if (e) return e;
-    a.codes = codes; a.ldx = (long long)kb * 128; a.xs = scales; a.ld_xs = kb;
+    if ((e = launch_pdl(fp8_linear_quant_kernel, dim3(unsigned((groups + 7) / 8)), dim3(256), 0, st, a.src, groups, kb, q, scales))) return e;
+    xc = q; pitch = cols = (unsigned long long)kb * 128; a.xs = scales; a.ld_xs = kb;
   }
-  return launch_pdl(fp8_linear_kernel, dim3((d->n + 31) / 32, unsigned((d->m + 31) / 32 < 65535 ? (d->m + 31) / 32 : 65535)), dim3(256), 0, st, a);
+  CUtensorMap mw, mx;
+  if (!byte_map(&mw, d->w, d->n, d->k, d->ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return cudaErrorInvalidValue;
+  if (p.fused) mx = mw;                 // not read
+  else if (!byte_map(&mx, xc, d->m, cols, pitch, p.nt, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return cudaErrorInvalidValue;
+  const long long tiles = (long long)a.tiles_n * ((d->m + p.nt - 1) / p.nt);
+  if (tiles * p.splits > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (p.fused) return launch_stream<16, true>(mw, mx, a, int(tiles), p.splits, st);
+  switch (p.nt) {
+    case 16: return launch_stream<16, false>(mw, mx, a, int(tiles), p.splits, st);
+    case 32: return launch_stream<32, false>(mw, mx, a, int(tiles), p.splits, st);
+    case 64: return launch_stream<64, false>(mw, mx, a, int(tiles), p.splits, st);
+    default: return launch_stream<128, false>(mw, mx, a, int(tiles), p.splits, st);
+  }
 }
 
 extern "C" int darask_fp8_linear_status(unsigned* host_status, cudaStream_t st) {

@@ -1,0 +1,279 @@
+// Few rows of x: the dense block-scaled FP8 product as a stream of the weights.
+// A block computes 128 weight rows x NT rows of x over its part of k: the weight tile is the M = 128 operand and the rows of x
+// are the N operand of tcgen05.mma kind::f8f6f4, so a single token costs a 16-wide tile and not a 128-wide one. The `cluster`
+// blocks of a cluster split k (128-column blocks) among them and add their float32 tiles through distributed shared memory in
+// rank order: no scratch in HBM, no atomics, the same bits in every call.
+//   warp 0      TMA: weight tile (and the tile of x unless it is quantized here) of one 128-column block per ring stage
+//   warp 1      tcgen05.mma, four per block of k, into one of four TMEM buffers of NT columns
+//   warps 2-3   the factors sx * sw of the blocks, eight blocks of k at a time, two groups ahead of their use
+//   warps 4-7   tcgen05.ld of the block's partial tile (thread = one weight row), times the factors, added in registers
+// FUSED: x comes as float rows; before the loop all warps but 0 and 1 quantize this block's part of x straight into the
+// swizzled operand tiles, which stay in shared memory (16 rows, at most kFsResident blocks of k): one launch in all.
+#pragma once
+#include <cuda_fp8.h>
+#include "row_source.cuh"
+#include "tcgen05.cuh"
+
+namespace dmoe {
+
+constexpr int kFsThreads = 256;
+constexpr int kFsResident = 32;              // blocks of k a FUSED block holds of x
+constexpr int kFsGroup = 8;                  // blocks of k whose factors travel together
+constexpr int kFsBufs = 4;                   // TMEM buffers
+
+struct FsArgs {
+  int m, n, kb;                              // kb: blocks of k in all
+  RowSource src;                             // FUSED
+  const float* xs;                           // otherwise [m][ld_xs]
+  long long ld_xs;
+  const float* ws;                           // [ceil(n/128)][ld_ws]
+  long long ld_ws;
+  void* out;
+  int out_ty;
+  long long ldo;
+  int tiles_n;                               // ceil(n/128)
+  unsigned* status;
+};
+
+template <int NT>
+struct FsShape {
+  static constexpr int kStages = NT <= 32 ? 5 : NT == 64 ? 8 : 6;
+  static constexpr int kStageBytes = 128 * 128 + NT * 128;
+  static constexpr int kFactorFloats = 2 * kFsGroup * NT;
+  static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr int kTmemCols = kFsBufs * NT < 32 ? 32 : kFsBufs * NT;
+  static constexpr int kSmem = 1024 + kRingBytes + kFactorFloats * 4;
+  static_assert(kRingBytes >= NT * 128 * 4, "the joined tile reuses the ring");
+};
+// FUSED (16 rows): ring of weight tiles only, resident x tiles and their factors
+constexpr int kFsFusedStages = 5;
+constexpr int kFsFusedSmem = 1024 + kFsFusedStages * 128 * 128;       // + blocks of k of this block * (16 * 128 + 16 * 4)
+
+// scale and e4m3 codes of one 128-column group, four columns per lane (see fp8_linear_quant_kernel)
+DEVI float fp8_group(const float (&v)[4], uint32_t* codes) {
+  // the bits of |v| grow with |v|, infinity and NaN on top
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float scale = top == 0u ? 1.f : top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(top) / 448.f;
+  const float inv = 1.f / scale;
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = v[i] * inv;            // 0 times the infinite reciprocal of a subnormal scale stays 0
+    out |= uint32_t(__nv_cvt_float_to_fp8(y == y ? fminf(fmaxf(y, -448.f), 448.f) : 0.f, __NV_SATFINITE, __NV_E4M3)) << (8 * i);
+  }
+  *codes = out;
+  return scale;
+}
+
+template <int NT, bool FUSED>
+__global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                       const __grid_constant__ CUtensorMap map_x, const FsArgs a) {
+  static_assert(!FUSED || NT == 16, "rows quantized in the kernel: one tile of 16");
+  using S = FsShape<NT>;
+  constexpr int kStages = FUSED ? kFsFusedStages : S::kStages;
+  constexpr int kStageBytes = FUSED ? 128 * 128 : S::kStageBytes;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kStages], empty[kStages], tfull[kFsBufs], tempty[kFsBufs], ffull[2], fempty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const uint32_t rank = cluster_rank();
+  const int tile = int(blockIdx.x / splits), n0 = (tile % a.tiles_n) * 128, t0 = (tile / a.tiles_n) * NT;
+  const int kb0 = int((long long)a.kb * rank / splits), kbs = int((long long)a.kb * (rank + 1) / splits) - kb0;
+  uint8_t* xres = ring + kFsFusedStages * 128 * 128;                               // FUSED: kbs tiles of 16 x 128 bytes
+  float* factors = reinterpret_cast<float*>(FUSED ? xres + size_t(kbs) * 16 * 128 : ring + S::kRingBytes);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+    for (int b = 0; b < kFsBufs; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, 4); }
+    for (int b = 0; b < 2; ++b) { mbar_init(ffull + b, 2); mbar_init(fempty + b, 4); }
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc<S::kTmemCols>(&tmem_slot);
+  pdl_wait();
+  pdl_launch();
+  auto load_stage = [&](int i) {
+    const int s = i % kStages;
+    const uint32_t dst = smem_u32(ring + s * kStageBytes);
+    mbar_arrive_expect_tx(full + s, kStageBytes);
+    tma_load_2d(dst, &map_w, (kb0 + i) * 128, n0, full + s);
+    if (!FUSED) tma_load_2d(dst + 128 * 128, &map_x, (kb0 + i) * 128, t0, full + s);
+  };
+  if (FUSED) {
+    // the first weight tiles travel while x is quantized (thread 0 has initialised the barriers that it uses here)
+    if (threadIdx.x == 0)
+      for (int i = 0; i < kStages && i < kbs; ++i) load_stage(i);
+    if (warp >= 2) {
+      // group = (block of k, row); rows past m: zero codes and factors
+      const int groups = kbs * 16;
+      for (int g0 = (warp - 2); g0 < groups; g0 += 6 * 4) {
+        float v[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int g = g0 + 6 * u, row = g & 15;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
+          if (g < groups && row < a.m) row_source_load4(a.src, row, (kb0 + (g >> 4)) * 128 + lane * 4, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int g = g0 + 6 * u, b = g >> 4, row = g & 15;
+          if (g >= groups) break;
+          uint32_t codes;
+          const float scale = fp8_group(v[u], &codes);
+          // 128-byte rows, 16-byte pieces swizzled by the row in its group of eight
+          *reinterpret_cast<uint32_t*>(xres + size_t(b) * 2048 + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = codes;
+          if (lane == 0) factors[b * 16 + row] = row < a.m ? scale * __ldg(a.ws + size_t(n0 / 128) * size_t(a.ld_ws) + kb0 + b) : 0.f;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
+  constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(NT >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+  float acc[NT];
+#pragma unroll
+  for (int c = 0; c < NT; ++c) acc[c] = 0.f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = FUSED ? (kbs < kStages ? kbs : kStages) : 0;
+      for (int i = issued; i < kbs && !abort_flag; ++i, ++issued) {
+        if (i >= kStages && !mbar_wait_suspend(empty + i % kStages, ((i / kStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+        load_stage(i);
+      }
+      // after a timeout the copies in flight land before the block ends
+      if (abort_flag)
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_wait_suspend(full + i % kStages, (i / kStages) & 1, a.status);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < kbs && !abort_flag; ++i) {
+        const int s = i % kStages, buf = i % kFsBufs;
+        if (i >= kFsBufs && !mbar_wait_suspend(tempty + buf, ((i / kFsBufs) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+        if (!mbar_wait_suspend(full + s, (i / kStages) & 1, a.status)) { abort_flag = 1; break; }
+        tmem_fence_after();
+        const uint32_t sw = smem_u32(ring + s * kStageBytes);
+        const uint64_t dw = umma_desc_k128(sw), dx = umma_desc_k128(FUSED ? smem_u32(xres + size_t(i) * 2048) : sw + 128 * 128);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          asm volatile(
+              "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+              "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+              ::"r"(tmem + buf * NT), "l"(dw + 2 * q), "l"(dx + 2 * q), "r"(kIdesc), "r"(q ? 1u : 0u), "r"(0u) : "memory");
+        umma_commit(empty + s);
+        umma_commit(tfull + buf);
+      }
+    }
+  } else if (warp < 4) {
+    if (!FUSED) {
+      const int ft = threadIdx.x - 64;                            // 0 .. 63
+      const float* ws = a.ws + size_t(n0 / 128) * size_t(a.ld_ws) + kb0;
+      for (int g = 0; g * kFsGroup < kbs; ++g) {
+        const int slot = g & 1, b0 = g * kFsGroup;
+        float v[NT * kFsGroup / 64];
+#pragma unroll
+        for (int j = 0; j < NT * kFsGroup / 64; ++j) {             // element = (row, block of k): eight neighbours share a row
+          const int e = j * 64 + ft, row = e / kFsGroup, b = b0 + e % kFsGroup;
+          v[j] = t0 + row < a.m && b < kbs ? __ldg(a.xs + size_t(t0 + row) * size_t(a.ld_xs) + kb0 + b) * __ldg(ws + b) : 0.f;
+        }
+        int ok = 1;
+        if (g >= 2 && lane == 0) ok = mbar_wait_suspend(fempty + slot, ((g >> 1) & 1) ^ 1, a.status) ? 1 : 0;
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok || abort_flag) { abort_flag = 1; break; }
+#pragma unroll
+        for (int j = 0; j < NT * kFsGroup / 64; ++j) {
+          const int e = j * 64 + ft;
+          factors[slot * kFsGroup * NT + (e % kFsGroup) * NT + e / kFsGroup] = v[j];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ffull + slot);
+      }
+    }
+  } else {
+    const uint32_t tl = tmem + (uint32_t((warp - 4) * 32) << 16);
+    for (int i = 0; i < kbs; ++i) {
+      const int buf = i % kFsBufs, g = i / kFsGroup;
+      int ok = 1;
+      if (lane == 0) {
+        ok = mbar_wait_suspend(tfull + buf, (i / kFsBufs) & 1, a.status) ? 1 : 0;
+        if (ok && !FUSED && i % kFsGroup == 0) ok = mbar_wait_suspend(ffull + (g & 1), (g >> 1) & 1, a.status) ? 1 : 0;
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok || abort_flag) { abort_flag = 1; break; }
+      tmem_fence_after();
+      const float4* f = reinterpret_cast<const float4*>(factors + (FUSED ? i : (g & 1) * kFsGroup + i % kFsGroup) * NT);
+      if (NT == 16) {
+        uint32_t v[16];
+        tmem_ld16(tl + buf * NT, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 fq = f[q];
+          acc[4 * q] = fmaf(__uint_as_float(v[4 * q]), fq.x, acc[4 * q]);
+          acc[4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), fq.y, acc[4 * q + 1]);
+          acc[4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), fq.z, acc[4 * q + 2]);
+          acc[4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), fq.w, acc[4 * q + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NT; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tl + buf * NT + c, v);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 fq = f[c / 4 + q];
+            acc[(c + 4 * q) % NT] = fmaf(__uint_as_float(v[4 * q]), fq.x, acc[(c + 4 * q) % NT]);
+            acc[(c + 4 * q + 1) % NT] = fmaf(__uint_as_float(v[4 * q + 1]), fq.y, acc[(c + 4 * q + 1) % NT]);
+            acc[(c + 4 * q + 2) % NT] = fmaf(__uint_as_float(v[4 * q + 2]), fq.z, acc[(c + 4 * q + 2) % NT]);
+            acc[(c + 4 * q + 3) % NT] = fmaf(__uint_as_float(v[4 * q + 3]), fq.w, acc[(c + 4 * q + 3) % NT]);
+          }
+        }
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(tempty + buf);
+        if (!FUSED && (i % kFsGroup == kFsGroup - 1)) mbar_arrive(fempty + (g & 1));
+      }
+    }
+  }
+  __syncwarp();
+  // ---- join and store: thread = one weight row, one element per row of x -----------------------------------------------
+  const int row = threadIdx.x - 128, col = n0 + row;              // epilogue threads
+  if (splits == 1) {
+    if (warp >= 4 && col < a.n) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+        if (t0 + c < a.m) store_elem(a.out, a.out_ty, size_t(t0 + c) * size_t(a.ldo) + col, acc[c]);
+    }
+  } else {
+    float* part = reinterpret_cast<float*>(ring);                  // [NT][128]: every copy into the ring has been read
+    if (warp >= 4) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) part[c * 128 + row] = acc[c];
+    }
+    cluster_sync();
+    // block `rank` joins every splits-th row of x
+    const int half = threadIdx.x >> 7, r = threadIdx.x & 127;
+    for (int c = int(rank) + half * int(splits); c < NT && t0 + c < a.m; c += 2 * int(splits)) {
+      float v = 0.f;
+      for (uint32_t s = 0; s < splits; ++s) v += ld_cluster_f32(cluster_map(smem_u32(part + c * 128 + r), s));
+      if (n0 + r < a.n) store_elem(a.out, a.out_ty, size_t(t0 + c) * size_t(a.ldo) + n0 + r, v);
+    }
+    cluster_sync();                                                // nobody leaves while its tile is being read
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_free<S::kTmemCols>(tmem);
+}
+
+}  // namespace dmoe
