@@ -210,6 +210,15 @@ def float_type(dtype) -> int | None:
     return _FLOAT_TYPES.get(dtype)
 
 
+def row_stride(t) -> int:
+    """Elements from row to row of a 2D tensor, or -1 when its columns are strided or its rows overlap. A single row has
+    whatever stride; the kernels want at least its length, in steps of 16."""
+    (rows, cols), (ld, unit) = t.shape, t.stride()
+    if rows <= 1:
+        return (cols + 15) // 16 * 16 if unit == 1 or cols <= 1 else -1
+    return ld if (unit == 1 or cols <= 1) and ld >= cols else -1
+
+
 def check(code: int, what: str) -> None:
     if code != 0:
         raise CudaError(f"{what} failed with cudaError {code}")

@@ -5,6 +5,7 @@
 #include "../../include/darask_moe_b200.h"
 #include <cuda_fp8.h>
 #include "fp8_linear_stream.cuh"
+#include "fp8_linear_tile.cuh"
 
 namespace dmoe {
 
@@ -26,15 +27,20 @@ __global__ void __launch_bounds__(256) fp8_linear_quant_kernel(const RowSource s
   reinterpret_cast<uint32_t*>(codes)[w * 32 + lane] = out;
 }
 
-// What a call runs: rows of x per tile, blocks per cluster, whether the rows are quantized inside the product's launch.
-struct LinearPlan { int nt, splits; bool fused; };
+// What a call runs. `fused` (rows quantized in the product's launch) depends on m and k alone, as the workspace does.
+struct LinearPlan { int nt, splits; bool fused, tile; };
+static bool linear_fused(int m, int kb, bool codes) { return !codes && m <= 16 && kb <= 8 * kFsResident; }
 static LinearPlan linear_plan(int m, int n, int kb, bool codes) {
   LinearPlan p;
+  const int sms = sm_count();
+  p.fused = linear_fused(m, kb, codes);
+  // 256 x 256 tiles once they occupy half of the pairs of SMs
+  p.tile = m > 128 && (long long)((n + 255) / 256) * ((m + 255) / 256) * 4 >= sms;
   p.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
   const long long tiles = (long long)((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
   p.splits = 1;
-  while (p.splits < 8 && tiles * p.splits * 2 <= sm_count() && p.splits * 2 <= kb) p.splits *= 2;
-  p.fused = !codes && m <= 16 && (kb + p.splits - 1) / p.splits <= kFsResident;
+  while (p.splits < 8 && p.splits * 2 <= kb && (tiles * p.splits * 2 <= sms || (p.fused && (kb + p.splits - 1) / p.splits > kFsResident)))
+    p.splits *= 2;
   return p;
 }
 
@@ -54,6 +60,32 @@ static cudaError_t launch_stream(const CUtensorMap& mw, const CUtensorMap& mx, c
   return launch_cluster(kernel, dim3(unsigned(tiles) * unsigned(splits)), dim3(kFsThreads), smem, unsigned(splits), st, mw, mx, a);
 }
 
+static cudaError_t launch_tile(const DaraskFp8Linear* d, const FsArgs& s, const uint8_t* xc, unsigned long long cols, unsigned long long pitch,
+                               cudaStream_t st) {
+  CUtensorMap mx, mw, mo;
+  if (!byte_map(&mx, xc, d->m, cols, pitch, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return cudaErrorInvalidValue;
+  if (!byte_map(&mw, d->w, d->n, d->k, d->ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return cudaErrorInvalidValue;
+  const unsigned long long es = row_type_bytes(d->out_ty);
+  // a TMA store writes whole 16-byte pieces: rows that end inside one would lose what lies behind them
+  const bool aligned = reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->ldo * es % 16 == 0 && d->n * es % 16 == 0;
+  FtArgs a = {};
+  a.m = d->m; a.n = d->n; a.kb = s.kb; a.xs = s.xs; a.ld_xs = s.ld_xs; a.ws = s.ws; a.ld_ws = s.ld_ws;
+  a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo; a.status = s.status;
+  a.tma_store = aligned && byte_map(&mo, d->out, d->m, d->n * es, d->ldo * es, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B, unsigned(es));
+  if (!a.tma_store) mo = mx;            // not used
+  a.tiles_m = (d->m + 255) / 256; a.tiles_n = (d->n + 255) / 256;
+  if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffll) return cudaErrorInvalidValue;
+  static bool configured[64] = {};      // the opt-in is per device
+  const int dev = current_device_slot();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(fp8_linear_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFtSmem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch_pdl(fp8_linear_tile_kernel, dim3(unsigned(sm_count() / 2 * 2)), dim3(kFtThreads), size_t(kFtSmem), st, mx, mw, mo, a);
+}
+
 static size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 }  // namespace dmoe
@@ -63,6 +95,7 @@ using namespace dmoe;
 extern "C" size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_ty) {
   if (m < 1 || n < 1 || k < 1 || x_ty == DARASK_E4M3) return 0;
   const size_t kb = (size_t(k) + 127) / 128;
+  if (linear_fused(m, int(kb), false)) return 0;
   return round_up(size_t(m) * kb * 128, 256) + round_up(size_t(m) * kb * 4, 256);
 }
 
@@ -77,8 +110,9 @@ static bool linear_ok(const DaraskFp8Linear* d) {
     return d->x_scales && d->ld_xs >= kb && !d->swiglu && reinterpret_cast<uintptr_t>(d->x) % 16 == 0 && d->ldx % 16 == 0 && d->ldx >= d->k;
   const size_t eb = row_type_bytes(d->x_ty);
   if (!eb || d->x_scales || reinterpret_cast<uintptr_t>(d->x) % eb || d->ldx < (d->swiglu ? 2ll : 1ll) * d->k) return false;
-  return d->workspace && reinterpret_cast<uintptr_t>(d->workspace) % 256 == 0 &&
-         d->workspace_bytes >= darask_fp8_linear_workspace_bytes(d->m, d->n, d->k, d->x_ty);
+  const size_t need = darask_fp8_linear_workspace_bytes(d->m, d->n, d->k, d->x_ty);
+  return need == 0 || (d->workspace && reinterpret_cast<uintptr_t>(d->workspace) % 256 == 0 &&
+         d->workspace_bytes >= need);
 }
 
 extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
@@ -108,6 +142,7 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
     xc = q; pitch = cols = (unsigned long long)kb * 128; a.xs = scales; a.ld_xs = kb;
   }
   CUtensorMap mw, mx;
+  if (p.tile) return launch_tile(d, a, xc, cols, pitch, st);
   if (!byte_map(&mw, d->w, d->n, d->k, d->ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return cudaErrorInvalidValue;
   if (p.fused) mx = mw;                 // not read
   else if (!byte_map(&mx, xc, d->m, cols, pitch, p.nt, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return cudaErrorInvalidValue;

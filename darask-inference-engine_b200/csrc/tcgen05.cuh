@@ -19,15 +19,15 @@ inline TensorMapEncode tensor_map_encode() {
   }();
   return fn;
 }
-// Byte tensor [rows][cols], rows `pitch` bytes apart (16-byte aligned base and pitch), box [box_rows][box_cols]; reads past
+// Tensor [rows][cols] of `es`-byte elements (box and columns given in bytes), rows `pitch` bytes apart (16-byte aligned base and pitch), box [box_rows][box_cols]; reads past
 // the last row or column give zeros.
 inline bool byte_map(CUtensorMap* m, const void* base, unsigned long long rows, unsigned long long cols, unsigned long long pitch,
-                     unsigned box_rows, unsigned box_cols, CUtensorMapSwizzle swizzle) {
+                     unsigned box_rows, unsigned box_cols, CUtensorMapSwizzle swizzle, unsigned es = 1) {
   const TensorMapEncode enc = tensor_map_encode();
   if (!enc) return false;
-  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
-  const cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+  const cuuint64_t dims[2] = {cols / es, rows}, strides[1] = {pitch};
+  const cuuint32_t box[2] = {box_cols / es, box_rows}, estr[2] = {1, 1};
+  return enc(m, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : es == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -75,6 +75,21 @@ DEVI void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr) : "memory");
 }
 
+// 64 columns, complete on return
+#define DMOE_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define DMOE_R16(r, i) DMOE_R4(r, i), DMOE_R4(r, i + 4), DMOE_R4(r, i + 8), DMOE_R4(r, i + 12)
+DEVI void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : DMOE_R16(r, 0), DMOE_R16(r, 16), DMOE_R16(r, 32), DMOE_R16(r, 48)
+      : "r"(taddr) : "memory");
+}
+#undef DMOE_R16
+#undef DMOE_R4
+
 // ---- clusters --------------------------------------------------------------------------------------------------------
 DEVI uint32_t cluster_rank() {
   uint32_t r;
@@ -89,6 +104,9 @@ DEVI uint32_t cluster_map(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
+}
+DEVI void mbar_arrive_cluster(uint32_t addr) {      // barrier anywhere in the cluster, address from cluster_map
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 DEVI float ld_cluster_f32(uint32_t addr) {
   float v;

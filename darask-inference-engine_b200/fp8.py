@@ -46,48 +46,48 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
     [m, >= ceil(k/128)] (``quantize.fp8_act``).  Sums are float32; `out_dtype` (float32, float16, bfloat16) defaults to x's type, or
     bfloat16 for codes.  Rows may be strided; rows of w and of codes start on 16-byte boundaries.  Any m, including 0; k as w has it.
     Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
-    if w.dim() != 2 or w.dtype != torch.uint8 or w_scales.dim() != 2 or w_scales.dtype != torch.float32:
+    if w.dim() != 2 or w.dtype is not torch.uint8 or w_scales.dim() != 2 or w_scales.dtype is not torch.float32:
         raise ValueError("w must be uint8 [n, k] and w_scales float32 [n blocks, k blocks]")
     n, k = w.shape
     kb = (k + 127) // 128
-    if n < 1 or k < 1 or w_scales.shape[0] < (n + 127) // 128 or w_scales.shape[1] < kb:
+    ws_rows, ws_cols = w_scales.shape
+    if n < 1 or k < 1 or ws_rows < (n + 127) // 128 or ws_cols < kb:
         raise ValueError(f"w [{n}, {k}] needs scales [{(n + 127) // 128}, {kb}], got {list(w_scales.shape)}")
-    codes = x.dtype == torch.uint8
+    codes = x.dtype is torch.uint8
     ty = E4M3 if codes else _lib.float_type(x.dtype)
     if ty is None or x.dim() != 2 or x.shape[1] != (2 * k if swiglu else k) or (codes and swiglu):
         raise ValueError(f"x must be uint8 codes or float32 / float16 / bfloat16 rows of {2 * k if swiglu else k} columns")
     m = x.shape[0]
-    if codes != (x_scales is not None) or (codes and (x_scales.dim() != 2 or x_scales.dtype != torch.float32 or x_scales.shape[0] != m or
-                                                      x_scales.shape[1] < kb)):
+    if codes is (x_scales is None) or (codes and (x_scales.dim() != 2 or x_scales.dtype is not torch.float32 or x_scales.shape[0] != m or
+                                                  x_scales.shape[1] < kb)):
         raise ValueError(f"codes come with x_scales float32 [{m}, {kb}], float rows without")
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype or (torch.bfloat16 if codes else x.dtype), device=x.device)
     elif tuple(out.shape) != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be [{m}, {n}]")
     out_ty = _lib.float_type(out.dtype)
-    tensors = [x, w, w_scales, out] + ([x_scales] if codes else [])
-    if out_ty is None or not x.is_cuda or any(t.device != x.device or t.stride(1) != 1 for t in tensors):
-        raise ValueError("tensors must share one CUDA device and have unit column stride, out must be float32, float16 or bfloat16")
-    if w.data_ptr() % 16 or w.stride(0) % 16 or (codes and m and (x.data_ptr() % 16 or x.stride(0) % 16)):
+    dev = x.get_device()
+    ldx, ldw, ldws, ldo, ldxs = _lib.row_stride(x), _lib.row_stride(w), _lib.row_stride(w_scales), _lib.row_stride(out), 0
+    if codes:
+        ldxs = _lib.row_stride(x_scales) if x_scales.get_device() == dev else -1
+    if out_ty is None or dev < 0 or w.get_device() != dev or w_scales.get_device() != dev or out.get_device() != dev or \
+            min(ldx, ldw, ldws, ldo, ldxs) < 0:
+        raise ValueError("tensors must share one CUDA device, with unit column stride and rows that do not overlap; "
+                         "out must be float32, float16 or bfloat16")
+    xp, wp = x.data_ptr(), w.data_ptr()
+    if wp % 16 or ldw % 16 or (codes and m and (xp % 16 or ldx % 16)):
         raise ValueError("rows of w and of codes must start on 16-byte boundaries")
-    if any(t.stride(0) < t.shape[1] for t in tensors if t.shape[0] > 1):
-        raise ValueError("rows must not overlap")
     if m == 0:
         return out
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return linear(x, w, w_scales, x_scales, swiglu, None, out)
     lib = _lib.lib()
-    d = _lib.DaraskFp8Linear()
-    d.m, d.n, d.k, d.swiglu = m, n, k, int(swiglu)
-    d.x, d.x_ty, d.ldx = x.data_ptr(), ty, _row_stride(x)
-    if codes:
-        d.x_scales, d.ld_xs = x_scales.data_ptr(), _row_stride(x_scales)
-    d.w, d.ldw, d.w_scales, d.ld_ws = w.data_ptr(), _row_stride(w), w_scales.data_ptr(), _row_stride(w_scales)
-    d.out, d.out_ty, d.ldo = out.data_ptr(), out_ty, _row_stride(out)
-    with torch.cuda.device(x.device):
-        nbytes = lib.darask_fp8_linear_workspace_bytes(m, n, k, ty)
-        if nbytes:
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            d.workspace, d.workspace_bytes = scratch.data_ptr(), nbytes
-        _lib.check(lib.darask_fp8_linear(ctypes.byref(d), torch.cuda.current_stream(x.device).cuda_stream), "darask_fp8_linear")
+    nbytes = lib.darask_fp8_linear_workspace_bytes(m, n, k, ty)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    d = _lib.DaraskFp8Linear(m, n, k, xp, ty, ldx, x_scales.data_ptr() if codes else None, ldxs, 1 if swiglu else 0, wp, ldw,
+                             w_scales.data_ptr(), ldws, out.data_ptr(), out_ty, ldo, scratch.data_ptr() if nbytes else None, nbytes)
+    _lib.check(lib.darask_fp8_linear(ctypes.byref(d), torch.cuda.current_stream().cuda_stream), "darask_fp8_linear")
     return out
 
 
@@ -98,11 +98,6 @@ def linear_status(device="cuda") -> int:
     with torch.cuda.device(device):
         _lib.check(_lib.lib().darask_fp8_linear_status(ctypes.byref(s), torch.cuda.current_stream(device).cuda_stream), "darask_fp8_linear_status")
     return s.value
-
-
-def _row_stride(t):
-    """Elements from row to row; a single row has whatever stride, the kernels want at least its length."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 class Fp8MoeLayer:

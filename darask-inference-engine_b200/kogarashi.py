@@ -43,7 +43,7 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
         raise ValueError("up must have the type and shape of weight")
     row_bytes = k // 256 * 144 if weight.ty == GGML_Q4_K else q6k_r16_row_bytes(k)
     data = [w.data for w in (weight, up) if w is not None]
-    if any(t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != groups * n * row_bytes or t.data_ptr() % 16 for t in data):
+    if any(t.dtype is not torch.uint8 or not t.is_contiguous() or t.numel() != groups * n * row_bytes or t.data_ptr() % 16 for t in data):
         raise ValueError(f"weight data must be {groups * n * row_bytes} contiguous bytes on a 16-byte boundary")
     ty = _lib.float_type(x.dtype)
     if ty is None or x.dim() != 2 or x.shape[1] != (2 * k if swiglu else k):
@@ -61,27 +61,25 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
     elif tuple(out.shape) != (rows, width) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be [{rows}, {width}]")
     out_ty = _lib.float_type(out.dtype)
-    tensors = [x, ranges, out] + data + ([assignments] if assignments is not None else [])
-    if out_ty is None or not x.is_cuda or any(t.device != x.device for t in tensors):
-        raise ValueError("tensors must share one CUDA device, out must be float32, float16 or bfloat16")
-    if any(t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]) for t in (x, out)):
-        raise ValueError("x and out must have unit column stride and rows that do not overlap")
+    dev = x.get_device()
+    ldx, ldo = _lib.row_stride(x), _lib.row_stride(out)
+    if out_ty is None or dev < 0 or ldx < 0 or ldo < 0 or ranges.get_device() != dev or out.get_device() != dev or \
+            any(t.get_device() != dev for t in data) or (assignments is not None and assignments.get_device() != dev):
+        raise ValueError("tensors must share one CUDA device, x and out have unit column stride and rows that do not overlap; "
+                         "out must be float32, float16 or bfloat16")
     if rows == 0:
         return out
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return grouped_gemm(x, ranges, weight, up, assignments, topk, swiglu, None, out)
     lib = _lib.lib()
-    d = _lib.DaraskGgmlGrouped()
-    d.groups, d.n, d.k, d.rows, d.ranges = groups, n, k, rows, ranges.data_ptr()
-    d.x, d.x_ty, d.ldx, d.x_rows = x.data_ptr(), ty, max(x.stride(0), x.shape[1]), x.shape[0]
-    if assignments is not None:
-        d.assignments = assignments.data_ptr()
-    d.topk, d.swiglu = topk, int(swiglu)
-    d.w, d.w_up, d.w_ty = data[0].data_ptr(), data[1].data_ptr() if up is not None else None, weight.ty
-    d.out, d.out_ty, d.ldo = out.data_ptr(), out_ty, max(out.stride(0), width)
-    with torch.cuda.device(x.device):
-        nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        d.workspace, d.workspace_bytes = scratch.data_ptr(), nbytes
-        _lib.check(lib.darask_ggml_grouped_gemm(ctypes.byref(d), torch.cuda.current_stream(x.device).cuda_stream), "darask_ggml_grouped_gemm")
+    nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    d = _lib.DaraskGgmlGrouped(groups, n, k, rows, ranges.data_ptr(), x.data_ptr(), ty, ldx, x.shape[0],
+                               assignments.data_ptr() if assignments is not None else None, topk, 1 if swiglu else 0,
+                               data[0].data_ptr(), data[1].data_ptr() if up is not None else None, weight.ty,
+                               out.data_ptr(), out_ty, ldo, scratch.data_ptr(), nbytes)
+    _lib.check(lib.darask_ggml_grouped_gemm(ctypes.byref(d), torch.cuda.current_stream().cuda_stream), "darask_ggml_grouped_gemm")
     return out
 
 

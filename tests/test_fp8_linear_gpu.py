@@ -61,7 +61,8 @@ def check(y, xv, xs, w, ws):
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (2, 129, 144), (7, 1000, 272), (16, 256, 4096), (17, 130, 1040),
                                    (33, 384, 640), (64, 96, 2048), (77, 1000, 1552), (128, 128, 128), (129, 257, 384), (300, 512, 256),
-                                   (513, 1100, 912), (1025, 2304, 528), (2048, 2048, 256)])
+                                   (513, 1100, 912), (1025, 2304, 528), (2048, 2048, 256),
+                                   (40, 130, 77), (600, 4100, 205)])
 @pytest.mark.parametrize("x_ty,out_ty", [("bf16", "bf16"), ("f32", "f32"), ("f16", "f16"), ("codes", "f32")])
 def test_product(m, n, k, x_ty, out_ty):
     import darask_inference_engine_b200 as D
@@ -189,3 +190,19 @@ def test_empty_batch():
     import darask_inference_engine_b200 as D
     w, ws = weights(9, 64, 128)
     assert tuple(D.fp8.linear(torch.empty(0, 128, device="cuda"), w, ws).shape) == (0, 64)
+
+
+@pytest.mark.parametrize("out_ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,shift", [(2201, 0), (2201, 1), (2208, 0), (2208, 1)])
+def test_many_rows_into_a_view(out_ty, n, shift):
+    """256 x 256 tiles cut at both edges, into rows that start and end on a 16-byte boundary and into rows that do not."""
+    import darask_inference_engine_b200 as D
+    m, k = 1111, 528
+    w, ws = weights(12, n, k)
+    x = torch.randn(m, k, device="cuda", dtype=torch.bfloat16)
+    pitch = (n + 31) // 16 * 16
+    out = torch.full((m + 1, pitch + shift), -1.5, dtype=TYPES[out_ty], device="cuda")
+    D.fp8.linear(x, w, ws, out=out[:m, shift:shift + n])
+    check(out[:m, shift:shift + n], *quantized(x), w, ws)
+    assert bool((out[m] == -1.5).all()) and bool((out[:, :shift] == -1.5).all()) and bool((out[:, shift + n:] == -1.5).all())
+    assert D.fp8.linear_status() == 0
