@@ -3,109 +3,55 @@
 // Q4_K: w = d sc_b q - dmin m_b (sub-blocks of 32 columns), Q6_K: w = d sc_b (q - 32) (sub-blocks of 16 columns), per block
 // of 256 columns (kogarashi kernels/native.cu:21-41).
 #include "../../include/darask_moe_b200.h"
-#include "row_source.cuh"
-#include "stream_launch.cuh"
+#include "ggml_grouped.cuh"
 
 namespace dmoe {
 
 static __device__ unsigned g_ggml_grouped_status;
 
-struct GgmlArgs {
-  int groups, n, k;
-  long long rows;
-  const unsigned* ranges;
-  RowSource x;
-  long long x_rows;
-  const unsigned* assignments;
-  int topk;
-  const uint8_t* w[2];
-  int w_ty, row_bytes;
-  void* out;
-  int out_ty;
-  long long ldo;
-  unsigned* status;
-};
-
-// column c of a 256-column block at `b` (Q4_K: 144 bytes; Q6_K: the 208 bytes of the device layout, block scale d apart)
-DEVI float q4k_value(const uint8_t* b, int c) {
-  const float d = __half2float(*reinterpret_cast<const __half*>(b)), dm = __half2float(*reinterpret_cast<const __half*>(b + 2));
-  const int s = c >> 5, q = (b[16 + (c >> 6) * 32 + (c & 31)] >> (4 * (s & 1))) & 15;
-  const int sc = s < 4 ? b[4 + s] & 63 : (b[8 + s] & 15) | ((b[s] >> 6) << 4);
-  const int mi = s < 4 ? b[8 + s] & 63 : (b[8 + s] >> 4) | ((b[4 + s] >> 6) << 4);
-  return fmaf(d * sc, float(q), -dm * mi);
-}
-DEVI float q6k_value(const uint8_t* b, float d, int c) {
-  const int h = c >> 7, p = (c >> 5) & 3, l = c & 31;
-  const int q = ((b[h * 64 + (p & 1) * 32 + l] >> (p >> 1) * 4) & 15) | (((b[128 + h * 32 + l] >> (2 * p)) & 3) << 4);
-  return d * float(int(static_cast<int8_t>(b[192 + (c >> 4)])) * (q - 32));
+static int ggml_row_bytes(int ty, int k) {
+  return ty == DARASK_GGML_Q4_K ? k / 256 * 144 : ty == DARASK_GGML_Q6_K ? k / 256 * 208 + (2 * (k / 256) + 15) / 16 * 16 : 0;
 }
 
-// Block (32 weight rows, matrix and group): 32 rows at a time, one 256-column block of both operands in shared memory.
-__global__ void __launch_bounds__(256) ggml_grouped_kernel(const GgmlArgs a) {
-  extern __shared__ float sm[];
-  float(*wt)[257] = reinterpret_cast<float(*)[257]>(sm);
-  float(*xt)[257] = reinterpret_cast<float(*)[257]>(sm + 32 * 257);
-  pdl_wait();
-  pdl_launch();
-  const int j0 = blockIdx.x * 32, g = blockIdx.y, mat = blockIdx.z, nblk = a.k / 256;
-  long long rows = a.ranges[2 * g];
-  const long long first = a.ranges[2 * g + 1];
-  if (first + rows > a.rows) {
-    if (threadIdx.x == 0) atomicOr(a.status, kStatusBadRoute);
-    rows = first < a.rows ? a.rows - first : 0;
+// f16 parts of a row: float32 numbers (the rows themselves, or SwiGLU products of any rows) take two
+static int row_parts(int x_ty, int swiglu) { return x_ty == DARASK_GGML_F32 || swiglu ? 2 : 1; }
+
+struct GroupedWs { __half* planes; __half* sum; float* scale; size_t bytes; };
+static GroupedWs carve(void* base, long long rows, int k, int parts) {
+  GroupedWs w;
+  uint8_t* p = static_cast<uint8_t*>(base);
+  size_t off = 0;
+  auto take = [&](size_t bytes) { uint8_t* q = p ? p + off : nullptr; off = (off + bytes + 255) / 256 * 256; return q; };
+  w.planes = reinterpret_cast<__half*>(take(size_t(parts) * size_t(rows) * k * 2));
+  w.sum = reinterpret_cast<__half*>(take(size_t(rows) * (k / 256) * 32));
+  w.scale = reinterpret_cast<float*>(take(size_t(rows) * 4));
+  w.bytes = off;
+  return w;
+}
+
+template <bool Q6, int NX, int NA>
+static cudaError_t launch_products(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& sum, const GgArgs& a,
+                                   cudaStream_t st) {
+  static_assert(GgShape<Q6, NX>::kSmem <= kSmemBudget, "rings must fit one block");
+  static bool configured[64] = {};      // the opt-in is per device and per kernel
+  const int dev = current_device_slot();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  auto kernel = ggml_grouped_kernel<Q6, NX, NA>;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GgShape<Q6, NX>::kSmem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
   }
-  const uint8_t* w = a.w[mat] + size_t(g) * a.n * a.row_bytes;
-  const int tj = threadIdx.x & 31, ti = threadIdx.x >> 5;
-  for (long long i0 = 0; i0 < rows; i0 += 32) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int b = 0; b < nblk; ++b) {
-      __syncthreads();
-      for (int e = threadIdx.x; e < 32 * 256; e += 256) {
-        const int r = e >> 8, c = e & 255;
-        float v = 0.f;
-        if (j0 + r < a.n) {
-          const uint8_t* row = w + size_t(j0 + r) * a.row_bytes;
-          v = a.w_ty == DARASK_GGML_Q4_K
-                  ? q4k_value(row + b * 144, c)
-                  : q6k_value(row + b * 208, __half2float(*reinterpret_cast<const __half*>(row + nblk * 208 + 2 * b)), c);
-        }
-        wt[r][c] = v;
-      }
-      for (int e = threadIdx.x; e < 32 * 64; e += 256) {
-        const int r = e >> 6, c = (e & 63) * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (i0 + r < rows) {
-          const long long row = a.assignments ? a.assignments[first + i0 + r] / a.topk : first + i0 + r;
-          if (row < a.x_rows) row_source_load4(a.x, row, b * 256 + c, v);
-          else atomicOr(a.status, kStatusBadRoute);
-        }
-        for (int q = 0; q < 4; ++q) xt[r][c + q] = v[q] - v[q] == 0.f ? v[q] : __uint_as_float(0x7fffffffu);   // infinities as NaN
-      }
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float p = 0.f;
-        for (int c = 0; c < 256; ++c) p = fmaf(xt[ti + 8 * q][c], wt[tj][c], p);
-        acc[q] += p;
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (i0 + ti + 8 * q < rows && j0 + tj < a.n)
-        store_elem(a.out, a.out_ty, size_t(first + i0 + ti + 8 * q) * size_t(a.ldo) + size_t(mat) * a.n + j0 + tj, acc[q]);
-  }
+  return launch_pdl(kernel, dim3(sm_count()), dim3(kGgThreads), size_t(GgShape<Q6, NX>::kSmem), st, w0, w1, x, sum, a);
 }
 
 }  // namespace dmoe
 
 using namespace dmoe;
 
-static int ggml_row_bytes(int ty, int k) {
-  return ty == DARASK_GGML_Q4_K ? k / 256 * 144 : ty == DARASK_GGML_Q6_K ? k / 256 * 208 + (2 * (k / 256) + 15) / 16 * 16 : 0;
-}
-
-extern "C" size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int x_ty) {
-  return rows < 1 || k < 1 || !row_type_bytes(x_ty) ? 0 : 256;
+extern "C" size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int x_ty, int swiglu) {
+  if (rows < 1 || k < 256 || k % 256 || !row_type_bytes(x_ty)) return 0;
+  return carve(nullptr, rows, k, row_parts(x_ty, swiglu)).bytes;
 }
 
 static bool grouped_ok(const DaraskGgmlGrouped* d) {
@@ -115,11 +61,13 @@ static bool grouped_ok(const DaraskGgmlGrouped* d) {
   const size_t eb = row_type_bytes(d->x_ty), ob = row_type_bytes(d->out_ty);
   if (!eb || !ob || d->ldx < (d->swiglu ? 2ll : 1ll) * d->k || d->ldo < (d->w_up ? 2ll : 1ll) * d->n) return false;
   if (d->assignments && d->topk < 1) return false;
+  // tiles of 128 rows x 128 columns are counted in 32 bits
+  if ((d->rows / 128 + d->groups) * ((d->n + 127) / 128) * 2 > 0x7fffffffll) return false;
   if (d->rows == 0) return true;
   if (!d->ranges || !d->out || reinterpret_cast<uintptr_t>(d->out) % ob) return false;
   if (d->x_rows > 0 && (!d->x || reinterpret_cast<uintptr_t>(d->x) % eb)) return false;
   return d->workspace && reinterpret_cast<uintptr_t>(d->workspace) % 256 == 0 &&
-         d->workspace_bytes >= darask_ggml_grouped_workspace_bytes(d->rows, d->k, d->x_ty);
+         d->workspace_bytes >= darask_ggml_grouped_workspace_bytes(d->rows, d->k, d->x_ty, d->swiglu);
 }
 
 extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t st) {
@@ -128,16 +76,31 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   void* status = nullptr;
   cudaError_t e = cudaGetSymbolAddress(&status, g_ggml_grouped_status);
   if (e) return e;
-  GgmlArgs a = {};
-  a.groups = d->groups; a.n = d->n; a.k = d->k; a.rows = d->rows; a.ranges = d->ranges;
-  a.x = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
-  a.x_rows = d->x_rows; a.assignments = d->assignments; a.topk = d->topk;
+  const bool q6 = d->w_ty == DARASK_GGML_Q6_K;
+  const int parts = row_parts(d->x_ty, d->swiglu), row_bytes = ggml_row_bytes(d->w_ty, d->k), nblk = d->k / 256;
+  // a bf16 result keeps 8 bits: one f16 part (11 bits) of float32 rows is enough in front of it
+  const int nx = d->out_ty == DARASK_GGML_BF16 ? 1 : parts, na = q6 && d->out_ty == DARASK_GGML_F32 ? 2 : 1;
+  const GroupedWs ws = carve(d->workspace, d->rows, d->k, parts);
+  GgRowsArgs r = {};
+  r.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
+  r.rows = d->rows; r.x_rows = d->x_rows; r.assignments = d->assignments; r.topk = d->topk; r.parts = nx; r.sums = !q6;
+  r.planes = ws.planes; r.sum = ws.sum; r.scale = ws.scale;
+  CUtensorMap w0, w1, x, sum;
+  const unsigned long long wrows = (unsigned long long)d->groups * d->n;
+  const unsigned box = q6 ? 208 : 144;
+  if (!byte_map(&w0, d->w, wrows, (unsigned long long)nblk * box, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !byte_map(&w1, d->w_up ? d->w_up : d->w, wrows, (unsigned long long)nblk * box, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !byte_map(&x, ws.planes, (unsigned long long)nx * d->rows, d->k * 2ull, d->k * 2ull, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !byte_map(&sum, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B))
+    return cudaErrorInvalidValue;
+  if ((e = launch_pdl(ggml_rows_kernel, dim3(unsigned(d->rows)), dim3(kGgRowThreads), 0, st, r))) return e;
+  GgArgs a = {};
+  a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);
-  a.w_ty = d->w_ty; a.row_bytes = ggml_row_bytes(d->w_ty, d->k);
-  a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo; a.status = static_cast<unsigned*>(status);
-  const size_t smem = 2 * 32 * 257 * 4;
-  if ((e = cudaFuncSetAttribute(ggml_grouped_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)))) return e;
-  return launch_pdl(ggml_grouped_kernel, dim3((d->n + 31) / 32, d->groups, d->w_up ? 2 : 1), dim3(256), smem, st, a);
+  a.xscale = ws.scale; a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo; a.status = static_cast<unsigned*>(status);
+  if (!q6) return nx == 2 ? launch_products<false, 2, 1>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1>(w0, w1, x, sum, a, st);
+  if (nx == 2) return na == 2 ? launch_products<true, 2, 2>(w0, w1, x, sum, a, st) : launch_products<true, 2, 1>(w0, w1, x, sum, a, st);
+  return na == 2 ? launch_products<true, 1, 2>(w0, w1, x, sum, a, st) : launch_products<true, 1, 1>(w0, w1, x, sum, a, st);
 }
 
 extern "C" int darask_ggml_grouped_status(unsigned* host_status, cudaStream_t st) {

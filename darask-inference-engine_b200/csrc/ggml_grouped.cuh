@@ -1,0 +1,506 @@
+// Product grouped by expert over GGUF Q4_K / Q6_K weights on the 5th-generation tensor cores:
+//   out[i][j] = x[row(i)] . W_g[j]      for the dispatch rows i of every group g
+// A block of 256 weights is d times integers, sc_b q (Q4_K, at most 945) or sc_b (q - 32) (Q6_K, at most 4096), less dmin
+// times integers m_b that multiply the sums of x over 32 columns (Q4_K). The tensor cores multiply these integers: f16 holds
+// Q4_K's exactly (11 significant bits) and Q6_K's to 2^-12 (a second f16 term holds the rest where the output is float32), so
+// a weight is never rounded and has no range to lose. d and dmin are applied in float32 once per 256 columns, when the partial
+// product leaves TMEM. A row of x is divided by a power of two (largest value into [2^9, 2^10)) and split into one or two f16
+// parts (float32: 22 bits); the power of two comes back in the store.
+//
+// One block computes 128 weight rows x up to 128 dispatch rows of one group; the weight rows are the M operand, so that few
+// rows cost a narrow tile (N a multiple of 16). The weight operand is written straight into TMEM (tcgen05.st), where
+// tcgen05.mma reads it: it costs shared memory neither space nor bandwidth.
+//   warp 0        TMA: packed weight rows (128 x 144 or 208 bytes) per 256 columns, rows of x per 64 columns, their sums
+//   warp 1        tcgen05.mma kind::f16; per 256 columns one accumulator buffer of two
+//   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 64 columns at a time in four slots
+//   warps 12-15   promotion (thread = one weight row): acc += d * main - dmin * min, and the store at the end of a tile
+// TMEM: two main buffers of 128 columns, 128 columns for Q4_K's min products or Q6_K's second terms, 128 for the slots.
+// Persistent: tiles are dealt out in steps of the grid, the row tiles of a group's weight tile next to each other.
+#pragma once
+#include "row_source.cuh"
+#include "tcgen05.cuh"
+
+namespace dmoe {
+
+constexpr int kGgThreads = 512;
+constexpr int kGgMaxGroups = 1024;
+constexpr int kGgChunkBytes = 128 * 128;                 // 128 rows x 64 columns of f16
+constexpr int kGgSumBytes = 128 * 32;                    // 128 rows x 16 f16: the sums of eight groups of 32 columns, twice
+
+struct GgArgs {
+  const unsigned* ranges;                                // [groups][2]
+  int groups, n, nblk, mats, row_bytes;
+  long long rows;
+  const uint8_t* w[2];                                   // Q6_K: the block scales d are read from here
+  const float* xscale;                                   // [rows] powers of two; negative: row(i) does not exist
+  void* out;
+  int out_ty;
+  long long ldo;
+  unsigned* status;
+};
+
+template <bool Q6, int NX>
+struct GgShape {
+  static constexpr int kRawBytes = Q6 ? 208 : 144;
+  static constexpr int kRawStage = 128 * kRawBytes;
+  static constexpr int kRawStages = 3;
+  static constexpr int kXStage = NX * kGgChunkBytes;
+  static constexpr int kXStages = NX == 1 ? 6 : 3;
+  static constexpr int kOffX = 0;                        // 1024-byte aligned tiles first
+  static constexpr int kOffSum = kOffX + kXStages * kXStage;
+  static constexpr int kOffMin = kOffSum + (Q6 ? 0 : 2 * kGgSumBytes);
+  static constexpr int kOffRaw = kOffMin + (Q6 ? 0 : 2 * kGgSumBytes);
+  static constexpr int kOffD = kOffRaw + kRawStages * kRawStage;
+  static constexpr int kOffEnds = kOffD + 4 * 128 * 8;
+  static constexpr int kSmem = 1024 + kOffEnds + (kGgMaxGroups + 1) * 4;
+};
+
+// ---- rows of x -> f16 parts --------------------------------------------------------------------------------------------
+// One block per dispatch row: largest magnitude, then x * 2^-e as one or two f16 parts, four columns at a time in the order
+// 0 2 1 3 in which the expanders leave the weights, and (Q4_K) the sums of 32 columns as f16 high and low parts.
+struct GgRowsArgs {
+  RowSource src;
+  long long rows, x_rows;
+  const unsigned* assignments;
+  int topk, parts, sums;
+  __half* planes;                                        // [parts][rows][k]
+  __half* sum;                                           // [rows][k / 256][16]: 8 high, 8 low
+  float* scale;                                          // [rows]
+};
+constexpr int kGgRowThreads = 256;
+__global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsArgs a) {
+  __shared__ uint32_t red[kGgRowThreads / 32];
+  pdl_wait();
+  pdl_launch();
+  const long long i = blockIdx.x;
+  const int k = a.src.k;
+  long long row = i;
+  if (a.assignments) row = __ldg(a.assignments + i) / unsigned(a.topk);
+  const bool exists = row < a.x_rows;
+  uint32_t top = 0;
+  if (exists)
+    for (int c = threadIdx.x * 4; c < k; c += kGgRowThreads * 4) {
+      float v[4];
+      row_source_load4(a.src, row, c, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
+    }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kGgRowThreads / 32; ++q) top = max(top, red[q]);
+  // exponent of the largest magnitude (not below 2^-117: the factor stays finite), moved to 2^9
+  const bool finite = top < 0x7f800000u;
+  const int e = max(int(top >> 23) - 127, -117) - 9;
+  const float down = __uint_as_float(uint32_t(127 - e) << 23);
+  if (threadIdx.x == 0)
+    a.scale[i] = !exists ? -1.f : top == 0u ? 1.f : finite ? __uint_as_float(uint32_t(127 + e) << 23) : __uint_as_float(0x7fffffffu);
+  const bool live = exists && finite;
+  for (int c = threadIdx.x * 4; c < k; c += kGgRowThreads * 4) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) row_source_load4(a.src, row, c, v);
+    __half hi[4];
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[q] *= down;
+      hi[q] = __float2half_rn(v[q]);
+      s += v[q];
+    }
+    auto put = [&](__half* p, const __half (&h)[4]) {
+      const __half2 w0 = __halves2half2(h[0], h[2]), w1 = __halves2half2(h[1], h[3]);
+      *reinterpret_cast<uint2*>(p + size_t(i) * k + c) = make_uint2(*reinterpret_cast<const uint32_t*>(&w0), *reinterpret_cast<const uint32_t*>(&w1));
+    };
+    put(a.planes, hi);
+    if (a.parts > 1) {
+      __half lo[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) lo[q] = __float2half_rn(v[q] - __half2float(hi[q]));
+      put(a.planes + size_t(a.rows) * k, lo);
+    }
+    if (a.sums) {                                        // k is a multiple of 256: whole warps are here
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if ((threadIdx.x & 7) == 0) {
+        const __half h = __float2half_rn(s);
+        __half* p = a.sum + (size_t(i) * (k / 256) + c / 256) * 16 + (c % 256) / 32;
+        p[0] = h;
+        p[8] = __float2half_rn(s - __half2float(h));
+      }
+    }
+  }
+}
+
+// ---- expanders ---------------------------------------------------------------------------------------------------------
+DEVI __half2 as_half2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+DEVI uint32_t as_word(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// byte `i` of w as an integer in both halves (1024 + byte is exact in f16, so is the difference)
+template <int I>
+DEVI __half2 byte_half2(uint32_t w, float offset) {
+  return __hsub2(as_half2(__byte_perm(w, 0x64006400u, 0x5050 + 0x0101 * I)), __float2half2_rn(offset));
+}
+DEVI void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
+DEVI uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// d = a (TMEM) x b (shared memory) in f16, float32 accumulation
+DEVI void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+DEVI void umma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// K-major operand tile, rows of 32 bytes, 32-byte swizzle, 8-row groups 256 bytes apart
+DEVI uint64_t umma_desc_k32(uint32_t smem_addr) {
+  return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(256 >> 4) << 32) | (1ull << 46) | (6ull << 61);
+}
+
+struct GgTile { int group, n0, mat, rows; long long first; };      // rows of the tile, its first dispatch row
+
+// NX: f16 parts of a row of x; NA: f16 terms of a Q6_K integer
+template <bool Q6, int NX, int NA>
+__global__ void __launch_bounds__(kGgThreads, 1)
+ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
+                    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_sum, const GgArgs a) {
+  using S = GgShape<Q6, NX>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
+  int* ends = reinterpret_cast<int*>(smem + S::kOffEnds);                   // [groups + 1] cumulative tile counts
+  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], xfull[S::kXStages], xempty[S::kXStages], afull[4], aempty[4], sfull[2],
+      sempty[2], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < S::kRawStages; ++s) { mbar_init(wfull + s, 1); mbar_init(wempty + s, 8); }
+    for (int s = 0; s < S::kXStages; ++s) { mbar_init(xfull + s, 1); mbar_init(xempty + s, 1); }
+    for (int s = 0; s < 4; ++s) { mbar_init(afull + s, 4); mbar_init(aempty + s, 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(sfull + s, 5); mbar_init(sempty + s, 1); mbar_init(tfull + s, 1); mbar_init(tempty + s, 4); }
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc<512>(&tmem_slot);
+  pdl_wait();
+  pdl_launch();
+  // rows of a group that lie inside [0, a.rows)
+  auto group_rows = [&](int g, long long* first) {
+    const unsigned r = __ldcg(a.ranges + 2 * g), o = __ldcg(a.ranges + 2 * g + 1);
+    *first = o;
+    return (long long)o + r <= a.rows ? int(r) : o < a.rows ? int(a.rows - o) : 0;
+  };
+  const int tiles_n = (a.n + 127) / 128 * a.mats;
+  for (int g = threadIdx.x; g < a.groups; g += kGgThreads) {
+    long long first;
+    const int r = group_rows(g, &first);
+    if (unsigned(r) != __ldcg(a.ranges + 2 * g) && blockIdx.x == 0) atomicOr(a.status, kStatusBadRoute);
+    ends[g] = (r + 127) / 128 * tiles_n;
+  }
+  __syncthreads();
+  if (warp == 0) {                       // inclusive scan, consecutive groups per lane
+    const int per = (a.groups + 31) / 32;
+    int sum = 0;
+    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) sum += ends[g]; }
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += t; }
+    int off = run - sum;
+    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) { off += ends[g]; ends[g] = off; } }
+    if (lane == 31) ends[a.groups] = run;
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot, tmem_min = tmem + 256, tmem_a = tmem + 384;      // Q6_K: second terms at tmem_min
+  const int total = ends[a.groups];
+  auto locate = [&](int tile) {
+    int lo = 0, hi = a.groups;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (tile < ends[mid]) hi = mid; else lo = mid + 1; }
+    const int local = tile - (lo ? ends[lo - 1] : 0);
+    GgTile t;
+    t.group = lo;
+    const int r = group_rows(lo, &t.first);
+    // row tiles of equal height, a multiple of 16
+    const int tiles_m = (r + 127) / 128, h = ((r + tiles_m - 1) / tiles_m + 15) / 16 * 16;
+    const int m = local % tiles_m, nt = local / tiles_m;
+    t.first += m * h;
+    t.rows = r - m * h < h ? r - m * h : h;
+    t.n0 = nt / a.mats * 128;
+    t.mat = nt % a.mats;
+    return t;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0) {
+      // ---- TMA ---------------------------------------------------------------------------------------------------------
+      int wi = 0, xi = 0;                // 256-column and 64-column steps so far
+      for (int tile = blockIdx.x; tile < total && !abort_flag; tile += gridDim.x) {
+        const GgTile t = locate(tile);
+        const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
+        const int wrow = t.group * a.n + t.n0, boxes = (t.rows + 31) / 32;
+        for (int b = 0; b < a.nblk && !abort_flag; ++b, ++wi) {
+          const int ws = wi % S::kRawStages;
+          if (wi >= S::kRawStages && !mbar_wait_suspend(wempty + ws, ((wi / S::kRawStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+          mbar_arrive_expect_tx(wfull + ws, S::kRawStage);
+          tma_load_2d(smem_u32(smem + S::kOffRaw + ws * S::kRawStage), mw, b * S::kRawBytes, wrow, wfull + ws);
+          if (!Q6) {
+            const int ss = wi & 1;
+            if (wi >= 2 && !mbar_wait_suspend(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+            mbar_arrive_expect_tx(sfull + ss, boxes * 32 * 32);
+            for (int q = 0; q < boxes; ++q)
+              tma_load_2d(smem_u32(smem + S::kOffSum + ss * kGgSumBytes + q * 32 * 32), &map_sum, b * 32, int(t.first) + 32 * q, sfull + ss);
+          }
+          for (int c = 0; c < 4; ++c, ++xi) {
+            const int xs = xi % S::kXStages;
+            if (xi >= S::kXStages && !mbar_wait_suspend(xempty + xs, ((xi / S::kXStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+            mbar_arrive_expect_tx(xfull + xs, NX * boxes * 32 * 128);
+            const uint32_t dst = smem_u32(smem + S::kOffX + xs * S::kXStage);
+            for (int q = 0; q < boxes; ++q) {
+              tma_load_2d(dst + q * 32 * 128, &map_x, (b * 4 + c) * 128, int(t.first) + 32 * q, xfull + xs);
+              if (NX == 2) tma_load_2d(dst + kGgChunkBytes + q * 32 * 128, &map_x, (b * 4 + c) * 128, int(a.rows + t.first) + 32 * q, xfull + xs);
+            }
+          }
+        }
+      }
+      if (abort_flag) {                  // after a timeout the copies in flight land before the block ends
+        for (int i = wi > S::kRawStages ? wi - S::kRawStages : 0; i < wi; ++i) mbar_wait_suspend(wfull + i % S::kRawStages, (i / S::kRawStages) & 1, a.status);
+        for (int i = xi > S::kXStages ? xi - S::kXStages : 0; i < xi; ++i) mbar_wait_suspend(xfull + i % S::kXStages, (i / S::kXStages) & 1, a.status);
+      }
+    } else if (warp == 1 && lane == 0) {
+      // ---- MMA ---------------------------------------------------------------------------------------------------------
+      int wi = 0, xi = 0;
+      for (int tile = blockIdx.x; tile < total && !abort_flag; tile += gridDim.x) {
+        const GgTile t = locate(tile);
+        const uint32_t idesc = (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24);
+        for (int b = 0; b < a.nblk && !abort_flag; ++b, ++wi) {
+          const int buf = wi & 1;
+          if (wi >= 2 && !mbar_wait_suspend(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+          for (int c = 0; c < 4; ++c, ++xi) {
+            const int xs = xi % S::kXStages, as = xi & 3;
+            if (!mbar_wait_suspend(xfull + xs, (xi / S::kXStages) & 1, a.status) || !mbar_wait_suspend(afull + as, (xi >> 2) & 1, a.status)) {
+              abort_flag = 1;
+              break;
+            }
+            tmem_fence_after();
+            const uint32_t x = smem_u32(smem + S::kOffX + xs * S::kXStage), d = tmem + buf * 128;
+            const uint64_t dx = umma_desc_k128(x), dl = umma_desc_k128(x + kGgChunkBytes);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              umma_f16_ts(d, tmem_a + as * 32 + q * 8, dx + 2 * q, idesc, (c | q) ? 1u : 0u);
+              if (NX == 2) umma_f16_ts(d, tmem_a + as * 32 + q * 8, dl + 2 * q, idesc, 1u);
+              if (NA == 2) umma_f16_ts(d, tmem_min + as * 32 + q * 8, dx + 2 * q, idesc, 1u);
+            }
+            umma_commit(xempty + xs);
+            umma_commit(aempty + as);
+          }
+          if (abort_flag) break;
+          if (!Q6) {
+            // sums times mins: one step of 16; its accumulator is free once the block of 256 columns before has been promoted
+            const int ss = wi & 1;
+            if (wi >= 1 && !mbar_wait_suspend(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status)) { abort_flag = 1; break; }
+            if (!mbar_wait_suspend(sfull + ss, (wi >> 1) & 1, a.status)) { abort_flag = 1; break; }
+            tmem_fence_after();
+            umma_f16_ss(tmem_min, umma_desc_k32(smem_u32(smem + S::kOffMin + ss * kGgSumBytes)),
+                        umma_desc_k32(smem_u32(smem + S::kOffSum + ss * kGgSumBytes)), idesc, 0u);
+            umma_commit(sempty + ss);
+          }
+          umma_commit(tfull + buf);
+        }
+      }
+    }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    // ---- expanders: warps 4-7 the first 128 columns of a block, warps 8-11 the others --------------------------------------
+    const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tl = uint32_t((warp & 3) * 32) << 16;
+    int wi = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+      const GgTile t = locate(tile);
+      const __half* dq = nullptr;        // Q6_K: the row's block scales
+      float d_next = 0.f;
+      if (Q6 && set == 0) {
+        const int r = t.n0 + row < a.n ? t.n0 + row : a.n - 1;
+        dq = reinterpret_cast<const __half*>(a.w[t.mat] + (size_t(t.group) * a.n + r) * a.row_bytes + size_t(a.nblk) * 208);
+        d_next = __half2float(__ldg(dq));
+      }
+      for (int b = 0; b < a.nblk; ++b, ++wi) {
+        const int ws = wi % S::kRawStages;
+        const float d_now = d_next;
+        if (Q6 && set == 0 && b + 1 < a.nblk) d_next = __half2float(__ldg(dq + b + 1));
+        if (!warp_wait(wfull + ws, (wi / S::kRawStages) & 1, a.status)) { ok = false; break; }
+        const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
+        uint4 head;                      // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
+        head = lds128(raw + (Q6 ? 192 : 0));
+        uint32_t sc4 = 0;                // Q4_K: four scales of this set's columns
+        if (!Q6) sc4 = set == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const int c = set * 2 + cc, xi = wi * 4 + c;               // 64-column step of the slot
+          // all shared-memory reads of the step, then the wait for the slot
+          uint4 lw[4], hw[2];
+          if (!Q6) {
+            lw[0] = lds128(raw + 16 + c * 32);
+            lw[1] = lds128(raw + 16 + c * 32 + 16);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) lw[q] = lds128(raw + set * 64 + q * 16);
+            hw[0] = lds128(raw + 128 + set * 32);
+            hw[1] = lds128(raw + 128 + set * 32 + 16);
+          }
+          if (xi >= 4 && !warp_wait(aempty + c, ((xi >> 2) & 1) ^ 1, a.status)) { ok = false; break; }
+          tmem_fence_after();
+          if (cc == 0 && set == 0) {
+            if (Q6) dring[(wi & 3) * 128 + row] = make_float2(d_now, 0.f);
+            else {
+              const __half2 dd = as_half2(head.x);
+              dring[(wi & 3) * 128 + row] = make_float2(__low2float(dd), __high2float(dd));
+              // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
+              const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
+              auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
+              const uint4 m = make_uint4(pair(m0, 0x4140), pair(m0, 0x4342), pair(m1, 0x4140), pair(m1, 0x4342));
+              const int ss = wi & 1;
+              if (wi >= 2 && !warp_wait(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
+              uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + ss * kGgSumBytes + row * 32);
+              p[0] = m;
+              p[1] = m;
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(sfull + ss);
+            }
+          }
+          const uint32_t dst = tl + c * 32;             // slot of the step
+          if (!Q6) {
+            // low nibbles: columns 0-31 of the step, high nibbles: 32-63; (1024 + q) sc - 1024 sc, every term exact
+            const __half2 s0 = cc == 0 ? byte_half2<0>(sc4, 1024.f) : byte_half2<2>(sc4, 1024.f);
+            const __half2 s1 = cc == 0 ? byte_half2<1>(sc4, 1024.f) : byte_half2<3>(sc4, 1024.f);
+            const __half2 k0 = __hmul2(s0, __float2half2_rn(-1024.f)), s1d = __hmul2(s1, __float2half2_rn(0.0625f)), k1 = __hmul2(s1, __float2half2_rn(-64.f));
+            uint32_t lo[16], hi[16];
+            const uint32_t wd[8] = {lw[0].x, lw[0].y, lw[0].z, lw[0].w, lw[1].x, lw[1].y, lw[1].z, lw[1].w};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const uint32_t w = wd[q], u = w >> 8;
+              lo[2 * q] = as_word(__hfma2(as_half2((w & 0x000f000fu) | 0x64006400u), s0, k0));
+              lo[2 * q + 1] = as_word(__hfma2(as_half2((u & 0x000f000fu) | 0x64006400u), s0, k0));
+              hi[2 * q] = as_word(__hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), s1d, k1));
+              hi[2 * q + 1] = as_word(__hfma2(as_half2((u & 0x00f000f0u) | 0x64006400u), s1d, k1));
+            }
+            tmem_st16(tmem_a + dst, lo);
+            tmem_st16(tmem_a + dst + 16, hi);
+          } else {
+            const uint32_t scw = set == 0 ? (cc == 0 ? head.x : head.y) : (cc == 0 ? head.z : head.w);
+            const uint32_t scu = scw ^ 0x80808080u;
+            const uint32_t hq[8] = {hw[0].x, hw[0].y, hw[0].z, hw[0].w, hw[1].x, hw[1].y, hw[1].z, hw[1].w};
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {       // 32 columns: the first or the second 32 bytes of ql
+              const uint4 l0 = lw[2 * part], l1 = lw[2 * part + 1];
+              const uint32_t wd[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
+              const __half2 sa = part == 0 ? byte_half2<0>(scu, 1152.f) : byte_half2<2>(scu, 1152.f);
+              const __half2 sb = part == 0 ? byte_half2<1>(scu, 1152.f) : byte_half2<3>(scu, 1152.f);
+              uint32_t v[16], r[16];
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const __half2 sc = q < 4 ? sa : sb;
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {            // even and odd bytes
+                  const uint32_t w = o ? wd[q] >> 8 : wd[q], h = o ? hq[q] >> 8 : hq[q];
+                  __half2 z;                             // q - 32
+                  if (cc == 0) {
+                    const uint32_t top = (part ? h << 2 : h << 4) & 0x00300030u;
+                    z = __hsub2(as_half2((w & 0x000f000fu) | top | 0x64006400u), __float2half2_rn(1056.f));
+                  } else {
+                    const uint32_t top = (part ? h << 2 : h << 4) & 0x03000300u;
+                    z = __hfma2(as_half2((w & 0x00f000f0u) | top | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-96.f));
+                  }
+                  const __half2 p = __hmul2(z, sc);
+                  v[2 * q + o] = as_word(p);
+                  if (NA == 2) r[2 * q + o] = as_word(__hfma2(z, sc, __hneg2(p)));
+                }
+              }
+              tmem_st16(tmem_a + dst + part * 16, v);
+              if (NA == 2) tmem_st16(tmem_min + dst + part * 16, r);
+            }
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(afull + c);
+        }
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(wempty + ws);
+      }
+    }
+    if (!ok) abort_flag = 1;
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    // ---- promotion and store ---------------------------------------------------------------------------------------------
+    const int row = (warp - 12) * 32 + lane;
+    const uint32_t tl = uint32_t((warp - 12) * 32) << 16;
+    int wi = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+      const GgTile t = locate(tile);
+      float acc[128];
+#pragma unroll
+      for (int c = 0; c < 128; ++c) acc[c] = 0.f;
+      for (int b = 0; b < a.nblk; ++b, ++wi) {
+        const int buf = wi & 1;
+        if (!warp_wait(tfull + buf, (wi >> 1) & 1, a.status)) { ok = false; break; }
+        tmem_fence_after();
+        const float2 d = dring[(wi & 3) * 128 + row];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          if (c < t.rows) {
+            uint32_t v[32];
+            tmem_ld32(tmem + tl + buf * 128 + c, v);
+#pragma unroll
+            for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(d.x, __uint_as_float(v[q]), acc[c + q]);
+            if (!Q6) {
+              tmem_ld32(tmem_min + tl + c, v);
+#pragma unroll
+              for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(-d.y, __uint_as_float(v[q]), acc[c + q]);
+            }
+          }
+        }
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty + buf);
+      }
+      if (!ok) break;
+      const int col = t.n0 + row;
+      const bool in = col < a.n;
+      const size_t at = size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+#pragma unroll
+      for (int c = 0; c < 128; ++c) {
+        if (c < t.rows) {
+          const float s = __ldg(a.xscale + t.first + c);
+          if (s < 0.f && row == 0) atomicOr(a.status, kStatusBadRoute);
+          if (in) store_elem(a.out, a.out_ty, at + size_t(c) * size_t(a.ldo), acc[c] * fabsf(s));
+        }
+      }
+    }
+    if (!ok) abort_flag = 1;
+  }
+  __syncwarp();
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 1) tmem_free<512>(tmem);
+}
+
+}  // namespace dmoe

@@ -53,10 +53,9 @@ inline cudaError_t launch_cluster(Kernel kernel, dim3 grid, dim3 block, size_t s
 
 // ---- TMEM ------------------------------------------------------------------------------------------------------------
 template <int COLS>
-DEVI uint32_t tmem_alloc(uint32_t* slot) {      // one whole warp
+DEVI void tmem_alloc(uint32_t* slot) {      // one whole warp
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(uint32_t(COLS)) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  return 0;
 }
 template <int COLS>
 DEVI void tmem_free(uint32_t base) {            // the warp that allocated
@@ -89,6 +88,15 @@ DEVI void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
 }
 #undef DMOE_R16
 #undef DMOE_R4
+
+// A whole warp waits: one lane watches the barrier (32 probes of one word serialise in shared memory).
+DEVI bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait_suspend(bar, parity, status) ? 1 : 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
+}
 
 // ---- clusters --------------------------------------------------------------------------------------------------------
 DEVI uint32_t cluster_rank() {

@@ -73,7 +73,7 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
         with torch.cuda.device(dev):
             return grouped_gemm(x, ranges, weight, up, assignments, topk, swiglu, None, out)
     lib = _lib.lib()
-    nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty)
+    nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty, 1 if swiglu else 0)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     d = _lib.DaraskGgmlGrouped(groups, n, k, rows, ranges.data_ptr(), x.data_ptr(), ty, ldx, x.shape[0],
                                assignments.data_ptr() if assignments is not None else None, topk, 1 if swiglu else 0,

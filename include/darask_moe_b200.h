@@ -422,7 +422,7 @@ int darask_fp8_linear_status(unsigned* host_status /* host */, darask_stream_t s
  * parts (22 bits), f16 and bf16 rows as they are, with one power of two per row taken out first.  An infinity or a NaN in a row
  * makes the row's outputs NaN.  A range that leaves [0, rows) is cut and a row(i) >= x_rows reads as zeros; both set
  * DARASK_STATUS_BAD_ROUTE in the device's status word (darask_ggml_grouped_status, as darask_fp8_linear_status).
- * workspace: darask_ggml_grouped_workspace_bytes(rows, k, x_ty) bytes, 256-byte aligned, as for darask_fp8_linear. */
+ * workspace: darask_ggml_grouped_workspace_bytes(rows, k, x_ty, swiglu) bytes, 256-byte aligned, as for darask_fp8_linear. */
 typedef struct {
   int groups, n, k;
   long long rows;
@@ -434,7 +434,7 @@ typedef struct {
   void* out; int out_ty; long long ldo;
   void* workspace; size_t workspace_bytes;
 } DaraskGgmlGrouped;
-size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int x_ty);
+size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int x_ty, int swiglu);
 int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* desc /* host */, darask_stream_t stream);
 int darask_ggml_grouped_status(unsigned* host_status /* host */, darask_stream_t stream);
 

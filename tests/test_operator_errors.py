@@ -28,7 +28,7 @@ def grouped(**kw):
     d.groups, d.n, d.k, d.rows, d.ranges = 4, 200, 512, 30, FAKE
     d.x, d.x_ty, d.ldx, d.x_rows, d.topk = FAKE, 0, 512, 30, 1
     d.w, d.w_ty, d.out, d.out_ty, d.ldo = FAKE, 12, FAKE, 0, 200
-    d.workspace, d.workspace_bytes = FAKE, D._lib.lib().darask_ggml_grouped_workspace_bytes(30, 512, 0)
+    d.workspace, d.workspace_bytes = FAKE, D._lib.lib().darask_ggml_grouped_workspace_bytes(30, 512, 0, 0)
     for k, v in kw.items():
         setattr(d, k, v)
     return d
