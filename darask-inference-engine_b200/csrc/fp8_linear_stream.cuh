@@ -148,19 +148,19 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
     if (lane == 0) {
       int issued = FUSED ? (kbs < kStages ? kbs : kStages) : 0;
       for (int i = issued; i < kbs && !abort_flag; ++i, ++issued) {
-        if (i >= kStages && !mbar_wait_suspend(empty + i % kStages, ((i / kStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+        if (i >= kStages && !pipe_wait(empty + i % kStages, ((i / kStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
         load_stage(i);
       }
       // after a timeout the copies in flight land before the block ends
       if (abort_flag)
-        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_wait_suspend(full + i % kStages, (i / kStages) & 1, a.status);
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) pipe_wait(full + i % kStages, (i / kStages) & 1, a.status);
     }
   } else if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < kbs && !abort_flag; ++i) {
         const int s = i % kStages, buf = i % kFsBufs;
-        if (i >= kFsBufs && !mbar_wait_suspend(tempty + buf, ((i / kFsBufs) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-        if (!mbar_wait_suspend(full + s, (i / kStages) & 1, a.status)) { abort_flag = 1; break; }
+        if (i >= kFsBufs && !pipe_wait(tempty + buf, ((i / kFsBufs) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+        if (!pipe_wait(full + s, (i / kStages) & 1, a.status)) { abort_flag = 1; break; }
         tmem_fence_after();
         const uint32_t sw = smem_u32(ring + s * kStageBytes);
         const uint64_t dw = umma_desc_k128(sw), dx = umma_desc_k128(FUSED ? smem_u32(xres + size_t(i) * 2048) : sw + 128 * 128);
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
           v[j] = t0 + row < a.m && b < kbs ? __ldg(a.xs + size_t(t0 + row) * size_t(a.ld_xs) + kb0 + b) * __ldg(ws + b) : 0.f;
         }
         int ok = 1;
-        if (g >= 2 && lane == 0) ok = mbar_wait_suspend(fempty + slot, ((g >> 1) & 1) ^ 1, a.status) ? 1 : 0;
+        if (g >= 2 && lane == 0) ok = pipe_wait(fempty + slot, ((g >> 1) & 1) ^ 1, a.status) ? 1 : 0;
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok || abort_flag) { abort_flag = 1; break; }
 #pragma unroll
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
       const int buf = i % kFsBufs, g = i / kFsGroup;
       int ok = 1;
       if (lane == 0) {
-        ok = mbar_wait_suspend(tfull + buf, (i / kFsBufs) & 1, a.status) ? 1 : 0;
-        if (ok && !FUSED && i % kFsGroup == 0) ok = mbar_wait_suspend(ffull + (g & 1), (g >> 1) & 1, a.status) ? 1 : 0;
+        ok = pipe_wait(tfull + buf, (i / kFsBufs) & 1, a.status) ? 1 : 0;
+        if (ok && !FUSED && i % kFsGroup == 0) ok = pipe_wait(ffull + (g & 1), (g >> 1) & 1, a.status) ? 1 : 0;
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok || abort_flag) { abort_flag = 1; break; }

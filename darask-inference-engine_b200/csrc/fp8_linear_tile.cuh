@@ -90,7 +90,7 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         const int r0 = (tile % a.tiles_m) * 256 + int(rank) * 128, w0 = (tile / a.tiles_m) * 256 + int(rank) * 128;
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
           const int s = it % kFtStages;
-          if (it >= kFtStages && !mbar_wait_suspend(empty + s, ((it / kFtStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+          if (it >= kFtStages && !pipe_wait(empty + s, ((it / kFtStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
           const uint32_t dst = smem_u32(ring + s * kFtStageBytes), bar = cluster_map(smem_u32(full + s), 0);
           if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * kFtStageBytes);
           tma_load_pair(dst, &map_x, kb * 128, r0, bar);
@@ -99,15 +99,15 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       }
       // after a timeout the copies in flight land before the pair ends
       if (abort_flag && rank == 0)
-        for (int i = it > kFtStages ? it - kFtStages : 0; i < it; ++i) mbar_wait_suspend(full + i % kFtStages, (i / kFtStages) & 1, a.status);
+        for (int i = it > kFtStages ? it - kFtStages : 0; i < it; ++i) pipe_wait(full + i % kFtStages, (i / kFtStages) & 1, a.status);
     } else if (warp == 1 && lane == 0 && rank == 0) {
       constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(256 >> 3) << 17) | (uint32_t(256 >> 4) << 24);
       int it = 0;
       for (int tile = first; tile < total && !abort_flag; tile += step) {
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
           const int s = it % kFtStages, buf = it & 1;
-          if (it >= 2 && !mbar_wait_suspend(tempty + buf, ((it >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-          if (!mbar_wait_suspend(full + s, (it / kFtStages) & 1, a.status)) { abort_flag = 1; break; }
+          if (it >= 2 && !pipe_wait(tempty + buf, ((it >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
+          if (!pipe_wait(full + s, (it / kFtStages) & 1, a.status)) { abort_flag = 1; break; }
           tmem_fence_after();
           const uint32_t sx = smem_u32(ring + s * kFtStageBytes);
           const uint64_t dx = umma_desc_k128(sx), dw = umma_desc_k128(sx + 128 * 128);
@@ -138,7 +138,7 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
           if (ft < 2 * kFtGroup && (nb + (ft & 1)) * 128 < a.n && b0 + ft / 2 < a.kb)
             w = __ldg(a.ws + size_t(nb + (ft & 1)) * size_t(a.ld_ws) + b0 + ft / 2);
           int ok = 1;
-          if (fg >= 2 && lane == 0) ok = mbar_wait_suspend(fempty + slot, ((fg >> 1) & 1) ^ 1, a.status) ? 1 : 0;
+          if (fg >= 2 && lane == 0) ok = pipe_wait(fempty + slot, ((fg >> 1) & 1) ^ 1, a.status) ? 1 : 0;
           ok = __shfl_sync(0xffffffffu, ok, 0);
           if (!ok) abort_flag = 1;
           if (abort_flag) break;
@@ -166,8 +166,8 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         const int buf = it & 1, slot = fg & 1;
         int got = 1;
         if (lane == 0) {
-          if (kb % kFtGroup == 0) got = mbar_wait_suspend(ffull + slot, (fg >> 1) & 1, a.status) ? 1 : 0;
-          if (got) got = mbar_wait_suspend(tfull + buf, (it >> 1) & 1, a.status) ? 1 : 0;
+          if (kb % kFtGroup == 0) got = pipe_wait(ffull + slot, (fg >> 1) & 1, a.status) ? 1 : 0;
+          if (got) got = pipe_wait(tfull + buf, (it >> 1) & 1, a.status) ? 1 : 0;
         }
         got = __shfl_sync(0xffffffffu, got, 0);
         if (!got) { abort_flag = 1; ok = false; break; }

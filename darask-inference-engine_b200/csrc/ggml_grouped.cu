@@ -29,14 +29,14 @@ static GroupedWs carve(void* base, long long rows, int k, int parts) {
   return w;
 }
 
-template <bool Q6, int NX, int NA>
+template <bool Q6, int NX, int NA, typename OUT>
 static cudaError_t launch_products(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& sum, const GgArgs& a,
                                    cudaStream_t st) {
   static_assert(GgShape<Q6, NX>::kSmem <= kSmemBudget, "rings must fit one block");
   static bool configured[64] = {};      // the opt-in is per device and per kernel
   const int dev = current_device_slot();
   if (dev < 0) return cudaErrorInvalidDevice;
-  auto kernel = ggml_grouped_kernel<Q6, NX, NA>;
+  auto kernel = ggml_grouped_kernel<Q6, NX, NA, OUT>;
   if (!configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GgShape<Q6, NX>::kSmem);
     if (e != cudaSuccess) return e;
@@ -79,7 +79,7 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   const bool q6 = d->w_ty == DARASK_GGML_Q6_K;
   const int parts = row_parts(d->x_ty, d->swiglu), row_bytes = ggml_row_bytes(d->w_ty, d->k), nblk = d->k / 256;
   // a bf16 result keeps 8 bits: one f16 part (11 bits) of float32 rows is enough in front of it
-  const int nx = d->out_ty == DARASK_GGML_BF16 ? 1 : parts, na = q6 && d->out_ty == DARASK_GGML_F32 ? 2 : 1;
+  const int nx = d->out_ty == DARASK_GGML_BF16 ? 1 : parts;
   const GroupedWs ws = carve(d->workspace, d->rows, d->k, parts);
   GgRowsArgs r = {};
   r.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
@@ -97,10 +97,18 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   GgArgs a = {};
   a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);
-  a.xscale = ws.scale; a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo; a.status = static_cast<unsigned*>(status);
-  if (!q6) return nx == 2 ? launch_products<false, 2, 1>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1>(w0, w1, x, sum, a, st);
-  if (nx == 2) return na == 2 ? launch_products<true, 2, 2>(w0, w1, x, sum, a, st) : launch_products<true, 2, 1>(w0, w1, x, sum, a, st);
-  return na == 2 ? launch_products<true, 1, 2>(w0, w1, x, sum, a, st) : launch_products<true, 1, 1>(w0, w1, x, sum, a, st);
+  a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo; a.status = static_cast<unsigned*>(status);
+  // f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
+  switch (d->out_ty) {
+    case DARASK_GGML_F32:
+      if (q6) return nx == 2 ? launch_products<true, 2, 2, float>(w0, w1, x, sum, a, st) : launch_products<true, 1, 2, float>(w0, w1, x, sum, a, st);
+      return nx == 2 ? launch_products<false, 2, 1, float>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1, float>(w0, w1, x, sum, a, st);
+    case DARASK_GGML_F16:
+      if (q6) return nx == 2 ? launch_products<true, 2, 1, __half>(w0, w1, x, sum, a, st) : launch_products<true, 1, 1, __half>(w0, w1, x, sum, a, st);
+      return nx == 2 ? launch_products<false, 2, 1, __half>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1, __half>(w0, w1, x, sum, a, st);
+    default:
+      return q6 ? launch_products<true, 1, 1, __nv_bfloat16>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1, __nv_bfloat16>(w0, w1, x, sum, a, st);
+  }
 }
 
 extern "C" int darask_ggml_grouped_status(unsigned* host_status, cudaStream_t st) {

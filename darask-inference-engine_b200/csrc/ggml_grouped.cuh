@@ -10,9 +10,9 @@
 // One block computes 128 weight rows x up to 128 dispatch rows of one group; the weight rows are the M operand, so that few
 // rows cost a narrow tile (N a multiple of 16). The weight operand is written straight into TMEM (tcgen05.st), where
 // tcgen05.mma reads it: it costs shared memory neither space nor bandwidth.
-//   warp 0        TMA: packed weight rows (128 x 144 or 208 bytes) per 256 columns, rows of x per 64 columns, their sums
+//   warp 0        TMA: packed weight rows (128 x 144 or 208 bytes) per 256 columns, rows of x per 128 columns, their sums
 //   warp 1        tcgen05.mma kind::f16; per 256 columns one accumulator buffer of two
-//   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 64 columns at a time in four slots
+//   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 128 columns of k per slot
 //   warps 12-15   promotion (thread = one weight row): acc += d * main - dmin * min, and the store at the end of a tile
 // TMEM: two main buffers of 128 columns, 128 columns for Q4_K's min products or Q6_K's second terms, 128 for the slots.
 // Persistent: tiles are dealt out in steps of the grid, the row tiles of a group's weight tile next to each other.
@@ -24,7 +24,8 @@ namespace dmoe {
 
 constexpr int kGgThreads = 512;
 constexpr int kGgMaxGroups = 1024;
-constexpr int kGgChunkBytes = 128 * 128;                 // 128 rows x 64 columns of f16
+constexpr int kGgBoxBytes = 128 * 128;                   // 128 rows x 64 columns of f16
+constexpr int kGgStepBytes = 2 * kGgBoxBytes;            // a step: 128 columns of k
 constexpr int kGgSumBytes = 128 * 32;                    // 128 rows x 16 f16: the sums of eight groups of 32 columns, twice
 
 struct GgArgs {
@@ -34,7 +35,6 @@ struct GgArgs {
   const uint8_t* w[2];                                   // Q6_K: the block scales d are read from here
   const float* xscale;                                   // [rows] powers of two; negative: row(i) does not exist
   void* out;
-  int out_ty;
   long long ldo;
   unsigned* status;
 };
@@ -44,8 +44,8 @@ struct GgShape {
   static constexpr int kRawBytes = Q6 ? 208 : 144;
   static constexpr int kRawStage = 128 * kRawBytes;
   static constexpr int kRawStages = 3;
-  static constexpr int kXStage = NX * kGgChunkBytes;
-  static constexpr int kXStages = NX == 1 ? 6 : 3;
+  static constexpr int kXStage = NX * kGgStepBytes;
+  static constexpr int kXStages = NX == 1 ? 3 : 2;
   static constexpr int kOffX = 0;                        // 1024-byte aligned tiles first
   static constexpr int kOffSum = kOffX + kXStages * kXStage;
   static constexpr int kOffMin = kOffSum + (Q6 ? 0 : 2 * kGgSumBytes);
@@ -151,18 +151,23 @@ DEVI uint4 lds128(uint32_t addr) {
   return v;
 }
 
-// d = a (TMEM) x b (shared memory) in f16, float32 accumulation
-DEVI void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+// d = a (TMEM) x b (shared memory) in f16, float32 accumulation; issued by the lane with `go` set
+DEVI void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t go) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %5, 0;\n\t"
+      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
 }
-DEVI void umma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+DEVI void umma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t go) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %5, 0;\n\t"
+      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
+}
+DEVI void umma_commit_if(uint64_t* bar, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %1, 0;\n\t"
+      "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(go) : "memory");
 }
 // K-major operand tile, rows of 32 bytes, 32-byte swizzle, 8-row groups 256 bytes apart
 DEVI uint64_t umma_desc_k32(uint32_t smem_addr) {
@@ -172,7 +177,12 @@ DEVI uint64_t umma_desc_k32(uint32_t smem_addr) {
 struct GgTile { int group, n0, mat, rows; long long first; };      // rows of the tile, its first dispatch row
 
 // NX: f16 parts of a row of x; NA: f16 terms of a Q6_K integer
-template <bool Q6, int NX, int NA>
+template <typename T> DEVI T from_float(float v);
+template <> DEVI float from_float<float>(float v) { return v; }
+template <> DEVI __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> DEVI __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <bool Q6, int NX, int NA, typename OUT>
 __global__ void __launch_bounds__(kGgThreads, 1)
 ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_sum, const GgArgs a) {
@@ -181,17 +191,17 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
   int* ends = reinterpret_cast<int*>(smem + S::kOffEnds);                   // [groups + 1] cumulative tile counts
-  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], xfull[S::kXStages], xempty[S::kXStages], afull[4], aempty[4], sfull[2],
+  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], xfull[S::kXStages], xempty[S::kXStages], afull[2], aempty[2], sfull[2],
       sempty[2], tfull[2], tempty[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float xsc[4][128];
   __shared__ volatile int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < S::kRawStages; ++s) { mbar_init(wfull + s, 1); mbar_init(wempty + s, 8); }
     for (int s = 0; s < S::kXStages; ++s) { mbar_init(xfull + s, 1); mbar_init(xempty + s, 1); }
-    for (int s = 0; s < 4; ++s) { mbar_init(afull + s, 4); mbar_init(aempty + s, 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(sfull + s, 5); mbar_init(sempty + s, 1); mbar_init(tfull + s, 1); mbar_init(tempty + s, 4); }
+    for (int s = 0; s < 2; ++s) { mbar_init(afull + s, 4); mbar_init(aempty + s, 1); mbar_init(sfull + s, 5); mbar_init(sempty + s, 1); mbar_init(tfull + s, 1); mbar_init(tempty + s, 4); }
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc<512>(&tmem_slot);
@@ -246,82 +256,106 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       // ---- TMA ---------------------------------------------------------------------------------------------------------
-      int wi = 0, xi = 0;                // 256-column and 64-column steps so far
-      for (int tile = blockIdx.x; tile < total && !abort_flag; tile += gridDim.x) {
+      const uint32_t go = elect_lane();
+      int wi = 0, xi = 0;                // 256-column and 128-column steps so far
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
         const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
-        const int wrow = t.group * a.n + t.n0, boxes = (t.rows + 31) / 32;
-        for (int b = 0; b < a.nblk && !abort_flag; ++b, ++wi) {
-          const int ws = wi % S::kRawStages;
-          if (wi >= S::kRawStages && !mbar_wait_suspend(wempty + ws, ((wi / S::kRawStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-          mbar_arrive_expect_tx(wfull + ws, S::kRawStage);
-          tma_load_2d(smem_u32(smem + S::kOffRaw + ws * S::kRawStage), mw, b * S::kRawBytes, wrow, wfull + ws);
-          if (!Q6) {
-            const int ss = wi & 1;
-            if (wi >= 2 && !mbar_wait_suspend(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-            mbar_arrive_expect_tx(sfull + ss, boxes * 32 * 32);
-            for (int q = 0; q < boxes; ++q)
-              tma_load_2d(smem_u32(smem + S::kOffSum + ss * kGgSumBytes + q * 32 * 32), &map_sum, b * 32, int(t.first) + 32 * q, sfull + ss);
+        const int wrow = t.group * a.n + t.n0, boxes = (t.rows + 31) / 32, first = int(t.first);
+#pragma unroll 1
+        for (int b = 0; b < a.nblk; ++b, ++wi) {
+          const int ws = wi % S::kRawStages, ss = wi & 1;
+          if (wi >= S::kRawStages) ok = uniform_wait(wempty + ws, ((wi / S::kRawStages) & 1) ^ 1, a.status);
+          if (!ok) break;
+          if (go) {
+            mbar_arrive_expect_tx(wfull + ws, S::kRawStage);
+            tma_load_2d(smem_u32(smem + S::kOffRaw + ws * S::kRawStage), mw, b * S::kRawBytes, wrow, wfull + ws);
           }
-          for (int c = 0; c < 4; ++c, ++xi) {
-            const int xs = xi % S::kXStages;
-            if (xi >= S::kXStages && !mbar_wait_suspend(xempty + xs, ((xi / S::kXStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-            mbar_arrive_expect_tx(xfull + xs, NX * boxes * 32 * 128);
-            const uint32_t dst = smem_u32(smem + S::kOffX + xs * S::kXStage);
-            for (int q = 0; q < boxes; ++q) {
-              tma_load_2d(dst + q * 32 * 128, &map_x, (b * 4 + c) * 128, int(t.first) + 32 * q, xfull + xs);
-              if (NX == 2) tma_load_2d(dst + kGgChunkBytes + q * 32 * 128, &map_x, (b * 4 + c) * 128, int(a.rows + t.first) + 32 * q, xfull + xs);
+          if (!Q6) {
+            if (wi >= 2) ok = uniform_wait(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status);
+            if (!ok) break;
+            if (go) {
+              mbar_arrive_expect_tx(sfull + ss, boxes * 32 * 32);
+#pragma unroll 1
+              for (int q = 0; q < boxes; ++q)
+                tma_load_2d(smem_u32(smem + S::kOffSum + ss * kGgSumBytes + q * 32 * 32), &map_sum, b * 32, first + 32 * q, sfull + ss);
             }
           }
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c, ++xi) {
+            const int xs = xi % S::kXStages;
+            if (xi >= S::kXStages) ok = uniform_wait(xempty + xs, ((xi / S::kXStages) & 1) ^ 1, a.status);
+            if (!ok) break;
+            if (go) {
+              const uint32_t dst = smem_u32(smem + S::kOffX + xs * S::kXStage);
+              const int col = (b * 2 + c) * 256;
+              mbar_arrive_expect_tx(xfull + xs, NX * boxes * 2 * 32 * 128);
+#pragma unroll 1
+              for (int q = 0; q < boxes; ++q)
+#pragma unroll 1
+                for (int p = 0; p < 2 * NX; ++p)             // 64 columns of a part each
+                  tma_load_2d(dst + p * kGgBoxBytes + q * 32 * 128, &map_x, col + (p & 1) * 128, (p >> 1) * int(a.rows) + first + 32 * q, xfull + xs);
+            }
+          }
+          if (!ok) break;
         }
       }
-      if (abort_flag) {                  // after a timeout the copies in flight land before the block ends
-        for (int i = wi > S::kRawStages ? wi - S::kRawStages : 0; i < wi; ++i) mbar_wait_suspend(wfull + i % S::kRawStages, (i / S::kRawStages) & 1, a.status);
-        for (int i = xi > S::kXStages ? xi - S::kXStages : 0; i < xi; ++i) mbar_wait_suspend(xfull + i % S::kXStages, (i / S::kXStages) & 1, a.status);
+      if (!ok) {                         // after a timeout the copies in flight land before the block ends
+        abort_flag = 1;
+        for (int i = wi > S::kRawStages ? wi - S::kRawStages : 0; i < wi; ++i) pipe_wait(wfull + i % S::kRawStages, (i / S::kRawStages) & 1, a.status);
+        for (int i = xi > S::kXStages ? xi - S::kXStages : 0; i < xi; ++i) pipe_wait(xfull + i % S::kXStages, (i / S::kXStages) & 1, a.status);
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---- MMA ---------------------------------------------------------------------------------------------------------
+      const uint32_t go = elect_lane();
       int wi = 0, xi = 0;
-      for (int tile = blockIdx.x; tile < total && !abort_flag; tile += gridDim.x) {
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
-        const uint32_t idesc = (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24);
-        for (int b = 0; b < a.nblk && !abort_flag; ++b, ++wi) {
+        const uint32_t idesc = __shfl_sync(0xffffffffu, (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24), 0);
+#pragma unroll 1
+        for (int b = 0; b < a.nblk; ++b, ++wi) {
           const int buf = wi & 1;
-          if (wi >= 2 && !mbar_wait_suspend(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-          for (int c = 0; c < 4; ++c, ++xi) {
-            const int xs = xi % S::kXStages, as = xi & 3;
-            if (!mbar_wait_suspend(xfull + xs, (xi / S::kXStages) & 1, a.status) || !mbar_wait_suspend(afull + as, (xi >> 2) & 1, a.status)) {
-              abort_flag = 1;
-              break;
-            }
+          const uint32_t d = tmem + buf * 128;
+          if (wi >= 2) ok = uniform_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+          if (!ok) break;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c, ++xi) {
+            const int xs = xi % S::kXStages;
+            ok = uniform_wait(xfull + xs, (xi / S::kXStages) & 1, a.status) && uniform_wait(afull + c, wi & 1, a.status);
+            if (!ok) break;
             tmem_fence_after();
-            const uint32_t x = smem_u32(smem + S::kOffX + xs * S::kXStage), d = tmem + buf * 128;
-            const uint64_t dx = umma_desc_k128(x), dl = umma_desc_k128(x + kGgChunkBytes);
+            const uint64_t dx = umma_desc_k128(smem_u32(smem + S::kOffX + xs * S::kXStage));
+            const uint32_t at = tmem_a + c * 64, am = tmem_min + c * 64;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              umma_f16_ts(d, tmem_a + as * 32 + q * 8, dx + 2 * q, idesc, (c | q) ? 1u : 0u);
-              if (NX == 2) umma_f16_ts(d, tmem_a + as * 32 + q * 8, dl + 2 * q, idesc, 1u);
-              if (NA == 2) umma_f16_ts(d, tmem_min + as * 32 + q * 8, dx + 2 * q, idesc, 1u);
+            for (int q = 0; q < 8; ++q) {
+              const uint64_t box = (q >> 2) * (kGgBoxBytes >> 4) + 2 * (q & 3);      // 16 columns of k, in units of 16 bytes
+              umma_f16_ts(d, at + q * 8, dx + box, idesc, q ? 1u : uint32_t(c), go);
+              if (NX == 2) umma_f16_ts(d, at + q * 8, dx + (kGgStepBytes >> 4) + box, idesc, 1u, go);
+              if (NA == 2) umma_f16_ts(d, am + q * 8, dx + box, idesc, 1u, go);
             }
-            umma_commit(xempty + xs);
-            umma_commit(aempty + as);
+            umma_commit_if(xempty + xs, go);
+            umma_commit_if(aempty + c, go);
           }
-          if (abort_flag) break;
+          if (!ok) break;
           if (!Q6) {
             // sums times mins: one step of 16; its accumulator is free once the block of 256 columns before has been promoted
             const int ss = wi & 1;
-            if (wi >= 1 && !mbar_wait_suspend(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status)) { abort_flag = 1; break; }
-            if (!mbar_wait_suspend(sfull + ss, (wi >> 1) & 1, a.status)) { abort_flag = 1; break; }
+            if (wi >= 1) ok = uniform_wait(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status);
+            if (ok) ok = uniform_wait(sfull + ss, (wi >> 1) & 1, a.status);
+            if (!ok) break;
             tmem_fence_after();
             umma_f16_ss(tmem_min, umma_desc_k32(smem_u32(smem + S::kOffMin + ss * kGgSumBytes)),
-                        umma_desc_k32(smem_u32(smem + S::kOffSum + ss * kGgSumBytes)), idesc, 0u);
-            umma_commit(sempty + ss);
+                        umma_desc_k32(smem_u32(smem + S::kOffSum + ss * kGgSumBytes)), idesc, 0u, go);
+            umma_commit_if(sempty + ss, go);
           }
-          umma_commit(tfull + buf);
+          umma_commit_if(tfull + buf, go);
         }
       }
+      if (!ok) abort_flag = 1;
     }
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
@@ -347,51 +381,48 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
         uint4 head;                      // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
         head = lds128(raw + (Q6 ? 192 : 0));
-        uint32_t sc4 = 0;                // Q4_K: four scales of this set's columns
-        if (!Q6) sc4 = set == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const int c = set * 2 + cc, xi = wi * 4 + c;               // 64-column step of the slot
-          // all shared-memory reads of the step, then the wait for the slot
-          uint4 lw[4], hw[2];
+        uint32_t scales = 0;             // Q4_K: four scales of this set's columns
+        if (!Q6) scales = set == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
+        if (wi >= 1 && !warp_wait(aempty + set, (wi & 1) ^ 1, a.status)) { ok = false; break; }
+        tmem_fence_after();
+        if (set == 0) {
+          if (Q6) dring[(wi & 3) * 128 + row] = make_float2(d_now, 0.f);
+          else {
+            const __half2 dd = as_half2(head.x);
+            dring[(wi & 3) * 128 + row] = make_float2(__low2float(dd), __high2float(dd));
+            // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
+            const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
+            auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
+            const uint4 m = make_uint4(pair(m0, 0x4140), pair(m0, 0x4342), pair(m1, 0x4140), pair(m1, 0x4342));
+            const int ss = wi & 1;
+            if (wi >= 2 && !warp_wait(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
+            uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + ss * kGgSumBytes + row * 32);
+            p[0] = m;
+            p[1] = m;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfull + ss);
+          }
+        }
+#pragma unroll 1
+        for (int cc = 0; cc < 2; ++cc) {                  // 64 columns
+          const int c = set * 2 + cc;
+          uint4 w0, w1, h0, h1;
           if (!Q6) {
-            lw[0] = lds128(raw + 16 + c * 32);
-            lw[1] = lds128(raw + 16 + c * 32 + 16);
+            w0 = lds128(raw + 16 + c * 32);
+            w1 = lds128(raw + 16 + c * 32 + 16);
           } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) lw[q] = lds128(raw + set * 64 + q * 16);
-            hw[0] = lds128(raw + 128 + set * 32);
-            hw[1] = lds128(raw + 128 + set * 32 + 16);
+            h0 = lds128(raw + 128 + set * 32);
+            h1 = lds128(raw + 128 + set * 32 + 16);
           }
-          if (xi >= 4 && !warp_wait(aempty + c, ((xi >> 2) & 1) ^ 1, a.status)) { ok = false; break; }
-          tmem_fence_after();
-          if (cc == 0 && set == 0) {
-            if (Q6) dring[(wi & 3) * 128 + row] = make_float2(d_now, 0.f);
-            else {
-              const __half2 dd = as_half2(head.x);
-              dring[(wi & 3) * 128 + row] = make_float2(__low2float(dd), __high2float(dd));
-              // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
-              const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
-              auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
-              const uint4 m = make_uint4(pair(m0, 0x4140), pair(m0, 0x4342), pair(m1, 0x4140), pair(m1, 0x4342));
-              const int ss = wi & 1;
-              if (wi >= 2 && !warp_wait(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
-              uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + ss * kGgSumBytes + row * 32);
-              p[0] = m;
-              p[1] = m;
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) mbar_arrive(sfull + ss);
-            }
-          }
-          const uint32_t dst = tl + c * 32;             // slot of the step
+          const uint32_t dst = tl + c * 32;
+          const uint32_t scw = scales >> (16 * cc);     // Q4_K: two scales of 32 columns
           if (!Q6) {
             // low nibbles: columns 0-31 of the step, high nibbles: 32-63; (1024 + q) sc - 1024 sc, every term exact
-            const __half2 s0 = cc == 0 ? byte_half2<0>(sc4, 1024.f) : byte_half2<2>(sc4, 1024.f);
-            const __half2 s1 = cc == 0 ? byte_half2<1>(sc4, 1024.f) : byte_half2<3>(sc4, 1024.f);
+            const __half2 s0 = byte_half2<0>(scw, 1024.f), s1 = byte_half2<1>(scw, 1024.f);
             const __half2 k0 = __hmul2(s0, __float2half2_rn(-1024.f)), s1d = __hmul2(s1, __float2half2_rn(0.0625f)), k1 = __hmul2(s1, __float2half2_rn(-64.f));
             uint32_t lo[16], hi[16];
-            const uint32_t wd[8] = {lw[0].x, lw[0].y, lw[0].z, lw[0].w, lw[1].x, lw[1].y, lw[1].z, lw[1].w};
+            const uint32_t wd[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const uint32_t w = wd[q], u = w >> 8;
@@ -403,30 +434,24 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             tmem_st16(tmem_a + dst, lo);
             tmem_st16(tmem_a + dst + 16, hi);
           } else {
-            const uint32_t scw = set == 0 ? (cc == 0 ? head.x : head.y) : (cc == 0 ? head.z : head.w);
-            const uint32_t scu = scw ^ 0x80808080u;
-            const uint32_t hq[8] = {hw[0].x, hw[0].y, hw[0].z, hw[0].w, hw[1].x, hw[1].y, hw[1].z, hw[1].w};
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {       // 32 columns: the first or the second 32 bytes of ql
-              const uint4 l0 = lw[2 * part], l1 = lw[2 * part + 1];
+            uint32_t sc4 = (set == 0 ? (cc == 0 ? head.x : head.y) : (cc == 0 ? head.z : head.w)) ^ 0x80808080u;
+            const int down = 4 * cc;                     // the second step of a half block has the high nibbles and the upper bit pairs
+            const uint32_t hq[8] = {h0.x >> down, h0.y >> down, h0.z >> down, h0.w >> down, h1.x >> down, h1.y >> down, h1.z >> down, h1.w >> down};
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part, sc4 >>= 16) {       // 32 columns: the first or the second 32 bytes of ql
+              const uint4 l0 = lds128(raw + set * 64 + part * 32), l1 = lds128(raw + set * 64 + part * 32 + 16);
               const uint32_t wd[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
-              const __half2 sa = part == 0 ? byte_half2<0>(scu, 1152.f) : byte_half2<2>(scu, 1152.f);
-              const __half2 sb = part == 0 ? byte_half2<1>(scu, 1152.f) : byte_half2<3>(scu, 1152.f);
+              const __half2 sa = byte_half2<0>(sc4, 1152.f), sb = byte_half2<1>(sc4, 1152.f);
+              const int up = 4 - 2 * part;
               uint32_t v[16], r[16];
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 const __half2 sc = q < 4 ? sa : sb;
+                const uint32_t w = wd[q] >> down, h = hq[q] << up;
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {            // even and odd bytes
-                  const uint32_t w = o ? wd[q] >> 8 : wd[q], h = o ? hq[q] >> 8 : hq[q];
-                  __half2 z;                             // q - 32
-                  if (cc == 0) {
-                    const uint32_t top = (part ? h << 2 : h << 4) & 0x00300030u;
-                    z = __hsub2(as_half2((w & 0x000f000fu) | top | 0x64006400u), __float2half2_rn(1056.f));
-                  } else {
-                    const uint32_t top = (part ? h << 2 : h << 4) & 0x03000300u;
-                    z = __hfma2(as_half2((w & 0x00f000f0u) | top | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-96.f));
-                  }
+                  const __half2 z = __hsub2(as_half2(((o ? w >> 8 : w) & 0x000f000fu) | ((o ? h >> 8 : h) & 0x00300030u) | 0x64006400u),
+                                            __float2half2_rn(1056.f));                    // q - 32
                   const __half2 p = __hmul2(z, sc);
                   v[2 * q + o] = as_word(p);
                   if (NA == 2) r[2 * q + o] = as_word(__hfma2(z, sc, __hneg2(p)));
@@ -436,13 +461,14 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
               if (NA == 2) tmem_st16(tmem_min + dst + part * 16, r);
             }
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          tmem_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(afull + c);
         }
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(wempty + ws);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(afull + set);
+          mbar_arrive(wempty + ws);
+        }
       }
     }
     if (!ok) abort_flag = 1;
@@ -482,15 +508,27 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (lane == 0) mbar_arrive(tempty + buf);
       }
       if (!ok) break;
-      const int col = t.n0 + row;
-      const bool in = col < a.n;
-      const size_t at = size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+      // scales of the tile's rows to shared memory, then one store per element: a warp writes 32 neighbours of an output row
+      float* mine = xsc[warp - 12];
+      __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 128; ++c) {
+      for (int q = 0; q < 4; ++q) {
+        const int r = q * 32 + lane;
+        const float s = r < t.rows ? __ldg(a.xscale + t.first + r) : 0.f;
+        if (s < 0.f && warp == 12) atomicOr(a.status, kStatusBadRoute);
+        mine[r] = fabsf(s);
+      }
+      __syncwarp();
+      const int col = t.n0 + row;
+      OUT* p = static_cast<OUT*>(a.out) + size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+#pragma unroll
+      for (int c = 0; c < 128; c += 16) {
         if (c < t.rows) {
-          const float s = __ldg(a.xscale + t.first + c);
-          if (s < 0.f && row == 0) atomicOr(a.status, kStatusBadRoute);
-          if (in) store_elem(a.out, a.out_ty, at + size_t(c) * size_t(a.ldo), acc[c] * fabsf(s));
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            if (c + q < t.rows && col < a.n) *p = from_float<OUT>(acc[c + q] * mine[c + q]);
+            p += a.ldo;
+          }
         }
       }
     }

@@ -89,10 +89,37 @@ DEVI void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
 #undef DMOE_R16
 #undef DMOE_R4
 
+// Bounded wait for a phase, a handful of instructions (the roles of these kernels run side by side and fight for the
+// instruction cache). A probe suspends the thread for up to 2 us; a million of them end the wait and set the status bit.
+DEVI bool pipe_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
+  const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
+  for (uint32_t i = 0; i < 1000000u; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(2000u)
+        : "memory");
+    if (ok) return true;
+  }
+  atomicOr(status, kStatusWaitTimeout);
+  return false;
+}
+// The same for a warp whose lanes stay together, so that its loop stays on the uniform datapath (the operands of tcgen05.mma
+// and of the tensor copies live in uniform registers; a loop of one lane moves every one of them there anew).
+DEVI bool uniform_wait(uint64_t* bar, uint32_t parity, unsigned* status) { return __all_sync(0xffffffffu, pipe_wait(bar, parity, status)); }
+DEVI uint32_t elect_lane() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
+}
 // A whole warp waits: one lane watches the barrier (32 probes of one word serialise in shared memory).
 DEVI bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
   int ok = 1;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait_suspend(bar, parity, status) ? 1 : 0;
+  if ((threadIdx.x & 31) == 0) ok = pipe_wait(bar, parity, status) ? 1 : 0;
   ok = __shfl_sync(0xffffffffu, ok, 0);
   __syncwarp();
   return ok != 0;
