@@ -30,8 +30,7 @@ static GroupedWs carve(void* base, long long rows, int k, int parts) {
 }
 
 template <bool Q6, int NX, int NA, typename OUT>
-static cudaError_t launch_products(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& sum, const GgArgs& a,
-                                   cudaStream_t st) {
+static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
   static_assert(GgShape<Q6, NX>::kSmem <= kSmemBudget, "rings must fit one block");
   static bool configured[64] = {};      // the opt-in is per device and per kernel
   const int dev = current_device_slot();
@@ -42,7 +41,7 @@ static cudaError_t launch_products(const CUtensorMap& w0, const CUtensorMap& w1,
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_pdl(kernel, dim3(sm_count()), dim3(kGgThreads), size_t(GgShape<Q6, NX>::kSmem), st, w0, w1, x, sum, a);
+  return launch_pdl(kernel, dim3(sm_count()), dim3(kGgThreads), size_t(GgShape<Q6, NX>::kSmem), st, m[0], m[1], m[2], m[3], m[4], m[5], a);
 }
 
 }  // namespace dmoe
@@ -85,13 +84,15 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   r.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
   r.rows = d->rows; r.x_rows = d->x_rows; r.assignments = d->assignments; r.topk = d->topk; r.parts = nx; r.sums = !q6;
   r.planes = ws.planes; r.sum = ws.sum; r.scale = ws.scale;
-  CUtensorMap w0, w1, x, sum;
-  const unsigned long long wrows = (unsigned long long)d->groups * d->n;
+  const unsigned long long wrows = (unsigned long long)d->groups * d->n, wcols = (unsigned long long)nblk * (q6 ? 208 : 144);
   const unsigned box = q6 ? 208 : 144;
-  if (!byte_map(&w0, d->w, wrows, (unsigned long long)nblk * box, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-      !byte_map(&w1, d->w_up ? d->w_up : d->w, wrows, (unsigned long long)nblk * box, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-      !byte_map(&x, ws.planes, (unsigned long long)nx * d->rows, d->k * 2ull, d->k * 2ull, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !byte_map(&sum, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B))
+  CUtensorMap m[6];                     // weights (two matrices), rows of x by 32 and by 128, their sums by 32 and by 128
+  if (!byte_map(m + 0, d->w, wrows, wcols, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !byte_map(m + 1, d->w_up ? d->w_up : d->w, wrows, wcols, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !byte_map(m + 2, ws.planes, (unsigned long long)nx * d->rows, d->k * 2ull, d->k * 2ull, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !byte_map(m + 3, ws.planes, (unsigned long long)nx * d->rows, d->k * 2ull, d->k * 2ull, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !byte_map(m + 4, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B) ||
+      !byte_map(m + 5, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 128, 32, CU_TENSOR_MAP_SWIZZLE_32B))
     return cudaErrorInvalidValue;
   if ((e = launch_pdl(ggml_rows_kernel, dim3(unsigned(d->rows)), dim3(kGgRowThreads), 0, st, r))) return e;
   GgArgs a = {};
@@ -101,13 +102,13 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   // f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
   switch (d->out_ty) {
     case DARASK_GGML_F32:
-      if (q6) return nx == 2 ? launch_products<true, 2, 2, float>(w0, w1, x, sum, a, st) : launch_products<true, 1, 2, float>(w0, w1, x, sum, a, st);
-      return nx == 2 ? launch_products<false, 2, 1, float>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1, float>(w0, w1, x, sum, a, st);
+      if (q6) return nx == 2 ? launch_products<true, 2, 2, float>(m, a, st) : launch_products<true, 1, 2, float>(m, a, st);
+      return nx == 2 ? launch_products<false, 2, 1, float>(m, a, st) : launch_products<false, 1, 1, float>(m, a, st);
     case DARASK_GGML_F16:
-      if (q6) return nx == 2 ? launch_products<true, 2, 1, __half>(w0, w1, x, sum, a, st) : launch_products<true, 1, 1, __half>(w0, w1, x, sum, a, st);
-      return nx == 2 ? launch_products<false, 2, 1, __half>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1, __half>(w0, w1, x, sum, a, st);
+      if (q6) return nx == 2 ? launch_products<true, 2, 1, __half>(m, a, st) : launch_products<true, 1, 1, __half>(m, a, st);
+      return nx == 2 ? launch_products<false, 2, 1, __half>(m, a, st) : launch_products<false, 1, 1, __half>(m, a, st);
     default:
-      return q6 ? launch_products<true, 1, 1, __nv_bfloat16>(w0, w1, x, sum, a, st) : launch_products<false, 1, 1, __nv_bfloat16>(w0, w1, x, sum, a, st);
+      return q6 ? launch_products<true, 1, 1, __nv_bfloat16>(m, a, st) : launch_products<false, 1, 1, __nv_bfloat16>(m, a, st);
   }
 }
 

@@ -12,7 +12,7 @@
 // tcgen05.mma reads it: it costs shared memory neither space nor bandwidth.
 //   warp 0        TMA: packed weight rows (128 x 144 or 208 bytes) per 256 columns, rows of x per 128 columns, their sums
 //   warp 1        tcgen05.mma kind::f16; per 256 columns one accumulator buffer of two
-//   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 128 columns of k per slot
+//   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 128 columns of k in each of two slots
 //   warps 12-15   promotion (thread = one weight row): acc += d * main - dmin * min, and the store at the end of a tile
 // TMEM: two main buffers of 128 columns, 128 columns for Q4_K's min products or Q6_K's second terms, 128 for the slots.
 // Persistent: tiles are dealt out in steps of the grid, the row tiles of a group's weight tile next to each other.
@@ -44,12 +44,11 @@ struct GgShape {
   static constexpr int kRawBytes = Q6 ? 208 : 144;
   static constexpr int kRawStage = 128 * kRawBytes;
   static constexpr int kRawStages = 3;
-  static constexpr int kXStage = NX * kGgStepBytes;
-  static constexpr int kXStages = NX == 1 ? 3 : 2;
+  static constexpr int kXStage = NX * kGgStepBytes + (Q6 ? 0 : kGgSumBytes);      // Q4_K: the sums travel with the second step of a block
+  static constexpr int kXStages = NX == 1 ? 4 : 2;
   static constexpr int kOffX = 0;                        // 1024-byte aligned tiles first
-  static constexpr int kOffSum = kOffX + kXStages * kXStage;
-  static constexpr int kOffMin = kOffSum + (Q6 ? 0 : 2 * kGgSumBytes);
-  static constexpr int kOffRaw = kOffMin + (Q6 ? 0 : 2 * kGgSumBytes);
+  static constexpr int kOffMin = kOffX + kXStages * kXStage;
+  static constexpr int kOffRaw = kOffMin + (Q6 ? 0 : kGgSumBytes);
   static constexpr int kOffD = kOffRaw + kRawStages * kRawStage;
   static constexpr int kOffEnds = kOffD + 4 * 128 * 8;
   static constexpr int kSmem = 1024 + kOffEnds + (kGgMaxGroups + 1) * 4;
@@ -67,7 +66,8 @@ struct GgRowsArgs {
   __half* sum;                                           // [rows][k / 256][16]: 8 high, 8 low
   float* scale;                                          // [rows]
 };
-constexpr int kGgRowThreads = 256;
+constexpr int kGgRowThreads = 128;
+constexpr int kGgRowHeld = 8;                            // groups of four columns a thread keeps in registers (k <= 4096); longer rows are read twice
 __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsArgs a) {
   __shared__ uint32_t red[kGgRowThreads / 32];
   pdl_wait();
@@ -77,13 +77,25 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   long long row = i;
   if (a.assignments) row = __ldg(a.assignments + i) / unsigned(a.topk);
   const bool exists = row < a.x_rows;
+  float held[kGgRowHeld][4];
   uint32_t top = 0;
+  auto scan = [&](const float (&v)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int j = 0; j < kGgRowHeld; ++j) {
+    const int c = (j * kGgRowThreads + threadIdx.x) * 4;
+    held[j][0] = held[j][1] = held[j][2] = held[j][3] = 0.f;
+    if (exists && c < k) row_source_load4(a.src, row, c, held[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kGgRowHeld; ++j) scan(held[j]);
   if (exists)
-    for (int c = threadIdx.x * 4; c < k; c += kGgRowThreads * 4) {
+    for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 4; c < k; c += kGgRowThreads * 4) {
       float v[4];
       row_source_load4(a.src, row, c, v);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
+      scan(v);
     }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
@@ -97,31 +109,30 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   if (threadIdx.x == 0)
     a.scale[i] = !exists ? -1.f : top == 0u ? 1.f : finite ? __uint_as_float(uint32_t(127 + e) << 23) : __uint_as_float(0x7fffffffu);
   const bool live = exists && finite;
-  for (int c = threadIdx.x * 4; c < k; c += kGgRowThreads * 4) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) row_source_load4(a.src, row, c, v);
+  auto put = [&](int c, float (&v)[4]) {
     __half hi[4];
     float s = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      v[q] *= down;
+      v[q] = live ? v[q] * down : 0.f;
       hi[q] = __float2half_rn(v[q]);
       s += v[q];
     }
-    auto put = [&](__half* p, const __half (&h)[4]) {
+    auto store = [&](__half* p, const __half (&h)[4]) {
       const __half2 w0 = __halves2half2(h[0], h[2]), w1 = __halves2half2(h[1], h[3]);
       *reinterpret_cast<uint2*>(p + size_t(i) * k + c) = make_uint2(*reinterpret_cast<const uint32_t*>(&w0), *reinterpret_cast<const uint32_t*>(&w1));
     };
-    put(a.planes, hi);
+    store(a.planes, hi);
     if (a.parts > 1) {
       __half lo[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) lo[q] = __float2half_rn(v[q] - __half2float(hi[q]));
-      put(a.planes + size_t(a.rows) * k, lo);
+      store(a.planes + size_t(a.rows) * k, lo);
     }
-    if (a.sums) {                                        // k is a multiple of 256: whole warps are here
+    if (a.sums) {                                        // k is a multiple of 256: groups of eight lanes are here or not as one
+      const unsigned mask = 0xffu << (threadIdx.x & 24);
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(mask, s, o);
       if ((threadIdx.x & 7) == 0) {
         const __half h = __float2half_rn(s);
         __half* p = a.sum + (size_t(i) * (k / 256) + c / 256) * 16 + (c % 256) / 32;
@@ -129,6 +140,16 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
         p[8] = __float2half_rn(s - __half2float(h));
       }
     }
+  };
+#pragma unroll
+  for (int j = 0; j < kGgRowHeld; ++j) {
+    const int c = (j * kGgRowThreads + threadIdx.x) * 4;
+    if (c < k) put(c, held[j]);
+  }
+  for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 4; c < k; c += kGgRowThreads * 4) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) row_source_load4(a.src, row, c, v);
+    put(c, v);
   }
 }
 
@@ -185,14 +206,20 @@ template <> DEVI __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __flo
 template <bool Q6, int NX, int NA, typename OUT>
 __global__ void __launch_bounds__(kGgThreads, 1)
 ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
-                    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_sum, const GgArgs a) {
+                    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x4, const __grid_constant__ CUtensorMap map_sum,
+                    const __grid_constant__ CUtensorMap map_sum4, const GgArgs a) {
   using S = GgShape<Q6, NX>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
   int* ends = reinterpret_cast<int*>(smem + S::kOffEnds);                   // [groups + 1] cumulative tile counts
-  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], xfull[S::kXStages], xempty[S::kXStages], afull[2], aempty[2], sfull[2],
-      sempty[2], tfull[2], tempty[2];
+  // A step (128 columns of k) has one "full" barrier, on which its tile of x and its eight expander warps count, and one "empty"
+  // barrier, on which the tensor core reports it read: the loader, the expanders (two steps on) and, at the end of a block of
+  // 256 columns, the promotion all wait for that one. Waits and commits are what the MMA warp spends its time on.
+  // With two stages and nothing but the buffers between them (Q6_K) the tensor core could report the next block before a late warp
+  // has looked for this one, so the promotion has barriers of its own there.
+  constexpr bool kOwnDone = Q6 && S::kXStages == 2;
+  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], full[S::kXStages], empty[S::kXStages], tempty[2], done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float xsc[4][128];
   __shared__ volatile int abort_flag;
@@ -200,8 +227,8 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < S::kRawStages; ++s) { mbar_init(wfull + s, 1); mbar_init(wempty + s, 8); }
-    for (int s = 0; s < S::kXStages; ++s) { mbar_init(xfull + s, 1); mbar_init(xempty + s, 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(afull + s, 4); mbar_init(aempty + s, 1); mbar_init(sfull + s, 5); mbar_init(sempty + s, 1); mbar_init(tfull + s, 1); mbar_init(tempty + s, 4); }
+    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, 9); mbar_init(empty + s, 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(tempty + s, 4); mbar_init(done + s, 1); }
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc<512>(&tmem_slot);
@@ -259,110 +286,109 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     if (warp == 0) {
       // ---- TMA ---------------------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
-      int wi = 0, xi = 0;                // 256-column and 128-column steps so far
+      int ws = 0, xs = 0, used_w = 0, used_x = 0;        // stages, stages filled so far (up to the first round)
+      uint32_t wph = 1, xph = 1;                         // parities of the "empty" phases
       bool ok = true;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
+        // rows of x in boxes of 32, or one box of 128
+        const bool wide = t.rows > 96;
         const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
-        const int wrow = t.group * a.n + t.n0, boxes = (t.rows + 31) / 32, first = int(t.first);
+        const CUtensorMap *mx = wide ? &map_x4 : &map_x, *ms = wide ? &map_sum4 : &map_sum;
+        const int wrow = t.group * a.n + t.n0, boxes = wide ? 1 : (t.rows + 31) / 32, height = wide ? 128 : 32, first = int(t.first);
 #pragma unroll 1
-        for (int b = 0; b < a.nblk; ++b, ++wi) {
-          const int ws = wi % S::kRawStages, ss = wi & 1;
-          if (wi >= S::kRawStages) ok = uniform_wait(wempty + ws, ((wi / S::kRawStages) & 1) ^ 1, a.status);
+        for (int b = 0; b < a.nblk && ok; ++b) {
+          if (used_w == S::kRawStages) ok = warp_wait(wempty + ws, wph, a.status);
+          else ++used_w;
           if (!ok) break;
           if (go) {
             mbar_arrive_expect_tx(wfull + ws, S::kRawStage);
             tma_load_2d(smem_u32(smem + S::kOffRaw + ws * S::kRawStage), mw, b * S::kRawBytes, wrow, wfull + ws);
           }
-          if (!Q6) {
-            if (wi >= 2) ok = uniform_wait(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status);
-            if (!ok) break;
-            if (go) {
-              mbar_arrive_expect_tx(sfull + ss, boxes * 32 * 32);
+          if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
 #pragma unroll 1
-              for (int q = 0; q < boxes; ++q)
-                tma_load_2d(smem_u32(smem + S::kOffSum + ss * kGgSumBytes + q * 32 * 32), &map_sum, b * 32, first + 32 * q, sfull + ss);
-            }
-          }
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c, ++xi) {
-            const int xs = xi % S::kXStages;
-            if (xi >= S::kXStages) ok = uniform_wait(xempty + xs, ((xi / S::kXStages) & 1) ^ 1, a.status);
+          for (int c = 0; c < 2; ++c) {
+            if (used_x == S::kXStages) ok = warp_wait(empty + xs, xph, a.status);
+            else ++used_x;
             if (!ok) break;
             if (go) {
               const uint32_t dst = smem_u32(smem + S::kOffX + xs * S::kXStage);
               const int col = (b * 2 + c) * 256;
-              mbar_arrive_expect_tx(xfull + xs, NX * boxes * 2 * 32 * 128);
+              const bool with_sums = !Q6 && c;
+              mbar_arrive_expect_tx(full + xs, boxes * height * (NX * 256 + (with_sums ? 32 : 0)));
 #pragma unroll 1
-              for (int q = 0; q < boxes; ++q)
-#pragma unroll 1
-                for (int p = 0; p < 2 * NX; ++p)             // 64 columns of a part each
-                  tma_load_2d(dst + p * kGgBoxBytes + q * 32 * 128, &map_x, col + (p & 1) * 128, (p >> 1) * int(a.rows) + first + 32 * q, xfull + xs);
+              for (int q = 0; q < boxes; ++q) {
+                const int r = first + 32 * q;
+                tma_load_2d(dst + q * 32 * 128, mx, col, r, full + xs);
+                tma_load_2d(dst + q * 32 * 128 + kGgBoxBytes, mx, col + 128, r, full + xs);
+                if (NX == 2) {
+                  tma_load_2d(dst + q * 32 * 128 + 2 * kGgBoxBytes, mx, col, int(a.rows) + r, full + xs);
+                  tma_load_2d(dst + q * 32 * 128 + 3 * kGgBoxBytes, mx, col + 128, int(a.rows) + r, full + xs);
+                }
+                if (with_sums) tma_load_2d(dst + NX * kGgStepBytes + q * 32 * 32, ms, b * 32, r, full + xs);
+              }
             }
+            if (++xs == S::kXStages) { xs = 0; xph ^= 1; }
           }
-          if (!ok) break;
         }
       }
       if (!ok) {                         // after a timeout the copies in flight land before the block ends
         abort_flag = 1;
-        for (int i = wi > S::kRawStages ? wi - S::kRawStages : 0; i < wi; ++i) pipe_wait(wfull + i % S::kRawStages, (i / S::kRawStages) & 1, a.status);
-        for (int i = xi > S::kXStages ? xi - S::kXStages : 0; i < xi; ++i) pipe_wait(xfull + i % S::kXStages, (i / S::kXStages) & 1, a.status);
+        for (int i = 0; i < used_w; ++i) pipe_wait(wfull + i, i < ws ? wph ^ 1 : wph, a.status);
+        for (int i = 0; i < used_x; ++i) pipe_wait(full + i, i < xs ? xph ^ 1 : xph, a.status);
       }
     } else if (warp == 1) {
       // ---- MMA ---------------------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
-      int wi = 0, xi = 0;
+      const uint64_t dx0 = umma_desc_k128(smem_u32(smem + S::kOffX)), dmin = umma_desc_k32(smem_u32(smem + S::kOffMin));
+      const uint64_t dsum0 = umma_desc_k32(smem_u32(smem + S::kOffX + NX * kGgStepBytes));
+      uint32_t wi = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
         const uint32_t idesc = __shfl_sync(0xffffffffu, (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24), 0);
 #pragma unroll 1
-        for (int b = 0; b < a.nblk; ++b, ++wi) {
-          const int buf = wi & 1;
-          const uint32_t d = tmem + buf * 128;
-          if (wi >= 2) ok = uniform_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+        for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
+          const uint32_t buf = wi & 1, d = tmem + buf * 128;
+          // stage of the first step and its parity: two or four stages
+          const uint32_t x0 = S::kXStages == 4 ? buf * 2 : 0u, ph = S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1;
+          // the buffer is free: Q6_K waits for the block before the last here; Q4_K waited for it in the last round
+          if (Q6 && wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+          ok = warp_wait(full + x0, ph, a.status) && ok;
           if (!ok) break;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c, ++xi) {
-            const int xs = xi % S::kXStages;
-            ok = uniform_wait(xfull + xs, (xi / S::kXStages) & 1, a.status) && uniform_wait(afull + c, wi & 1, a.status);
-            if (!ok) break;
-            tmem_fence_after();
-            const uint64_t dx = umma_desc_k128(smem_u32(smem + S::kOffX + xs * S::kXStage));
-            const uint32_t at = tmem_a + c * 64, am = tmem_min + c * 64;
+          tmem_fence_after();
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const uint64_t box = (q >> 2) * (kGgBoxBytes >> 4) + 2 * (q & 3);      // 16 columns of k, in units of 16 bytes
-              umma_f16_ts(d, at + q * 8, dx + box, idesc, q ? 1u : uint32_t(c), go);
-              if (NX == 2) umma_f16_ts(d, at + q * 8, dx + (kGgStepBytes >> 4) + box, idesc, 1u, go);
-              if (NA == 2) umma_f16_ts(d, am + q * 8, dx + box, idesc, 1u, go);
+          for (int step = 0; step < 2; ++step) {
+            if (step == 1) {
+              // the accumulator of the mins is free once the last block has been promoted
+              if (!Q6 && wi >= 1) ok = warp_wait(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status);
+              ok = warp_wait(full + x0 + 1, ph, a.status) && ok;
+              if (!ok) break;
+              tmem_fence_after();
             }
-            umma_commit_if(xempty + xs, go);
-            umma_commit_if(aempty + c, go);
+            const uint64_t dx = dx0 + (x0 + step) * uint32_t(S::kXStage >> 4);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {                    // 16 columns of k
+              const uint64_t box = (q >> 2) * (kGgBoxBytes >> 4) + 2 * (q & 3);
+              umma_f16_ts(d, tmem_a + step * 64 + q * 8, dx + box, idesc, step | q ? 1u : 0u, go);
+              if (NX == 2) umma_f16_ts(d, tmem_a + step * 64 + q * 8, dx + (kGgStepBytes >> 4) + box, idesc, 1u, go);
+              if (NA == 2) umma_f16_ts(d, tmem_min + step * 64 + q * 8, dx + box, idesc, 1u, go);
+            }
+            if (!Q6 && step == 1) umma_f16_ss(tmem_min, dmin, dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);      // sums times mins
+            umma_commit_if(empty + x0 + step, go);
           }
-          if (!ok) break;
-          if (!Q6) {
-            // sums times mins: one step of 16; its accumulator is free once the block of 256 columns before has been promoted
-            const int ss = wi & 1;
-            if (wi >= 1) ok = uniform_wait(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status);
-            if (ok) ok = uniform_wait(sfull + ss, (wi >> 1) & 1, a.status);
-            if (!ok) break;
-            tmem_fence_after();
-            umma_f16_ss(tmem_min, umma_desc_k32(smem_u32(smem + S::kOffMin + ss * kGgSumBytes)),
-                        umma_desc_k32(smem_u32(smem + S::kOffSum + ss * kGgSumBytes)), idesc, 0u, go);
-            umma_commit_if(sempty + ss, go);
-          }
-          umma_commit_if(tfull + buf, go);
+          if (kOwnDone && ok) umma_commit_if(done + buf, go);
         }
       }
       if (!ok) abort_flag = 1;
     }
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    // ---- expanders: warps 4-7 the first 128 columns of a block, warps 8-11 the others --------------------------------------
+    // ---- expanders: warps 4-7 the first 64 columns of every step, warps 8-11 the other 64 ------------------
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = uint32_t((warp & 3) * 32) << 16;
-    int wi = 0;
+    int ws = 0;
+    uint32_t wph = 0, wi = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
       const GgTile t = locate(tile);
@@ -373,50 +399,45 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         dq = reinterpret_cast<const __half*>(a.w[t.mat] + (size_t(t.group) * a.n + r) * a.row_bytes + size_t(a.nblk) * 208);
         d_next = __half2float(__ldg(dq));
       }
+#pragma unroll 1
       for (int b = 0; b < a.nblk; ++b, ++wi) {
-        const int ws = wi % S::kRawStages;
         const float d_now = d_next;
         if (Q6 && set == 0 && b + 1 < a.nblk) d_next = __half2float(__ldg(dq + b + 1));
-        if (!warp_wait(wfull + ws, (wi / S::kRawStages) & 1, a.status)) { ok = false; break; }
+        if (!warp_wait(wfull + ws, wph, a.status)) { ok = false; break; }
         const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
-        uint4 head;                      // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
-        head = lds128(raw + (Q6 ? 192 : 0));
-        uint32_t scales = 0;             // Q4_K: four scales of this set's columns
-        if (!Q6) scales = set == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
-        if (wi >= 1 && !warp_wait(aempty + set, (wi & 1) ^ 1, a.status)) { ok = false; break; }
-        tmem_fence_after();
-        if (set == 0) {
-          if (Q6) dring[(wi & 3) * 128 + row] = make_float2(d_now, 0.f);
-          else {
+        // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
+        const uint4 head = lds128(raw + (Q6 ? 192 : 0));
+#pragma unroll 1
+        for (int cc = 0; cc < 2; ++cc) {                  // 64 columns
+          const int c = cc * 2 + set;
+          uint4 w0, w1;                                   // Q4_K: codes; Q6_K: upper bits
+          w0 = lds128(raw + (Q6 ? 128 + cc * 32 : 16 + c * 32));
+          w1 = lds128(raw + (Q6 ? 128 + cc * 32 : 16 + c * 32) + 16);
+          // the TMEM slot is free when the step before the last has been read: stage and parity of step 2 (wi - 1) + cc
+          const uint32_t pw = wi - 1;
+          if (wi >= 1 && !warp_wait(empty + (S::kXStages == 4 ? (pw & 1) * 2 + cc : cc), S::kXStages == 4 ? (pw >> 1) & 1 : pw & 1, a.status)) {
+            ok = false;
+            break;
+          }
+          tmem_fence_after();
+          if (c == 0) {
             const __half2 dd = as_half2(head.x);
-            dring[(wi & 3) * 128 + row] = make_float2(__low2float(dd), __high2float(dd));
+            dring[(wi & 3) * 128 + row] = Q6 ? make_float2(d_now, 0.f) : make_float2(__low2float(dd), -__high2float(dd));
+          }
+          if (!Q6 && c == 3) {
             // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
             const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
             auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
             const uint4 m = make_uint4(pair(m0, 0x4140), pair(m0, 0x4342), pair(m1, 0x4140), pair(m1, 0x4342));
-            const int ss = wi & 1;
-            if (wi >= 2 && !warp_wait(sempty + ss, ((wi >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
-            uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + ss * kGgSumBytes + row * 32);
+            uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + row * 32);
             p[0] = m;
             p[1] = m;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sfull + ss);
-          }
-        }
-#pragma unroll 1
-        for (int cc = 0; cc < 2; ++cc) {                  // 64 columns
-          const int c = set * 2 + cc;
-          uint4 w0, w1, h0, h1;
-          if (!Q6) {
-            w0 = lds128(raw + 16 + c * 32);
-            w1 = lds128(raw + 16 + c * 32 + 16);
-          } else {
-            h0 = lds128(raw + 128 + set * 32);
-            h1 = lds128(raw + 128 + set * 32 + 16);
           }
           const uint32_t dst = tl + c * 32;
-          const uint32_t scw = scales >> (16 * cc);     // Q4_K: two scales of 32 columns
+          // Q4_K: scales of sub-blocks 2c and 2c + 1
+          const uint32_t scales = cc == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
+          const uint32_t scw = scales >> (16 * set);
           if (!Q6) {
             // low nibbles: columns 0-31 of the step, high nibbles: 32-63; (1024 + q) sc - 1024 sc, every term exact
             const __half2 s0 = byte_half2<0>(scw, 1024.f), s1 = byte_half2<1>(scw, 1024.f);
@@ -434,12 +455,12 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             tmem_st16(tmem_a + dst, lo);
             tmem_st16(tmem_a + dst + 16, hi);
           } else {
-            uint32_t sc4 = (set == 0 ? (cc == 0 ? head.x : head.y) : (cc == 0 ? head.z : head.w)) ^ 0x80808080u;
-            const int down = 4 * cc;                     // the second step of a half block has the high nibbles and the upper bit pairs
-            const uint32_t hq[8] = {h0.x >> down, h0.y >> down, h0.z >> down, h0.w >> down, h1.x >> down, h1.y >> down, h1.z >> down, h1.w >> down};
+            uint32_t sc4 = (cc == 0 ? (set == 0 ? head.x : head.y) : (set == 0 ? head.z : head.w)) ^ 0x80808080u;
+            const int down = 4 * set;                    // the second 64 columns of a half block have the high nibbles and the upper bit pairs
+            const uint32_t hq[8] = {w0.x >> down, w0.y >> down, w0.z >> down, w0.w >> down, w1.x >> down, w1.y >> down, w1.z >> down, w1.w >> down};
 #pragma unroll 1
             for (int part = 0; part < 2; ++part, sc4 >>= 16) {       // 32 columns: the first or the second 32 bytes of ql
-              const uint4 l0 = lds128(raw + set * 64 + part * 32), l1 = lds128(raw + set * 64 + part * 32 + 16);
+              const uint4 l0 = lds128(raw + cc * 64 + part * 32), l1 = lds128(raw + cc * 64 + part * 32 + 16);
               const uint32_t wd[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
               const __half2 sa = byte_half2<0>(sc4, 1152.f), sb = byte_half2<1>(sc4, 1152.f);
               const int up = 4 - 2 * part;
@@ -461,14 +482,14 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
               if (NA == 2) tmem_st16(tmem_min + dst + part * 16, r);
             }
           }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + (S::kXStages == 4 ? (wi & 1) * 2 + cc : cc));
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(afull + set);
-          mbar_arrive(wempty + ws);
-        }
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(wempty + ws);
+        if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
       }
     }
     if (!ok) abort_flag = 1;
@@ -477,29 +498,32 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     // ---- promotion and store ---------------------------------------------------------------------------------------------
     const int row = (warp - 12) * 32 + lane;
     const uint32_t tl = uint32_t((warp - 12) * 32) << 16;
-    int wi = 0;
+    uint32_t wi = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
       const GgTile t = locate(tile);
-      float acc[128];
+      unsigned long long acc[64];                         // pairs of float32 sums
 #pragma unroll
-      for (int c = 0; c < 128; ++c) acc[c] = 0.f;
+      for (int c = 0; c < 64; ++c) acc[c] = 0ull;
+#pragma unroll 1
       for (int b = 0; b < a.nblk; ++b, ++wi) {
-        const int buf = wi & 1;
-        if (!warp_wait(tfull + buf, (wi >> 1) & 1, a.status)) { ok = false; break; }
+        const uint32_t buf = wi & 1;
+        uint64_t* bar = kOwnDone ? done + buf : empty + (S::kXStages == 4 ? buf * 2 + 1 : 1);
+        if (!warp_wait(bar, kOwnDone || S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1, a.status)) { ok = false; break; }
         tmem_fence_after();
-        const float2 d = dring[(wi & 3) * 128 + row];
+        const float2 d = dring[(wi & 3) * 128 + row];     // {d, -dmin}
+        const unsigned long long dd = pack2(d.x, d.x), dm = pack2(d.y, d.y);
 #pragma unroll
         for (int c = 0; c < 128; c += 32) {
           if (c < t.rows) {
             uint32_t v[32];
             tmem_ld32(tmem + tl + buf * 128 + c, v);
 #pragma unroll
-            for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(d.x, __uint_as_float(v[q]), acc[c + q]);
+            for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dd, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
             if (!Q6) {
               tmem_ld32(tmem_min + tl + c, v);
 #pragma unroll
-              for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(-d.y, __uint_as_float(v[q]), acc[c + q]);
+              for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dm, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
             }
           }
         }
@@ -525,8 +549,11 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int c = 0; c < 128; c += 16) {
         if (c < t.rows) {
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            if (c + q < t.rows && col < a.n) *p = from_float<OUT>(acc[c + q] * mine[c + q]);
+          for (int q = 0; q < 8; ++q) {
+            const float2 y = unpack2(acc[c / 2 + q]);
+            if (c + 2 * q < t.rows && col < a.n) *p = from_float<OUT>(y.x * mine[c + 2 * q]);
+            p += a.ldo;
+            if (c + 2 * q + 1 < t.rows && col < a.n) *p = from_float<OUT>(y.y * mine[c + 2 * q + 1]);
             p += a.ldo;
           }
         }

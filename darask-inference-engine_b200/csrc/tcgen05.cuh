@@ -61,6 +61,22 @@ template <int COLS>
 DEVI void tmem_free(uint32_t base) {            // the warp that allocated
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(uint32_t(COLS)) : "memory");
 }
+// Two float32 sums at a time: {a.lo * b.lo + c.lo, a.hi * b.hi + c.hi}, each rounded once
+DEVI unsigned long long pack2(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+DEVI float2 unpack2(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+DEVI unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // 32 columns of this warp's 32 TMEM lanes -> registers, complete on return
 DEVI void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -89,42 +105,45 @@ DEVI void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
 #undef DMOE_R16
 #undef DMOE_R4
 
-// Bounded wait for a phase, a handful of instructions (the roles of these kernels run side by side and fight for the
-// instruction cache). A probe suspends the thread for up to 2 us; a million of them end the wait and set the status bit.
+// Bounded wait for a phase. A probe of a phase that is over costs 43 cycles (74 with a suspension limit), so the first one goes
+// without; then each probe suspends the thread for up to 2 us, and a million of them end the wait and set the status bit.
 DEVI bool pipe_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
   const uint32_t addr = smem_u32(bar);
-#pragma unroll 1
-  for (uint32_t i = 0; i < 1000000u; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(addr), "r"(parity), "r"(2000u)
-        : "memory");
-    if (ok) return true;
-  }
-  atomicOr(status, kStatusWaitTimeout);
-  return false;
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  if (ok) return true;
+  // (the loop is one statement so that the compiler does not unroll, rotate or duplicate it)
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .u32 i;\n\t"
+      "mov.u32 i, 1000000;\n\t"
+      "probe:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+      "@p bra over;\n\t"
+      "sub.u32 i, i, 1;\n\t"
+      "setp.ne.u32 p, i, 0;\n\t"
+      "@p bra probe;\n\t"
+      "over:\n\t"
+      "min.u32 %0, i, 1;\n\t}"
+      : "=r"(ok)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  if (!ok) atomicOr(status, kStatusWaitTimeout);
+  return ok != 0;
 }
-// The same for a warp whose lanes stay together, so that its loop stays on the uniform datapath (the operands of tcgen05.mma
-// and of the tensor copies live in uniform registers; a loop of one lane moves every one of them there anew).
-DEVI bool uniform_wait(uint64_t* bar, uint32_t parity, unsigned* status) { return __all_sync(0xffffffffu, pipe_wait(bar, parity, status)); }
+// The same for a whole warp, every lane probing (cheaper than one lane and a broadcast); the lanes stay together, so that loops
+// around it stay on the uniform datapath, where the operands of tcgen05.mma and of the tensor copies live.
+DEVI bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* status) { return __all_sync(0xffffffffu, pipe_wait(bar, parity, status)); }
 DEVI uint32_t elect_lane() {
   uint32_t one;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one;
 }
-// A whole warp waits: one lane watches the barrier (32 probes of one word serialise in shared memory).
-DEVI bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
-  int ok = 1;
-  if ((threadIdx.x & 31) == 0) ok = pipe_wait(bar, parity, status) ? 1 : 0;
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  __syncwarp();
-  return ok != 0;
-}
-
 // ---- clusters --------------------------------------------------------------------------------------------------------
 DEVI uint32_t cluster_rank() {
   uint32_t r;
