@@ -29,19 +29,29 @@ static GroupedWs carve(void* base, long long rows, int k, int parts) {
   return w;
 }
 
-template <bool Q6, int NX, int NA, typename OUT>
+template <bool Q6, int NT, int NX, int NA, typename OUT>
 static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
-  static_assert(GgShape<Q6, NX>::kSmem <= kSmemBudget, "rings must fit one block");
+  using S = GgShape<Q6, NT, NX, NA>;
+  static_assert(S::kSmem + 5 * 1024 - 1024 <= kSmemBudget, "rings must fit one block");
   static bool configured[64] = {};      // the opt-in is per device and per kernel
   const int dev = current_device_slot();
   if (dev < 0) return cudaErrorInvalidDevice;
-  auto kernel = ggml_grouped_kernel<Q6, NX, NA, OUT>;
+  auto kernel = ggml_grouped_kernel<Q6, NT, NX, NA, OUT>;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GgShape<Q6, NX>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_pdl(kernel, dim3(sm_count()), dim3(kGgThreads), size_t(GgShape<Q6, NX>::kSmem), st, m[0], m[1], m[2], m[3], m[4], m[5], a);
+  return launch_pdl(kernel, dim3(sm_count()), dim3(S::kThreads), size_t(S::kSmem), st, m[0], m[1], m[2], m[3], m[4], m[5], a);
+}
+
+// f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
+template <bool Q6, int NT>
+static cudaError_t launch_by_type(int out_ty, int nx, const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
+  constexpr int NA = Q6 ? 2 : 1;
+  if (out_ty == DARASK_GGML_F32) return nx == 2 ? launch_products<Q6, NT, 2, NA, float>(m, a, st) : launch_products<Q6, NT, 1, NA, float>(m, a, st);
+  if (out_ty == DARASK_GGML_F16) return nx == 2 ? launch_products<Q6, NT, 2, 1, __half>(m, a, st) : launch_products<Q6, NT, 1, 1, __half>(m, a, st);
+  return launch_products<Q6, NT, 1, 1, __nv_bfloat16>(m, a, st);
 }
 
 }  // namespace dmoe
@@ -99,17 +109,10 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);
   a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo; a.status = static_cast<unsigned*>(status);
-  // f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
-  switch (d->out_ty) {
-    case DARASK_GGML_F32:
-      if (q6) return nx == 2 ? launch_products<true, 2, 2, float>(m, a, st) : launch_products<true, 1, 2, float>(m, a, st);
-      return nx == 2 ? launch_products<false, 2, 1, float>(m, a, st) : launch_products<false, 1, 1, float>(m, a, st);
-    case DARASK_GGML_F16:
-      if (q6) return nx == 2 ? launch_products<true, 2, 1, __half>(m, a, st) : launch_products<true, 1, 1, __half>(m, a, st);
-      return nx == 2 ? launch_products<false, 2, 1, __half>(m, a, st) : launch_products<false, 1, 1, __half>(m, a, st);
-    default:
-      return q6 ? launch_products<true, 1, 1, __nv_bfloat16>(m, a, st) : launch_products<false, 1, 1, __nv_bfloat16>(m, a, st);
-  }
+  // narrow tiles while the groups have few rows on average: the weights' bytes pace the product then
+  const bool narrow = d->rows <= 32ll * d->groups;
+  if (q6) return narrow ? launch_by_type<true, 32>(d->out_ty, nx, m, a, st) : launch_by_type<true, 128>(d->out_ty, nx, m, a, st);
+  return narrow ? launch_by_type<false, 32>(d->out_ty, nx, m, a, st) : launch_by_type<false, 128>(d->out_ty, nx, m, a, st);
 }
 
 extern "C" int darask_ggml_grouped_status(unsigned* host_status, cudaStream_t st) {

@@ -22,11 +22,7 @@
 
 namespace dmoe {
 
-constexpr int kGgThreads = 512;
 constexpr int kGgMaxGroups = 1024;
-constexpr int kGgBoxBytes = 128 * 128;                   // 128 rows x 64 columns of f16
-constexpr int kGgStepBytes = 2 * kGgBoxBytes;            // a step: 128 columns of k
-constexpr int kGgSumBytes = 128 * 32;                    // 128 rows x 16 f16: the sums of eight groups of 32 columns, twice
 
 struct GgArgs {
   const unsigned* ranges;                                // [groups][2]
@@ -39,19 +35,32 @@ struct GgArgs {
   unsigned* status;
 };
 
-template <bool Q6, int NX>
+// NT: rows of x per tile, NX: f16 parts of a row of x, NA: f16 terms of a Q6_K integer. A step is 128 columns of k.
+template <bool Q6, int NT, int NX, int NA>
 struct GgShape {
+  // Expander sets of four warps; set e has every SETS-th step, and TMEM holds the weights of SETS steps. 128 rows leave TMEM for two;
+  // with 32 rows the weights pace everything and more sets hide their latencies from each other.
+  static constexpr int kSets = NT == 128 ? 2 : NA == 2 ? 3 : 4;
+  static constexpr int kThreads = 128 * (2 + kSets);
   static constexpr int kRawBytes = Q6 ? 208 : 144;
   static constexpr int kRawStage = 128 * kRawBytes;
-  static constexpr int kRawStages = 3;
-  static constexpr int kXStage = NX * kGgStepBytes + (Q6 ? 0 : kGgSumBytes);      // Q4_K: the sums travel with the second step of a block
-  static constexpr int kXStages = NX == 1 ? 4 : 2;
-  static constexpr int kOffX = 0;                        // 1024-byte aligned tiles first
-  static constexpr int kOffMin = kOffX + kXStages * kXStage;
-  static constexpr int kOffRaw = kOffMin + (Q6 ? 0 : kGgSumBytes);
+  static constexpr int kBox = NT * 128;                  // NT rows x 64 columns of f16
+  static constexpr int kPart = 2 * kBox;                 // one part of a step
+  static constexpr int kSums = Q6 ? 0 : NT * 32;         // NT rows x 16 f16: the sums of eight groups of 32 columns, high and low parts
+  static constexpr int kXStage = NX * kPart + kSums;     // Q4_K: the sums travel with the second step of a block
+  static constexpr int kXStages = NT == 128 && NX == 2 ? 2 : 4;
+  static constexpr int kMins = Q6 ? 0 : kSets / 2;       // 128 rows x 32 bytes each
+  static constexpr int kOffMin = kXStages * kXStage;
+  static constexpr int kOffRaw = kOffMin + kMins * 4096;
+  static constexpr int kTail = 4 * 128 * 8 + (kGgMaxGroups + 4) * 4;
+  static constexpr int kFit = (kSmemBudget - 5 * 1024 - kOffRaw - kTail) / kRawStage;
+  static constexpr int kRawStages = kFit < 8 ? kFit : 8;
   static constexpr int kOffD = kOffRaw + kRawStages * kRawStage;
   static constexpr int kOffEnds = kOffD + 4 * 128 * 8;
-  static constexpr int kSmem = 1024 + kOffEnds + (kGgMaxGroups + 1) * 4;
+  static constexpr int kSmem = 1024 + kOffD + kTail;
+  // TMEM columns: two main buffers, the min products, the weights, their second terms
+  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + (Q6 ? 0 : NT), kColA2 = kColA + 64 * kSets;
+  static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSets : 0) <= 512, "rings must fit");
 };
 
 // ---- rows of x -> f16 parts --------------------------------------------------------------------------------------------
@@ -197,37 +206,36 @@ DEVI uint64_t umma_desc_k32(uint32_t smem_addr) {
 
 struct GgTile { int group, n0, mat, rows; long long first; };      // rows of the tile, its first dispatch row
 
-// NX: f16 parts of a row of x; NA: f16 terms of a Q6_K integer
 template <typename T> DEVI T from_float(float v);
 template <> DEVI float from_float<float>(float v) { return v; }
 template <> DEVI __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> DEVI __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <bool Q6, int NX, int NA, typename OUT>
-__global__ void __launch_bounds__(kGgThreads, 1)
+template <bool Q6, int NT, int NX, int NA, typename OUT>
+__global__ void __launch_bounds__((GgShape<Q6, NT, NX, NA>::kThreads), 1)
 ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x4, const __grid_constant__ CUtensorMap map_sum,
                     const __grid_constant__ CUtensorMap map_sum4, const GgArgs a) {
-  using S = GgShape<Q6, NX>;
+  using S = GgShape<Q6, NT, NX, NA>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
   int* ends = reinterpret_cast<int*>(smem + S::kOffEnds);                   // [groups + 1] cumulative tile counts
-  // A step (128 columns of k) has one "full" barrier, on which its tile of x and its eight expander warps count, and one "empty"
-  // barrier, on which the tensor core reports it read: the loader, the expanders (two steps on) and, at the end of a block of
+  // A step (128 columns of k) has one "full" barrier, on which its tile of x and its four expander warps count, and one "empty"
+  // barrier, on which the tensor core reports it read: the loader, the expanders (kSets steps on) and, at the end of a block of
   // 256 columns, the promotion all wait for that one. Waits and commits are what the MMA warp spends its time on.
   // With two stages and nothing but the buffers between them (Q6_K) the tensor core could report the next block before a late warp
   // has looked for this one, so the promotion has barriers of its own there.
   constexpr bool kOwnDone = Q6 && S::kXStages == 2;
   __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], full[S::kXStages], empty[S::kXStages], tempty[2], done[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float xsc[4][128];
+  __shared__ __align__(16) float xsc[4][NT];
   __shared__ volatile int abort_flag;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < S::kRawStages; ++s) { mbar_init(wfull + s, 1); mbar_init(wempty + s, 8); }
-    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, 9); mbar_init(empty + s, 1); }
+    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, 5); mbar_init(empty + s, 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(tempty + s, 4); mbar_init(done + s, 1); }
     mbar_fence_init();
   }
@@ -241,11 +249,11 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     return (long long)o + r <= a.rows ? int(r) : o < a.rows ? int(a.rows - o) : 0;
   };
   const int tiles_n = (a.n + 127) / 128 * a.mats;
-  for (int g = threadIdx.x; g < a.groups; g += kGgThreads) {
+  for (int g = threadIdx.x; g < a.groups; g += S::kThreads) {
     long long first;
     const int r = group_rows(g, &first);
     if (unsigned(r) != __ldcg(a.ranges + 2 * g) && blockIdx.x == 0) atomicOr(a.status, kStatusBadRoute);
-    ends[g] = (r + 127) / 128 * tiles_n;
+    ends[g] = (r + NT - 1) / NT * tiles_n;
   }
   __syncthreads();
   if (warp == 0) {                       // inclusive scan, consecutive groups per lane
@@ -262,7 +270,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = tmem_slot, tmem_min = tmem + 256, tmem_a = tmem + 384;      // Q6_K: second terms at tmem_min
+  const uint32_t tmem = tmem_slot, tmem_min = tmem + S::kColMin, tmem_a = tmem + S::kColA, tmem_a2 = tmem + S::kColA2;
   const int total = ends[a.groups];
   auto locate = [&](int tile) {
     int lo = 0, hi = a.groups;
@@ -272,7 +280,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     t.group = lo;
     const int r = group_rows(lo, &t.first);
     // row tiles of equal height, a multiple of 16
-    const int tiles_m = (r + 127) / 128, h = ((r + tiles_m - 1) / tiles_m + 15) / 16 * 16;
+    const int tiles_m = (r + NT - 1) / NT, h = ((r + tiles_m - 1) / tiles_m + 15) / 16 * 16;
     const int m = local % tiles_m, nt = local / tiles_m;
     t.first += m * h;
     t.rows = r - m * h < h ? r - m * h : h;
@@ -282,7 +290,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ---- TMA ---------------------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
@@ -292,7 +300,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
         // rows of x in boxes of 32, or one box of 128
-        const bool wide = t.rows > 96;
+        const bool wide = NT == 128 && t.rows > 96;
         const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
         const CUtensorMap *mx = wide ? &map_x4 : &map_x, *ms = wide ? &map_sum4 : &map_sum;
         const int wrow = t.group * a.n + t.n0, boxes = wide ? 1 : (t.rows + 31) / 32, height = wide ? 128 : 32, first = int(t.first);
@@ -312,7 +320,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             else ++used_x;
             if (!ok) break;
             if (go) {
-              const uint32_t dst = smem_u32(smem + S::kOffX + xs * S::kXStage);
+              const uint32_t dst = smem_u32(smem + xs * S::kXStage);
               const int col = (b * 2 + c) * 256;
               const bool with_sums = !Q6 && c;
               mbar_arrive_expect_tx(full + xs, boxes * height * (NX * 256 + (with_sums ? 32 : 0)));
@@ -320,12 +328,12 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
               for (int q = 0; q < boxes; ++q) {
                 const int r = first + 32 * q;
                 tma_load_2d(dst + q * 32 * 128, mx, col, r, full + xs);
-                tma_load_2d(dst + q * 32 * 128 + kGgBoxBytes, mx, col + 128, r, full + xs);
+                tma_load_2d(dst + q * 32 * 128 + S::kBox, mx, col + 128, r, full + xs);
                 if (NX == 2) {
-                  tma_load_2d(dst + q * 32 * 128 + 2 * kGgBoxBytes, mx, col, int(a.rows) + r, full + xs);
-                  tma_load_2d(dst + q * 32 * 128 + 3 * kGgBoxBytes, mx, col + 128, int(a.rows) + r, full + xs);
+                  tma_load_2d(dst + q * 32 * 128 + S::kPart, mx, col, int(a.rows) + r, full + xs);
+                  tma_load_2d(dst + q * 32 * 128 + S::kPart + S::kBox, mx, col + 128, int(a.rows) + r, full + xs);
                 }
-                if (with_sums) tma_load_2d(dst + NX * kGgStepBytes + q * 32 * 32, ms, b * 32, r, full + xs);
+                if (with_sums) tma_load_2d(dst + NX * S::kPart + q * 32 * 32, ms, b * 32, r, full + xs);
               }
             }
             if (++xs == S::kXStages) { xs = 0; xph ^= 1; }
@@ -340,18 +348,21 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     } else if (warp == 1) {
       // ---- MMA ---------------------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
-      const uint64_t dx0 = umma_desc_k128(smem_u32(smem + S::kOffX)), dmin = umma_desc_k32(smem_u32(smem + S::kOffMin));
-      const uint64_t dsum0 = umma_desc_k32(smem_u32(smem + S::kOffX + NX * kGgStepBytes));
-      uint32_t wi = 0;
+      const uint64_t dx0 = umma_desc_k128(smem_u32(smem)), dmin = umma_desc_k32(smem_u32(smem + S::kOffMin));
+      const uint64_t dsum0 = umma_desc_k32(smem_u32(smem + NX * S::kPart));
+      uint32_t wi = 0, slot = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
         const uint32_t idesc = __shfl_sync(0xffffffffu, (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24), 0);
 #pragma unroll 1
         for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
-          const uint32_t buf = wi & 1, d = tmem + buf * 128;
+          const uint32_t buf = wi & 1, d = tmem + buf * NT;
           // stage of the first step and its parity: two or four stages
           const uint32_t x0 = S::kXStages == 4 ? buf * 2 : 0u, ph = S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1;
+          // TMEM slots of the two steps
+          const uint32_t a0 = slot, a1 = slot + 1 == S::kSets ? 0u : slot + 1;
+          slot = a1 + 1 == S::kSets ? 0u : a1 + 1;
           // the buffer is free: Q6_K waits for the block before the last here; Q4_K waited for it in the last round
           if (Q6 && wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
           ok = warp_wait(full + x0, ph, a.status) && ok;
@@ -367,14 +378,16 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
               tmem_fence_after();
             }
             const uint64_t dx = dx0 + (x0 + step) * uint32_t(S::kXStage >> 4);
+            const uint32_t at = tmem_a + (step ? a1 : a0) * 64, a2 = tmem_a2 + (step ? a1 : a0) * 64;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {                    // 16 columns of k
-              const uint64_t box = (q >> 2) * (kGgBoxBytes >> 4) + 2 * (q & 3);
-              umma_f16_ts(d, tmem_a + step * 64 + q * 8, dx + box, idesc, step | q ? 1u : 0u, go);
-              if (NX == 2) umma_f16_ts(d, tmem_a + step * 64 + q * 8, dx + (kGgStepBytes >> 4) + box, idesc, 1u, go);
-              if (NA == 2) umma_f16_ts(d, tmem_min + step * 64 + q * 8, dx + box, idesc, 1u, go);
+              const uint64_t box = (q >> 2) * (S::kBox >> 4) + 2 * (q & 3);
+              umma_f16_ts(d, at + q * 8, dx + box, idesc, step | q ? 1u : 0u, go);
+              if (NX == 2) umma_f16_ts(d, at + q * 8, dx + (S::kPart >> 4) + box, idesc, 1u, go);
+              if (NA == 2) umma_f16_ts(d, a2 + q * 8, dx + box, idesc, 1u, go);
             }
-            if (!Q6 && step == 1) umma_f16_ss(tmem_min, dmin, dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);      // sums times mins
+            if (!Q6 && step == 1)                            // sums times mins
+              umma_f16_ss(tmem_min, dmin + (S::kMins == 2 ? buf * (4096u >> 4) : 0u), dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);
             umma_commit_if(empty + x0 + step, go);
           }
           if (kOwnDone && ok) umma_commit_if(done + buf, go);
@@ -382,62 +395,62 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       }
       if (!ok) abort_flag = 1;
     }
-  } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    // ---- expanders: warps 4-7 the first 64 columns of every step, warps 8-11 the other 64 ------------------
+  } else if (warp < 4 + 4 * S::kSets) {
+    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    // ---- expanders: four warps, one for each quarter of the TMEM lanes, take every kSets-th step --------------------------------
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t tl = uint32_t((warp & 3) * 32) << 16;
-    int ws = 0;
+    const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + set * 64;       // the set's TMEM slot
+    int ws = 0, turn = 0;                // raw stage, set whose step comes next
     uint32_t wph = 0, wi = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
       const GgTile t = locate(tile);
       const __half* dq = nullptr;        // Q6_K: the row's block scales
       float d_next = 0.f;
-      if (Q6 && set == 0) {
+      if (Q6) {
         const int r = t.n0 + row < a.n ? t.n0 + row : a.n - 1;
         dq = reinterpret_cast<const __half*>(a.w[t.mat] + (size_t(t.group) * a.n + r) * a.row_bytes + size_t(a.nblk) * 208);
         d_next = __half2float(__ldg(dq));
       }
 #pragma unroll 1
-      for (int b = 0; b < a.nblk; ++b, ++wi) {
+      for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
         const float d_now = d_next;
-        if (Q6 && set == 0 && b + 1 < a.nblk) d_next = __half2float(__ldg(dq + b + 1));
-        if (!warp_wait(wfull + ws, wph, a.status)) { ok = false; break; }
-        const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
-        // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
-        const uint4 head = lds128(raw + (Q6 ? 192 : 0));
+        if (Q6 && b + 1 < a.nblk) d_next = __half2float(__ldg(dq + b + 1));
 #pragma unroll 1
-        for (int cc = 0; cc < 2; ++cc) {                  // 64 columns
-          const int c = cc * 2 + set;
-          uint4 w0, w1;                                   // Q4_K: codes; Q6_K: upper bits
-          w0 = lds128(raw + (Q6 ? 128 + cc * 32 : 16 + c * 32));
-          w1 = lds128(raw + (Q6 ? 128 + cc * 32 : 16 + c * 32) + 16);
-          // the TMEM slot is free when the step before the last has been read: stage and parity of step 2 (wi - 1) + cc
-          const uint32_t pw = wi - 1;
-          if (wi >= 1 && !warp_wait(empty + (S::kXStages == 4 ? (pw & 1) * 2 + cc : cc), S::kXStages == 4 ? (pw >> 1) & 1 : pw & 1, a.status)) {
-            ok = false;
-            break;
-          }
+        for (int h = 0; h < 2; ++h) {                     // the block's two steps
+          const bool mine = turn == set;
+          if (++turn == S::kSets) turn = 0;
+          if (!mine) continue;
+          ok = warp_wait(wfull + ws, wph, a.status);
+          const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
+          // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
+          const uint4 head = lds128(raw + (Q6 ? 192 : 0));
+          // the TMEM slot is free when the step kSets before has been read
+          const uint32_t ps = 2 * wi + h - S::kSets;
+          if (2 * wi + h >= uint32_t(S::kSets)) ok = warp_wait(empty + ps % S::kXStages, (ps / S::kXStages) & 1, a.status) && ok;
+          if (!ok) break;
           tmem_fence_after();
-          if (c == 0) {
+          if (h == 0) {
             const __half2 dd = as_half2(head.x);
             dring[(wi & 3) * 128 + row] = Q6 ? make_float2(d_now, 0.f) : make_float2(__low2float(dd), -__high2float(dd));
-          }
-          if (!Q6 && c == 3) {
+          } else if (!Q6) {
             // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
             const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
             auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
             const uint4 m = make_uint4(pair(m0, 0x4140), pair(m0, 0x4342), pair(m1, 0x4140), pair(m1, 0x4342));
-            uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + row * 32);
+            uint4* p = reinterpret_cast<uint4*>(smem + S::kOffMin + (S::kMins == 2 ? (wi & 1) * 4096 : 0) + row * 32);
             p[0] = m;
             p[1] = m;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
-          const uint32_t dst = tl + c * 32;
-          // Q4_K: scales of sub-blocks 2c and 2c + 1
-          const uint32_t scales = cc == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
-          const uint32_t scw = scales >> (16 * set);
+          // Q4_K: the four scales of the step; Q6_K: the step is one half of the block
+          const uint32_t scales = h == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
+#pragma unroll 1
+          for (int cc = 0; cc < 2; ++cc) {                // 64 columns
+            const uint32_t dst = tl + cc * 32;
+            const uint32_t at = raw + (Q6 ? 128 + h * 32 : 16 + (h * 2 + cc) * 32);
+            const uint4 w0 = lds128(at), w1 = lds128(at + 16);        // Q4_K: codes; Q6_K: upper bits
+            const uint32_t scw = scales >> (16 * cc);
           if (!Q6) {
             // low nibbles: columns 0-31 of the step, high nibbles: 32-63; (1024 + q) sc - 1024 sc, every term exact
             const __half2 s0 = byte_half2<0>(scw, 1024.f), s1 = byte_half2<1>(scw, 1024.f);
@@ -455,12 +468,12 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             tmem_st16(tmem_a + dst, lo);
             tmem_st16(tmem_a + dst + 16, hi);
           } else {
-            uint32_t sc4 = (cc == 0 ? (set == 0 ? head.x : head.y) : (set == 0 ? head.z : head.w)) ^ 0x80808080u;
-            const int down = 4 * set;                    // the second 64 columns of a half block have the high nibbles and the upper bit pairs
+            uint32_t sc4 = (h == 0 ? (cc == 0 ? head.x : head.y) : (cc == 0 ? head.z : head.w)) ^ 0x80808080u;
+            const int down = 4 * cc;                    // the second 64 columns of a half block have the high nibbles and the upper bit pairs
             const uint32_t hq[8] = {w0.x >> down, w0.y >> down, w0.z >> down, w0.w >> down, w1.x >> down, w1.y >> down, w1.z >> down, w1.w >> down};
 #pragma unroll 1
             for (int part = 0; part < 2; ++part, sc4 >>= 16) {       // 32 columns: the first or the second 32 bytes of ql
-              const uint4 l0 = lds128(raw + cc * 64 + part * 32), l1 = lds128(raw + cc * 64 + part * 32 + 16);
+              const uint4 l0 = lds128(raw + h * 64 + part * 32), l1 = lds128(raw + h * 64 + part * 32 + 16);
               const uint32_t wd[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
               const __half2 sa = byte_half2<0>(sc4, 1152.f), sb = byte_half2<1>(sc4, 1152.f);
               const int up = 4 - 2 * part;
@@ -479,32 +492,46 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
                 }
               }
               tmem_st16(tmem_a + dst + part * 16, v);
-              if (NA == 2) tmem_st16(tmem_min + dst + part * 16, r);
+              if (NA == 2) tmem_st16(tmem_a2 + dst + part * 16, r);
             }
+          }
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           tmem_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(full + (S::kXStages == 4 ? (wi & 1) * 2 + cc : cc));
+          if (lane == 0) {
+            mbar_arrive(full + (2 * wi + h) % S::kXStages);
+            mbar_arrive(wempty + ws);
+          }
         }
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(wempty + ws);
         if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
       }
     }
     if (!ok) abort_flag = 1;
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if (NT == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ---- promotion and store ---------------------------------------------------------------------------------------------
-    const int row = (warp - 12) * 32 + lane;
-    const uint32_t tl = uint32_t((warp - 12) * 32) << 16;
+    constexpr int kFirst = 4 + 4 * S::kSets;
+    const int row = (warp - kFirst) * 32 + lane;
+    const uint32_t tl = uint32_t((warp - kFirst) * 32) << 16;
     uint32_t wi = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
       const GgTile t = locate(tile);
-      unsigned long long acc[64];                         // pairs of float32 sums
+      // scales of the tile's rows
+      float* scale = xsc[warp - kFirst];
+      __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = 0ull;
+      for (int q = 0; q < NT / 32; ++q) {
+        const int r = q * 32 + lane;
+        const float v = r < t.rows ? __ldg(a.xscale + t.first + r) : 0.f;
+        if (v < 0.f && warp == kFirst) atomicOr(a.status, kStatusBadRoute);
+        scale[r] = fabsf(v);
+      }
+      __syncwarp();
+      unsigned long long acc[NT / 2];                    // pairs of float32 sums
+#pragma unroll
+      for (int c = 0; c < NT / 2; ++c) acc[c] = 0ull;
 #pragma unroll 1
       for (int b = 0; b < a.nblk; ++b, ++wi) {
         const uint32_t buf = wi & 1;
@@ -514,10 +541,10 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         const float2 d = dring[(wi & 3) * 128 + row];     // {d, -dmin}
         const unsigned long long dd = pack2(d.x, d.x), dm = pack2(d.y, d.y);
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
+        for (int c = 0; c < NT; c += 32) {
           if (c < t.rows) {
             uint32_t v[32];
-            tmem_ld32(tmem + tl + buf * 128 + c, v);
+            tmem_ld32(tmem + tl + buf * NT + c, v);
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dd, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
             if (!Q6) {
@@ -527,37 +554,45 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             }
           }
         }
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tempty + buf);
-      }
-      if (!ok) break;
-      // scales of the tile's rows to shared memory, then one store per element: a warp writes 32 neighbours of an output row
-      float* mine = xsc[warp - 12];
-      __syncwarp();
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = q * 32 + lane;
-        const float s = r < t.rows ? __ldg(a.xscale + t.first + r) : 0.f;
-        if (s < 0.f && warp == 12) atomicOr(a.status, kStatusBadRoute);
-        mine[r] = fabsf(s);
-      }
-      __syncwarp();
-      const int col = t.n0 + row;
-      OUT* p = static_cast<OUT*>(a.out) + size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
-#pragma unroll
-      for (int c = 0; c < 128; c += 16) {
-        if (c < t.rows) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float2 y = unpack2(acc[c / 2 + q]);
-            if (c + 2 * q < t.rows && col < a.n) *p = from_float<OUT>(y.x * mine[c + 2 * q]);
-            p += a.ldo;
-            if (c + 2 * q + 1 < t.rows && col < a.n) *p = from_float<OUT>(y.y * mine[c + 2 * q + 1]);
-            p += a.ldo;
-          }
+        if (b + 1 < a.nblk) {
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tempty + buf);
         }
       }
+      if (!ok) break;
+      // The sums go through the buffer just read, which is not handed back yet: a loop of few instructions stores them (128 stores
+      // in a row would come through the instruction cache anew for every tile). A warp writes 32 neighbours of an output row.
+      const uint32_t last = (wi - 1) & 1, stage = tmem + tl + last * NT;
+#pragma unroll
+      for (int c = 0; c < NT; c += 16) {
+        if (c < t.rows) {
+          uint32_t v[16];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2 y = unpack2(acc[c / 2 + j]);
+            v[2 * j] = __float_as_uint(y.x);
+            v[2 * j + 1] = __float_as_uint(y.y);
+          }
+          tmem_st16(stage + c, v);
+        }
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      const int col = t.n0 + row;
+      OUT* p = static_cast<OUT*>(a.out) + size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+#pragma unroll 1
+      for (int c = 0; c < t.rows; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(stage + c, v);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          if (c + q < t.rows && col < a.n) *p = from_float<OUT>(__uint_as_float(v[q]) * scale[c + q]);
+          p += a.ldo;
+        }
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty + last);
     }
     if (!ok) abort_flag = 1;
   }
