@@ -10,7 +10,7 @@
 // One block computes 128 weight rows x up to 128 dispatch rows of one group; the weight rows are the M operand, so that few
 // rows cost a narrow tile (N a multiple of 16). The weight operand is written straight into TMEM (tcgen05.st), where
 // tcgen05.mma reads it: it costs shared memory neither space nor bandwidth.
-//   warp 0        TMA: packed weight rows (128 x 144 or 208 bytes) per 256 columns, rows of x per 128 columns, their sums
+//   warps 0, 2    TMA: rows of x and their sums per 128 columns; packed weight rows (128 x 144 or 208 bytes) per 256 columns
 //   warp 1        tcgen05.mma kind::f16; per 256 columns one accumulator buffer of two
 //   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 128 columns of k in each of two slots
 //   warps 12-15   promotion (thread = one weight row): acc += d * main - dmin * min, and the store at the end of a tile
@@ -292,58 +292,70 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   if (warp < 4) {
     if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
-      // ---- TMA ---------------------------------------------------------------------------------------------------------
+      // ---- TMA, rows of x ----------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
-      int ws = 0, xs = 0, used_w = 0, used_x = 0;        // stages, stages filled so far (up to the first round)
-      uint32_t wph = 1, xph = 1;                         // parities of the "empty" phases
+      int xs = 0, used = 0;              // stage; stages filled so far (up to the first round)
+      uint32_t ph = 1;                   // parity of the "empty" phase
       bool ok = true;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         const GgTile t = locate(tile);
         // rows of x in boxes of 32, or one box of 128
         const bool wide = NT == 128 && t.rows > 96;
-        const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
         const CUtensorMap *mx = wide ? &map_x4 : &map_x, *ms = wide ? &map_sum4 : &map_sum;
-        const int wrow = t.group * a.n + t.n0, boxes = wide ? 1 : (t.rows + 31) / 32, height = wide ? 128 : 32, first = int(t.first);
+        const int boxes = wide ? 1 : (t.rows + 31) / 32, height = wide ? 128 : 32, first = int(t.first);
 #pragma unroll 1
-        for (int b = 0; b < a.nblk && ok; ++b) {
-          if (used_w == S::kRawStages) ok = warp_wait(wempty + ws, wph, a.status);
-          else ++used_w;
+        for (int c = 0; c < 2 * a.nblk; ++c) {
+          if (used == S::kXStages) ok = warp_wait(empty + xs, ph, a.status);
+          else ++used;
+          if (!ok) break;
+          if (go) {
+            const uint32_t dst = smem_u32(smem + xs * S::kXStage);
+            const bool with_sums = !Q6 && (c & 1);
+            mbar_arrive_expect_tx(full + xs, boxes * height * (NX * 256 + (with_sums ? 32 : 0)));
+#pragma unroll 1
+            for (int q = 0; q < boxes; ++q) {
+              const int r = first + 32 * q;
+              tma_load_2d(dst + q * 32 * 128, mx, c * 256, r, full + xs);
+              tma_load_2d(dst + q * 32 * 128 + S::kBox, mx, c * 256 + 128, r, full + xs);
+              if (NX == 2) {
+                tma_load_2d(dst + q * 32 * 128 + S::kPart, mx, c * 256, int(a.rows) + r, full + xs);
+                tma_load_2d(dst + q * 32 * 128 + S::kPart + S::kBox, mx, c * 256 + 128, int(a.rows) + r, full + xs);
+              }
+              if (with_sums) tma_load_2d(dst + NX * S::kPart + q * 32 * 32, ms, (c >> 1) * 32, r, full + xs);
+            }
+          }
+          if (++xs == S::kXStages) { xs = 0; ph ^= 1; }
+        }
+      }
+      if (!ok) {                         // after a timeout the copies in flight land before the block ends
+        abort_flag = 1;
+        for (int i = 0; i < used; ++i) pipe_wait(full + i, i < xs ? ph ^ 1 : ph, a.status);
+      }
+    } else if (warp == 2) {
+      // ---- TMA, packed weights: on their own, as far ahead as the ring allows ------------------------------------------------
+      const uint32_t go = elect_lane();
+      int ws = 0, used = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+        const GgTile t = locate(tile);
+        const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
+        const int wrow = t.group * a.n + t.n0;
+#pragma unroll 1
+        for (int b = 0; b < a.nblk; ++b) {
+          if (used == S::kRawStages) ok = warp_wait(wempty + ws, ph, a.status);
+          else ++used;
           if (!ok) break;
           if (go) {
             mbar_arrive_expect_tx(wfull + ws, S::kRawStage);
             tma_load_2d(smem_u32(smem + S::kOffRaw + ws * S::kRawStage), mw, b * S::kRawBytes, wrow, wfull + ws);
           }
-          if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            if (used_x == S::kXStages) ok = warp_wait(empty + xs, xph, a.status);
-            else ++used_x;
-            if (!ok) break;
-            if (go) {
-              const uint32_t dst = smem_u32(smem + xs * S::kXStage);
-              const int col = (b * 2 + c) * 256;
-              const bool with_sums = !Q6 && c;
-              mbar_arrive_expect_tx(full + xs, boxes * height * (NX * 256 + (with_sums ? 32 : 0)));
-#pragma unroll 1
-              for (int q = 0; q < boxes; ++q) {
-                const int r = first + 32 * q;
-                tma_load_2d(dst + q * 32 * 128, mx, col, r, full + xs);
-                tma_load_2d(dst + q * 32 * 128 + S::kBox, mx, col + 128, r, full + xs);
-                if (NX == 2) {
-                  tma_load_2d(dst + q * 32 * 128 + S::kPart, mx, col, int(a.rows) + r, full + xs);
-                  tma_load_2d(dst + q * 32 * 128 + S::kPart + S::kBox, mx, col + 128, int(a.rows) + r, full + xs);
-                }
-                if (with_sums) tma_load_2d(dst + NX * S::kPart + q * 32 * 32, ms, b * 32, r, full + xs);
-              }
-            }
-            if (++xs == S::kXStages) { xs = 0; xph ^= 1; }
-          }
+          if (++ws == S::kRawStages) { ws = 0; ph ^= 1; }
         }
       }
-      if (!ok) {                         // after a timeout the copies in flight land before the block ends
+      if (!ok) {
         abort_flag = 1;
-        for (int i = 0; i < used_w; ++i) pipe_wait(wfull + i, i < ws ? wph ^ 1 : wph, a.status);
-        for (int i = 0; i < used_x; ++i) pipe_wait(full + i, i < xs ? xph ^ 1 : xph, a.status);
+        for (int i = 0; i < used; ++i) pipe_wait(wfull + i, i < ws ? ph ^ 1 : ph, a.status);
       }
     } else if (warp == 1) {
       // ---- MMA ---------------------------------------------------------------------------------------------------------

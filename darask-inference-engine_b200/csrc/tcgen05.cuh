@@ -105,40 +105,51 @@ DEVI void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
 #undef DMOE_R16
 #undef DMOE_R4
 
-// Bounded wait for a phase. A probe of a phase that is over costs 43 cycles (74 with a suspension limit), so the first one goes
-// without; then each probe suspends the thread for up to 2 us, and a million of them end the wait and set the status bit.
-DEVI bool pipe_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
-  const uint32_t addr = smem_u32(bar);
+// Bounded waits for a phase. What a wait costs when the phase is over already is most of what these kernels' single warps spend:
+// one probe without a branch around it (70 cycles beside twenty busy warps; a probe inside a loop of its own 160, a broadcast from
+// one lane 250). After that each probe suspends the thread for up to 2 us, and a million of them set the status bit.
+DEVI uint32_t phase_over(uint32_t addr, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(addr), "r"(parity)
       : "memory");
-  if (ok) return true;
-  // (the loop is one statement so that the compiler does not unroll, rotate or duplicate it)
+  return ok;
+}
+DEVI uint32_t phase_probe(uint32_t addr, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .u32 i;\n\t"
-      "mov.u32 i, 1000000;\n\t"
-      "probe:\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
-      "@p bra over;\n\t"
-      "sub.u32 i, i, 1;\n\t"
-      "setp.ne.u32 p, i, 0;\n\t"
-      "@p bra probe;\n\t"
-      "over:\n\t"
-      "min.u32 %0, i, 1;\n\t}"
+      "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(addr), "r"(parity)
       : "memory");
-  if (!ok) atomicOr(status, kStatusWaitTimeout);
-  return ok != 0;
+  return ok;
 }
-// The same for a whole warp, every lane probing (cheaper than one lane and a broadcast); the lanes stay together, so that loops
-// around it stay on the uniform datapath, where the operands of tcgen05.mma and of the tensor copies live.
-DEVI bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* status) { return __all_sync(0xffffffffu, pipe_wait(bar, parity, status)); }
+DEVI bool pipe_wait(uint64_t* bar, uint32_t parity, unsigned* status) {      // one thread
+  const uint32_t addr = smem_u32(bar);
+  if (__builtin_expect(phase_over(addr, parity), 1)) return true;
+#pragma unroll 1
+  for (uint32_t i = 0; i < 1000000u; ++i)
+    if (phase_probe(addr, parity)) return true;
+  atomicOr(status, kStatusWaitTimeout);
+  return false;
+}
+// A whole warp; the vote keeps the lanes together, so that loops around the wait stay on the uniform datapath, where the operands of
+// tcgen05.mma and of the tensor copies live.
+DEVI bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* status) {
+  const uint32_t addr = smem_u32(bar);
+  if (__builtin_expect(__all_sync(0xffffffffu, phase_over(addr, parity)), 1)) return true;
+#pragma unroll 1
+  for (uint32_t i = 0; i < 1000000u; ++i)
+    if (__all_sync(0xffffffffu, phase_probe(addr, parity))) return true;
+  if ((threadIdx.x & 31) == 0) atomicOr(status, kStatusWaitTimeout);
+  return false;
+}
 DEVI uint32_t elect_lane() {
   uint32_t one;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
