@@ -58,8 +58,9 @@ struct GgShape {
   static constexpr int kOffD = kOffRaw + kRawStages * kRawStage;
   static constexpr int kOffEnds = kOffD + 4 * 128 * 8;
   static constexpr int kSmem = 1024 + kOffD + kTail;
-  // TMEM columns: two main buffers, the min products, the weights, their second terms
-  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + (Q6 ? 0 : NT), kColA2 = kColA + 64 * kSets;
+  // TMEM columns: two main buffers, one or two of min products, the weights, their second terms
+  static constexpr int kMinBufs = Q6 ? 0 : NT == 128 ? 1 : 2;
+  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSets;
   static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSets : 0) <= 512, "rings must fit");
 };
 
@@ -165,6 +166,17 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
 // ---- expanders ---------------------------------------------------------------------------------------------------------
 DEVI __half2 as_half2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 DEVI uint32_t as_word(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// (a & b) | c as one instruction: with both constants written out the compiler takes two, and the integer pipe paces the expanders
+DEVI uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+DEVI uint32_t opaque(uint32_t v) {       // a constant that stays in a register
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // byte `i` of w as an integer in both halves (1024 + byte is exact in f16, so is the difference)
 template <int I>
 DEVI __half2 byte_half2(uint32_t w, float offset) {
@@ -375,16 +387,16 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           // TMEM slots of the two steps
           const uint32_t a0 = slot, a1 = slot + 1 == S::kSets ? 0u : slot + 1;
           slot = a1 + 1 == S::kSets ? 0u : a1 + 1;
-          // the buffer is free: Q6_K waits for the block before the last here; Q4_K waited for it in the last round
-          if (Q6 && wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+          // the buffers are free: the block before the last has been promoted (with one buffer of mins the last round waited for it)
+          if (S::kMinBufs != 1 && wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
           ok = warp_wait(full + x0, ph, a.status) && ok;
           if (!ok) break;
           tmem_fence_after();
 #pragma unroll
           for (int step = 0; step < 2; ++step) {
             if (step == 1) {
-              // the accumulator of the mins is free once the last block has been promoted
-              if (!Q6 && wi >= 1) ok = warp_wait(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status);
+              // one buffer of mins: it is free once the last block has been promoted
+              if (S::kMinBufs == 1 && wi >= 1) ok = warp_wait(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status);
               ok = warp_wait(full + x0 + 1, ph, a.status) && ok;
               if (!ok) break;
               tmem_fence_after();
@@ -399,7 +411,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
               if (NA == 2) umma_f16_ts(d, a2 + q * 8, dx + box, idesc, 1u, go);
             }
             if (!Q6 && step == 1)                            // sums times mins
-              umma_f16_ss(tmem_min, dmin + (S::kMins == 2 ? buf * (4096u >> 4) : 0u), dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);
+              umma_f16_ss(tmem_min + (S::kMinBufs == 2 ? buf * NT : 0u), dmin + (S::kMins == 2 ? buf * (4096u >> 4) : 0u), dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);
             umma_commit_if(empty + x0 + step, go);
           }
           if (kOwnDone && ok) umma_commit_if(done + buf, go);
@@ -412,6 +424,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     // ---- expanders: four warps, one for each quarter of the TMEM lanes, take every kSets-th step --------------------------------
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + set * 64;       // the set's TMEM slot
+    const uint32_t magic = opaque(0x64006400u);      // 1024 in both halves
     int ws = 0, turn = 0;                // raw stage, set whose step comes next
     uint32_t wph = 0, wi = 0;
     bool ok = true;
@@ -472,10 +485,10 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const uint32_t w = wd[q], u = w >> 8;
-              lo[2 * q] = as_word(__hfma2(as_half2((w & 0x000f000fu) | 0x64006400u), s0, k0));
-              lo[2 * q + 1] = as_word(__hfma2(as_half2((u & 0x000f000fu) | 0x64006400u), s0, k0));
-              hi[2 * q] = as_word(__hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), s1d, k1));
-              hi[2 * q + 1] = as_word(__hfma2(as_half2((u & 0x00f000f0u) | 0x64006400u), s1d, k1));
+              lo[2 * q] = as_word(__hfma2(as_half2(and_or(w, 0x000f000fu, magic)), s0, k0));
+              lo[2 * q + 1] = as_word(__hfma2(as_half2(and_or(u, 0x000f000fu, magic)), s0, k0));
+              hi[2 * q] = as_word(__hfma2(as_half2(and_or(w, 0x00f000f0u, magic)), s1d, k1));
+              hi[2 * q + 1] = as_word(__hfma2(as_half2(and_or(u, 0x00f000f0u, magic)), s1d, k1));
             }
             tmem_st16(tmem_a + dst, lo);
             tmem_st16(tmem_a + dst + 16, hi);
@@ -496,7 +509,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
                 const uint32_t w = wd[q] >> down, h = hq[q] << up;
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {            // even and odd bytes
-                  const __half2 z = __hsub2(as_half2(((o ? w >> 8 : w) & 0x000f000fu) | ((o ? h >> 8 : h) & 0x00300030u) | 0x64006400u),
+                  const __half2 z = __hsub2(as_half2(and_or(o ? h >> 8 : h, 0x00300030u, and_or(o ? w >> 8 : w, 0x000f000fu, magic))),
                                             __float2half2_rn(1056.f));                    // q - 32
                   const __half2 p = __hmul2(z, sc);
                   v[2 * q + o] = as_word(p);
@@ -560,7 +573,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dd, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
             if (!Q6) {
-              tmem_ld32(tmem_min + tl + c, v);
+              tmem_ld32(tmem_min + tl + (S::kMinBufs == 2 ? buf * NT : 0u) + c, v);
 #pragma unroll
               for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dm, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
             }
