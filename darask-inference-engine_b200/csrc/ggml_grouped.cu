@@ -32,7 +32,7 @@ static GroupedWs carve(void* base, long long rows, int k, int parts) {
 template <bool Q6, int NT, int NX, int NA, typename OUT>
 static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
   using S = GgShape<Q6, NT, NX, NA>;
-  static_assert(S::kSmem + 5 * 1024 - 1024 <= kSmemBudget, "rings must fit one block");
+  static_assert(S::kSmem + 3 * 1024 <= kSmemBudget, "rings and 3 KB of barriers and scales must fit one block");
   static bool configured[64] = {};      // the opt-in is per device and per kernel
   const int dev = current_device_slot();
   if (dev < 0) return cudaErrorInvalidDevice;
@@ -92,7 +92,7 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   const GroupedWs ws = carve(d->workspace, d->rows, d->k, parts);
   GgRowsArgs r = {};
   r.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
-  r.rows = d->rows; r.x_rows = d->x_rows; r.assignments = d->assignments; r.topk = d->topk; r.parts = nx; r.sums = !q6;
+  r.rows = d->rows; r.x_rows = d->x_rows; r.assignments = d->assignments; r.topk = d->topk;
   r.planes = ws.planes; r.sum = ws.sum; r.scale = ws.scale;
   const unsigned long long wrows = (unsigned long long)d->groups * d->n, wcols = (unsigned long long)nblk * (q6 ? 208 : 144);
   const unsigned box = q6 ? 208 : 144;
@@ -104,11 +104,16 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
       !byte_map(m + 4, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !byte_map(m + 5, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 128, 32, CU_TENSOR_MAP_SWIZZLE_32B))
     return cudaErrorInvalidValue;
-  if ((e = launch_pdl(ggml_rows_kernel, dim3(unsigned(d->rows)), dim3(kGgRowThreads), 0, st, r))) return e;
+  const auto rows_kernel = nx == 2 ? (q6 ? ggml_rows_kernel<true, false> : ggml_rows_kernel<true, true>)
+                                   : (q6 ? ggml_rows_kernel<false, false> : ggml_rows_kernel<false, true>);
+  if ((e = launch_pdl(rows_kernel, dim3(unsigned(d->rows)), dim3(kGgRowThreads), 0, st, r))) return e;
   GgArgs a = {};
   a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);
-  a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo; a.status = static_cast<unsigned*>(status);
+  a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo;
+  const size_t ob = row_type_bytes(d->out_ty);
+  a.aligned = reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->ldo * ob % 16 == 0 && (!d->w_up || d->n * ob % 16 == 0);
+  a.status = static_cast<unsigned*>(status);
   // narrow tiles while the groups have few rows on average: the weights' bytes pace the product then
   const bool narrow = d->rows <= 32ll * d->groups;
   if (q6) return narrow ? launch_by_type<true, 32>(d->out_ty, nx, m, a, st) : launch_by_type<true, 128>(d->out_ty, nx, m, a, st);

@@ -32,6 +32,7 @@ struct GgArgs {
   const float* xscale;                                   // [rows] powers of two; negative: row(i) does not exist
   void* out;
   long long ldo;
+  int aligned;                                           // 16-byte pieces of the output's rows start on 16-byte boundaries
   unsigned* status;
 };
 
@@ -52,12 +53,14 @@ struct GgShape {
   static constexpr int kMins = Q6 ? 0 : kSets / 2;       // 128 rows x 32 bytes each
   static constexpr int kOffMin = kXStages * kXStage;
   static constexpr int kOffRaw = kOffMin + kMins * 4096;
-  static constexpr int kTail = 4 * 128 * 8 + (kGgMaxGroups + 4) * 4;
-  static constexpr int kFit = (kSmemBudget - 5 * 1024 - kOffRaw - kTail) / kRawStage;
+  static constexpr int kStore = 4 * 16 * 128;            // 4 warps x 16 output rows x 32 columns, up to 4 bytes each
+  static constexpr int kTail = kStore + 4 * 128 * 8 + (kGgMaxGroups + 4) * 4;
+  static constexpr int kFit = (kSmemBudget - 4 * 1024 - kOffRaw - kTail) / kRawStage;
   static constexpr int kRawStages = kFit < 8 ? kFit : 8;
-  static constexpr int kOffD = kOffRaw + kRawStages * kRawStage;
+  static constexpr int kOffStore = kOffRaw + kRawStages * kRawStage;
+  static constexpr int kOffD = kOffStore + kStore;
   static constexpr int kOffEnds = kOffD + 4 * 128 * 8;
-  static constexpr int kSmem = 1024 + kOffD + kTail;
+  static constexpr int kSmem = 1024 + kOffStore + kTail;
   // TMEM columns: two main buffers, one or two of min products, the weights, their second terms
   static constexpr int kMinBufs = Q6 ? 0 : NT == 128 ? 1 : 2;
   static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSets;
@@ -71,13 +74,31 @@ struct GgRowsArgs {
   RowSource src;
   long long rows, x_rows;
   const unsigned* assignments;
-  int topk, parts, sums;
+  int topk;
   __half* planes;                                        // [parts][rows][k]
   __half* sum;                                           // [rows][k / 256][16]: 8 high, 8 low
   float* scale;                                          // [rows]
 };
 constexpr int kGgRowThreads = 128;
-constexpr int kGgRowHeld = 8;                            // groups of four columns a thread keeps in registers (k <= 4096); longer rows are read twice
+constexpr int kGgRowHeld = 4;                            // groups of eight columns a thread keeps in registers (k <= 4096); longer rows are read twice
+DEVI void rows_load8(const RowSource& s, long long row, int c, float (&v)[8]) {
+  if (s.vec == 2 && s.ty != DARASK_GGML_F32 && !s.swiglu) {          // 16-byte aligned 16-bit rows: one load
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(s.x) + size_t(row) * size_t(s.ld) + c));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[2 * q] = s.ty == DARASK_GGML_F16 ? half_lo(w[q]) : __uint_as_float(w[q] << 16);
+      v[2 * q + 1] = s.ty == DARASK_GGML_F16 ? half_hi(w[q]) : __uint_as_float(w[q] & 0xffff0000u);
+    }
+    return;
+  }
+  float a[4], b[4];
+  row_source_load4(s, row, c, a);
+  row_source_load4(s, row, c + 4, b);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+}
+template <bool PARTS, bool SUMS>
 __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsArgs a) {
   __shared__ uint32_t red[kGgRowThreads / 32];
   pdl_wait();
@@ -87,24 +108,27 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   long long row = i;
   if (a.assignments) row = __ldg(a.assignments + i) / unsigned(a.topk);
   const bool exists = row < a.x_rows;
-  float held[kGgRowHeld][4];
+  float held[kGgRowHeld][8];
   uint32_t top = 0;
-  auto scan = [&](const float (&v)[4]) {
+  auto scan = [&](const float (&v)[8]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
+    for (int q = 0; q < 8; ++q) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
   };
 #pragma unroll
   for (int j = 0; j < kGgRowHeld; ++j) {
-    const int c = (j * kGgRowThreads + threadIdx.x) * 4;
-    held[j][0] = held[j][1] = held[j][2] = held[j][3] = 0.f;
-    if (exists && c < k) row_source_load4(a.src, row, c, held[j]);
+    const int c = (j * kGgRowThreads + threadIdx.x) * 8;
+    if (exists && c < k) rows_load8(a.src, row, c, held[j]);
+    else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) held[j][q] = 0.f;
+    }
   }
 #pragma unroll
   for (int j = 0; j < kGgRowHeld; ++j) scan(held[j]);
   if (exists)
-    for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 4; c < k; c += kGgRowThreads * 4) {
-      float v[4];
-      row_source_load4(a.src, row, c, v);
+    for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 8; c < k; c += kGgRowThreads * 8) {
+      float v[8];
+      rows_load8(a.src, row, c, v);
       scan(v);
     }
   top = __reduce_max_sync(0xffffffffu, top);
@@ -115,35 +139,36 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   // exponent of the largest magnitude (not below 2^-117: the factor stays finite), moved to 2^9
   const bool finite = top < 0x7f800000u;
   const int e = max(int(top >> 23) - 127, -117) - 9;
-  const float down = __uint_as_float(uint32_t(127 - e) << 23);
+  const bool live = exists && finite;
+  const float down = live ? __uint_as_float(uint32_t(127 - e) << 23) : 0.f;
   if (threadIdx.x == 0)
     a.scale[i] = !exists ? -1.f : top == 0u ? 1.f : finite ? __uint_as_float(uint32_t(127 + e) << 23) : __uint_as_float(0x7fffffffu);
-  const bool live = exists && finite;
-  auto put = [&](int c, float (&v)[4]) {
-    __half hi[4];
+  auto put = [&](int c, float (&v)[8]) {
+    uint32_t hi[4], lo[4];
     float s = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 8; ++q) {
       v[q] = live ? v[q] * down : 0.f;
-      hi[q] = __float2half_rn(v[q]);
       s += v[q];
     }
-    auto store = [&](__half* p, const __half (&h)[4]) {
-      const __half2 w0 = __halves2half2(h[0], h[2]), w1 = __halves2half2(h[1], h[3]);
-      *reinterpret_cast<uint2*>(p + size_t(i) * k + c) = make_uint2(*reinterpret_cast<const uint32_t*>(&w0), *reinterpret_cast<const uint32_t*>(&w1));
-    };
-    store(a.planes, hi);
-    if (a.parts > 1) {
-      __half lo[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) lo[q] = __float2half_rn(v[q] - __half2float(hi[q]));
-      store(a.planes + size_t(a.rows) * k, lo);
+    for (int q = 0; q < 4; ++q) {                        // columns 0 2 | 1 3 of each four
+      const float p0 = v[(q >> 1) * 4 + (q & 1)], p1 = v[(q >> 1) * 4 + (q & 1) + 2];
+      const __half2 h = __floats2half2_rn(p0, p1);
+      hi[q] = *reinterpret_cast<const uint32_t*>(&h);
+      if (PARTS) {
+        const float2 back = __half22float2(h);
+        const __half2 l = __floats2half2_rn(p0 - back.x, p1 - back.y);
+        lo[q] = *reinterpret_cast<const uint32_t*>(&l);
+      }
     }
-    if (a.sums) {                                        // k is a multiple of 256: groups of eight lanes are here or not as one
-      const unsigned mask = 0xffu << (threadIdx.x & 24);
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(mask, s, o);
-      if ((threadIdx.x & 7) == 0) {
+    *reinterpret_cast<uint4*>(a.planes + size_t(i) * k + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (PARTS) *reinterpret_cast<uint4*>(a.planes + (size_t(a.rows) + size_t(i)) * k + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (SUMS) {                                          // k is a multiple of 256: groups of four lanes are here or not as one
+      const unsigned mask = 0xfu << (threadIdx.x & 28);
+      s += __shfl_xor_sync(mask, s, 1);
+      s += __shfl_xor_sync(mask, s, 2);
+      if ((threadIdx.x & 3) == 0) {
         const __half h = __float2half_rn(s);
         __half* p = a.sum + (size_t(i) * (k / 256) + c / 256) * 16 + (c % 256) / 32;
         p[0] = h;
@@ -153,12 +178,14 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   };
 #pragma unroll
   for (int j = 0; j < kGgRowHeld; ++j) {
-    const int c = (j * kGgRowThreads + threadIdx.x) * 4;
+    const int c = (j * kGgRowThreads + threadIdx.x) * 8;
     if (c < k) put(c, held[j]);
   }
-  for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 4; c < k; c += kGgRowThreads * 4) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) row_source_load4(a.src, row, c, v);
+  for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 8; c < k; c += kGgRowThreads * 8) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = 0.f;
+    if (live) rows_load8(a.src, row, c, v);
     put(c, v);
   }
 }
@@ -216,7 +243,7 @@ DEVI uint64_t umma_desc_k32(uint32_t smem_addr) {
   return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(256 >> 4) << 32) | (1ull << 46) | (6ull << 61);
 }
 
-struct GgTile { int group, n0, mat, rows; long long first; };      // rows of the tile, its first dispatch row
+struct GgTile { int group = 0, n0, mat, rows; long long first; };  // rows of the tile, its first dispatch row
 
 template <typename T> DEVI T from_float(float v);
 template <> DEVI float from_float<float>(float v) { return v; }
@@ -284,33 +311,40 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   tmem_fence_after();
   const uint32_t tmem = tmem_slot, tmem_min = tmem + S::kColMin, tmem_a = tmem + S::kColA, tmem_a2 = tmem + S::kColA2;
   const int total = ends[a.groups];
-  auto locate = [&](int tile) {
-    int lo = 0, hi = a.groups;
-    while (lo < hi) { const int mid = (lo + hi) >> 1; if (tile < ends[mid]) hi = mid; else lo = mid + 1; }
-    const int local = tile - (lo ? ends[lo - 1] : 0);
-    GgTile t;
-    t.group = lo;
-    const int r = group_rows(lo, &t.first);
+  // a warp's tiles come in ascending order: the search for the group goes on from the last one
+  auto locate = [&](int tile, GgTile& t) {
+    int g = t.group;
+    while (tile >= ends[g]) ++g;
+    const int local = tile - (g ? ends[g - 1] : 0);
+    t.group = g;
+    const int r = group_rows(g, &t.first);
     // row tiles of equal height, a multiple of 16
-    const int tiles_m = (r + NT - 1) / NT, h = ((r + tiles_m - 1) / tiles_m + 15) / 16 * 16;
-    const int m = local % tiles_m, nt = local / tiles_m;
-    t.first += m * h;
-    t.rows = r - m * h < h ? r - m * h : h;
-    t.n0 = nt / a.mats * 128;
-    t.mat = nt % a.mats;
-    return t;
+    const int tiles_m = (r + NT - 1) / NT;
+    int m = 0, nt = local;
+    if (tiles_m > 1) {
+      const int h = ((r + tiles_m - 1) / tiles_m + 15) / 16 * 16;
+      nt = local / tiles_m;
+      m = local - nt * tiles_m;
+      t.first += m * h;
+      t.rows = r - m * h < h ? r - m * h : h;
+    } else {
+      t.rows = r;
+    }
+    t.n0 = (a.mats == 2 ? nt >> 1 : nt) * 128;
+    t.mat = a.mats == 2 ? nt & 1 : 0;
   };
 
   if (warp < 4) {
-    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
       // ---- TMA, rows of x ----------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
       int xs = 0, used = 0;              // stage; stages filled so far (up to the first round)
       uint32_t ph = 1;                   // parity of the "empty" phase
       bool ok = true;
+      GgTile t;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const GgTile t = locate(tile);
+        locate(tile, t);
         // rows of x in boxes of 32, or one box of 128
         const bool wide = NT == 128 && t.rows > 96;
         const CUtensorMap *mx = wide ? &map_x4 : &map_x, *ms = wide ? &map_sum4 : &map_sum;
@@ -349,8 +383,9 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       int ws = 0, used = 0;
       uint32_t ph = 1;
       bool ok = true;
+      GgTile t;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const GgTile t = locate(tile);
+        locate(tile, t);
         const CUtensorMap* mw = t.mat ? &map_w1 : &map_w0;
         const int wrow = t.group * a.n + t.n0;
 #pragma unroll 1
@@ -376,8 +411,9 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       const uint64_t dsum0 = umma_desc_k32(smem_u32(smem + NX * S::kPart));
       uint32_t wi = 0, slot = 0;
       bool ok = true;
+      GgTile t;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const GgTile t = locate(tile);
+        locate(tile, t);
         const uint32_t idesc = __shfl_sync(0xffffffffu, (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24), 0);
 #pragma unroll 1
         for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
@@ -420,7 +456,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       if (!ok) abort_flag = 1;
     }
   } else if (warp < 4 + 4 * S::kSets) {
-    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     // ---- expanders: four warps, one for each quarter of the TMEM lanes, take every kSets-th step --------------------------------
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + set * 64;       // the set's TMEM slot
@@ -428,8 +464,9 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     int ws = 0, turn = 0;                // raw stage, set whose step comes next
     uint32_t wph = 0, wi = 0;
     bool ok = true;
+    GgTile t;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-      const GgTile t = locate(tile);
+      locate(tile, t);
       const __half* dq = nullptr;        // Q6_K: the row's block scales
       float d_next = 0.f;
       if (Q6) {
@@ -541,8 +578,9 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     const uint32_t tl = uint32_t((warp - kFirst) * 32) << 16;
     uint32_t wi = 0;
     bool ok = true;
+    GgTile t;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-      const GgTile t = locate(tile);
+      locate(tile, t);
       // scales of the tile's rows
       float* scale = xsc[warp - kFirst];
       __syncwarp();
@@ -603,17 +641,37 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         }
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      const int col = t.n0 + row;
-      OUT* p = static_cast<OUT*>(a.out) + size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+      // 16 output rows at a time: this warp's 32 columns of them through shared memory, out in pieces of 16 bytes
+      constexpr int kPieces = sizeof(OUT) * 2;            // per row
+      OUT* mine = reinterpret_cast<OUT*>(smem + S::kOffStore + (warp - kFirst) * 16 * 128);
+      const int col = t.n0 + (warp - kFirst) * 32;
+      OUT* base = static_cast<OUT*>(a.out) + size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+      const bool whole = a.aligned && col + 32 <= a.n;
 #pragma unroll 1
       for (int c = 0; c < t.rows; c += 16) {
         uint32_t v[16];
         tmem_ld16(stage + c, v);
+        const float4* f = reinterpret_cast<const float4*>(scale + c);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          if (c + q < t.rows && col < a.n) *p = from_float<OUT>(__uint_as_float(v[q]) * scale[c + q]);
-          p += a.ldo;
+        for (int q = 0; q < 4; ++q) {
+          const float4 s4 = f[q];
+          mine[(4 * q) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q]) * s4.x);
+          mine[(4 * q + 1) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q + 1]) * s4.y);
+          mine[(4 * q + 2) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q + 2]) * s4.z);
+          mine[(4 * q + 3) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q + 3]) * s4.w);
         }
+        __syncwarp();
+        if (whole) {
+#pragma unroll
+          for (int i = lane; i < 16 * kPieces; i += 32) {
+            const int r = i / kPieces, part = i % kPieces;
+            if (c + r < t.rows)
+              reinterpret_cast<uint4*>(base + size_t(c + r) * size_t(a.ldo))[part] = reinterpret_cast<const uint4*>(mine + r * 32)[part];
+          }
+        } else if (col + lane < a.n) {
+          for (int r = 0; r < 16 && c + r < t.rows; ++r) base[size_t(c + r) * size_t(a.ldo) + lane] = mine[r * 32 + lane];
+        }
+        __syncwarp();
       }
       tmem_fence_before();
       __syncwarp();

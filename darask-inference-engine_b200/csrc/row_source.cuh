@@ -12,13 +12,14 @@ struct RowSource {
   int ty;                // DARASK_GGML_F32 / F16 / BF16
   int k;                 // columns of the operand; swiglu: column c of the gate half, k + c of the up half
   int swiglu;
-  int vec;               // every run of four elements that starts at a multiple of four columns can be loaded as one word
+  int vec;               // 1: four elements from a multiple of four columns can be loaded as one word; 2: eight 16-bit ones too
 };
 
 // The four-wide loads need the base and the row stride (and, for the up half, k) on a boundary of four elements.
 inline int row_source_vec(const void* x, int ty, long long ld, int k, int swiglu) {
-  const unsigned step = ty == DARASK_GGML_F32 ? 16 : 8;
-  return reinterpret_cast<uintptr_t>(x) % step == 0 && ld % 4 == 0 && (!swiglu || k % 4 == 0);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+  if (at % (ty == DARASK_GGML_F32 ? 16 : 8) || ld % 4 || (swiglu && k % 4)) return 0;
+  return ty != DARASK_GGML_F32 && at % 16 == 0 && ld % 8 == 0 ? 2 : 1;
 }
 inline size_t row_type_bytes(int ty) { return ty == DARASK_GGML_F32 ? 4 : ty == DARASK_GGML_F16 || ty == DARASK_GGML_BF16 ? 2 : 0; }
 
