@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
           const float scale = fp8_group(v[u], &codes);
           // 128-byte rows, 16-byte pieces swizzled by the row in its group of eight
           *reinterpret_cast<uint32_t*>(xres + size_t(b) * 2048 + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = codes;
-          if (lane == 0) factors[b * 16 + row] = row < a.m ? scale * __ldg(a.ws + size_t(n0 / 128) * size_t(a.ld_ws) + kb0 + b) : 0.f;
+          if (lane == 0) factors[b * 16 + row] = row < a.m ? scale * __ldcg(a.ws + size_t(n0 / 128) * size_t(a.ld_ws) + kb0 + b) : 0.f;
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
 #pragma unroll
         for (int j = 0; j < NT * kFsGroup / 64; ++j) {             // element = (row, block of k): eight neighbours share a row
           const int e = j * 64 + ft, row = e / kFsGroup, b = b0 + e % kFsGroup;
-          v[j] = t0 + row < a.m && b < kbs ? __ldg(a.xs + size_t(t0 + row) * size_t(a.ld_xs) + kb0 + b) * __ldg(ws + b) : 0.f;
+          v[j] = t0 + row < a.m && b < kbs ? __ldcg(a.xs + size_t(t0 + row) * size_t(a.ld_xs) + kb0 + b) * __ldcg(ws + b) : 0.f;
         }
         int ok = 1;
         if (g >= 2 && lane == 0) ok = pipe_wait(fempty + slot, ((g >> 1) & 1) ^ 1, a.status) ? 1 : 0;

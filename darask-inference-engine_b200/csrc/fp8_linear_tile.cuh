@@ -132,11 +132,11 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
 #pragma unroll
           for (int j = 0; j < 128 * kFtGroup / 64; ++j) {          // eight neighbouring threads share a row
             const int row = r0 + j * 8 + ft / 8, b = b0 + ft % 8;
-            v[j] = row < a.m && b < a.kb ? __ldg(a.xs + size_t(row) * size_t(a.ld_xs) + b) : 0.f;
+            v[j] = row < a.m && b < a.kb ? __ldcg(a.xs + size_t(row) * size_t(a.ld_xs) + b) : 0.f;
           }
           float w = 0.f;
           if (ft < 2 * kFtGroup && (nb + (ft & 1)) * 128 < a.n && b0 + ft / 2 < a.kb)
-            w = __ldg(a.ws + size_t(nb + (ft & 1)) * size_t(a.ld_ws) + b0 + ft / 2);
+            w = __ldcg(a.ws + size_t(nb + (ft & 1)) * size_t(a.ld_ws) + b0 + ft / 2);
           int ok = 1;
           if (fg >= 2 && lane == 0) ok = pipe_wait(fempty + slot, ((fg >> 1) & 1) ^ 1, a.status) ? 1 : 0;
           ok = __shfl_sync(0xffffffffu, ok, 0);

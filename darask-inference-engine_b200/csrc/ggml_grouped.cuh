@@ -39,21 +39,27 @@ struct GgArgs {
 // NT: rows of x per tile, NX: f16 parts of a row of x, NA: f16 terms of a Q6_K integer. A step is 128 columns of k.
 template <bool Q6, int NT, int NX, int NA>
 struct GgShape {
-  // Expander sets of four warps; set e has every SETS-th step, and TMEM holds the weights of SETS steps. 128 rows leave TMEM for two;
-  // with 32 rows the weights pace everything and more sets hide their latencies from each other.
-  static constexpr int kSets = NT == 128 ? 2 : NA == 2 ? 3 : 4;
-  static constexpr int kThreads = 128 * (2 + kSets);
+  // TMEM holds the weights of kSlots steps. Few rows: one set of four expander warps per slot, the sets hide their latencies from
+  // each other. Many rows leave TMEM for two slots, which two sets fill together (half a step each): a slot is filled, handed over,
+  // multiplied and handed back in turn, and that turn sets the pace.
+  static constexpr bool kWide = NT > 32;
+  static constexpr int kSlots = kWide ? 2 : NA == 2 ? 3 : 4, kSets = kWide ? 2 : kSlots;
+  static constexpr int kPromote = kWide ? 8 : 4;         // warps that promote and store: two per quarter of the weight rows, half of x each
+  static constexpr int kThreads = 128 * (1 + kSets) + 32 * kPromote;
+  // wide: registers of the roles, the expanders and the promotion; their sum is what the block is launched with (640 x 96)
+  static constexpr int kRegRoles = 48, kRegExpand = 88, kRegPromote = 128;
+  static_assert(kRegRoles + 2 * kRegExpand + 2 * kRegPromote <= 5 * 96, "setmaxnreg draws on the launch's registers");
   static constexpr int kRawBytes = Q6 ? 208 : 144;
   static constexpr int kRawStage = 128 * kRawBytes;
   static constexpr int kBox = NT * 128;                  // NT rows x 64 columns of f16
   static constexpr int kPart = 2 * kBox;                 // one part of a step
   static constexpr int kSums = Q6 ? 0 : NT * 32;         // NT rows x 16 f16: the sums of eight groups of 32 columns, high and low parts
   static constexpr int kXStage = NX * kPart + kSums;     // Q4_K: the sums travel with the second step of a block
-  static constexpr int kXStages = NT == 128 && NX == 2 ? 2 : 4;
-  static constexpr int kMins = Q6 ? 0 : kSets / 2;       // 128 rows x 32 bytes each
+  static constexpr int kXStages = kWide && NX == 2 ? 2 : 4;
+  static constexpr int kMins = Q6 ? 0 : kSlots / 2;       // 128 rows x 32 bytes each
   static constexpr int kOffMin = kXStages * kXStage;
   static constexpr int kOffRaw = kOffMin + kMins * 4096;
-  static constexpr int kStore = 4 * 16 * 128;            // 4 warps x 16 output rows x 32 columns, up to 4 bytes each
+  static constexpr int kStore = kPromote * 1024;         // per warp 16 output rows x 32 columns (8 rows of float32)
   static constexpr int kTail = kStore + 4 * 128 * 8 + (kGgMaxGroups + 4) * 4;
   static constexpr int kFit = (kSmemBudget - 4 * 1024 - kOffRaw - kTail) / kRawStage;
   static constexpr int kRawStages = kFit < 8 ? kFit : 8;
@@ -62,9 +68,9 @@ struct GgShape {
   static constexpr int kOffEnds = kOffD + 4 * 128 * 8;
   static constexpr int kSmem = 1024 + kOffStore + kTail;
   // TMEM columns: two main buffers, one or two of min products, the weights, their second terms
-  static constexpr int kMinBufs = Q6 ? 0 : NT == 128 ? 1 : 2;
-  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSets;
-  static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSets : 0) <= 512, "rings must fit");
+  static constexpr int kMinBufs = Q6 ? 0 : kWide ? 1 : 2;
+  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSlots;
+  static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSlots : 0) <= 512, "rings must fit");
 };
 
 // ---- rows of x -> f16 parts --------------------------------------------------------------------------------------------
@@ -83,7 +89,7 @@ constexpr int kGgRowThreads = 128;
 constexpr int kGgRowHeld = 4;                            // groups of eight columns a thread keeps in registers (k <= 4096); longer rows are read twice
 DEVI void rows_load8(const RowSource& s, long long row, int c, float (&v)[8]) {
   if (s.vec == 2 && s.ty != DARASK_GGML_F32 && !s.swiglu) {          // 16-byte aligned 16-bit rows: one load
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(s.x) + size_t(row) * size_t(s.ld) + c));
+    const uint4 u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(s.x) + size_t(row) * size_t(s.ld) + c));
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -106,7 +112,7 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   const long long i = blockIdx.x;
   const int k = a.src.k;
   long long row = i;
-  if (a.assignments) row = __ldg(a.assignments + i) / unsigned(a.topk);
+  if (a.assignments) row = __ldcg(a.assignments + i) / unsigned(a.topk);
   const bool exists = row < a.x_rows;
   float held[kGgRowHeld][8];
   uint32_t top = 0;
@@ -260,22 +266,23 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
   int* ends = reinterpret_cast<int*>(smem + S::kOffEnds);                   // [groups + 1] cumulative tile counts
-  // A step (128 columns of k) has one "full" barrier, on which its tile of x and its four expander warps count, and one "empty"
-  // barrier, on which the tensor core reports it read: the loader, the expanders (kSets steps on) and, at the end of a block of
+  // A step (128 columns of k) has one "full" barrier, on which its tile of x and its expander warps count, and one "empty"
+  // barrier, on which the tensor core reports it read: the loader, the expanders (kSlots steps on) and, at the end of a block of
   // 256 columns, the promotion all wait for that one. Waits and commits are what the MMA warp spends its time on.
   // With two stages and nothing but the buffers between them (Q6_K) the tensor core could report the next block before a late warp
   // has looked for this one, so the promotion has barriers of its own there.
   constexpr bool kOwnDone = Q6 && S::kXStages == 2;
-  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], full[S::kXStages], empty[S::kXStages], tempty[2], done[2];
+  __shared__ uint64_t wfull[S::kRawStages], wempty[S::kRawStages], full[S::kXStages], empty[S::kXStages], tempty[2], done[2], mfree;
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float xsc[4][NT];
+  __shared__ __align__(16) float xsc[S::kPromote][NT / (S::kPromote / 4)];
   __shared__ volatile int abort_flag;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < S::kRawStages; ++s) { mbar_init(wfull + s, 1); mbar_init(wempty + s, 8); }
-    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, 5); mbar_init(empty + s, 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(tempty + s, 4); mbar_init(done + s, 1); }
+    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, S::kWide ? 9 : 5); mbar_init(empty + s, 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(tempty + s, S::kPromote); mbar_init(done + s, 1); }
+    mbar_init(&mfree, S::kPromote);
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc<512>(&tmem_slot);
@@ -335,7 +342,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   };
 
   if (warp < 4) {
-    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (S::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegRoles));
     if (warp == 0) {
       // ---- TMA, rows of x ----------------------------------------------------------------------------------------------
       const uint32_t go = elect_lane();
@@ -346,7 +353,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
         locate(tile, t);
         // rows of x in boxes of 32, or one box of 128
-        const bool wide = NT == 128 && t.rows > 96;
+        const bool wide = S::kWide && t.rows > 96;
         const CUtensorMap *mx = wide ? &map_x4 : &map_x, *ms = wide ? &map_sum4 : &map_sum;
         const int boxes = wide ? 1 : (t.rows + 31) / 32, height = wide ? 128 : 32, first = int(t.first);
 #pragma unroll 1
@@ -421,18 +428,18 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           // stage of the first step and its parity: two or four stages
           const uint32_t x0 = S::kXStages == 4 ? buf * 2 : 0u, ph = S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1;
           // TMEM slots of the two steps
-          const uint32_t a0 = slot, a1 = slot + 1 == S::kSets ? 0u : slot + 1;
-          slot = a1 + 1 == S::kSets ? 0u : a1 + 1;
-          // the buffers are free: the block before the last has been promoted (with one buffer of mins the last round waited for it)
-          if (S::kMinBufs != 1 && wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+          const uint32_t a0 = slot, a1 = slot + 1 == S::kSlots ? 0u : slot + 1;
+          slot = a1 + 1 == S::kSlots ? 0u : a1 + 1;
+          // the buffers are free: the block before the last has been promoted
+          if (wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
           ok = warp_wait(full + x0, ph, a.status) && ok;
           if (!ok) break;
           tmem_fence_after();
 #pragma unroll
           for (int step = 0; step < 2; ++step) {
             if (step == 1) {
-              // one buffer of mins: it is free once the last block has been promoted
-              if (S::kMinBufs == 1 && wi >= 1) ok = warp_wait(tempty + (buf ^ 1), ((wi - 1) >> 1) & 1, a.status);
+              // one buffer of mins: the promotion of the last block has read it
+              if (S::kMinBufs == 1 && wi >= 1) ok = warp_wait(&mfree, (wi - 1) & 1, a.status);
               ok = warp_wait(full + x0 + 1, ph, a.status) && ok;
               if (!ok) break;
               tmem_fence_after();
@@ -456,10 +463,10 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       if (!ok) abort_flag = 1;
     }
   } else if (warp < 4 + 4 * S::kSets) {
-    if (NT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (S::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegExpand));
     // ---- expanders: four warps, one for each quarter of the TMEM lanes, take every kSets-th step --------------------------------
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + set * 64;       // the set's TMEM slot
+    const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + (S::kWide ? 0 : set * 64);       // narrow: the set's TMEM slot
     const uint32_t magic = opaque(0x64006400u);      // 1024 in both halves
     int ws = 0, turn = 0;                // raw stage, set whose step comes next
     uint32_t wph = 0, wi = 0;
@@ -472,30 +479,32 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       if (Q6) {
         const int r = t.n0 + row < a.n ? t.n0 + row : a.n - 1;
         dq = reinterpret_cast<const __half*>(a.w[t.mat] + (size_t(t.group) * a.n + r) * a.row_bytes + size_t(a.nblk) * 208);
-        d_next = __half2float(__ldg(dq));
+        d_next = __half2float(__ldcg(dq));
       }
 #pragma unroll 1
       for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
         const float d_now = d_next;
-        if (Q6 && b + 1 < a.nblk) d_next = __half2float(__ldg(dq + b + 1));
+        if (Q6 && b + 1 < a.nblk) d_next = __half2float(__ldcg(dq + b + 1));
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {                     // the block's two steps
-          const bool mine = turn == set;
-          if (++turn == S::kSets) turn = 0;
-          if (!mine) continue;
+          if (!S::kWide) {
+            const bool mine = turn == set;
+            if (++turn == S::kSets) turn = 0;
+            if (!mine) continue;
+          }
           ok = warp_wait(wfull + ws, wph, a.status);
           const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
           // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
           const uint4 head = lds128(raw + (Q6 ? 192 : 0));
-          // the TMEM slot is free when the step kSets before has been read
-          const uint32_t ps = 2 * wi + h - S::kSets;
-          if (2 * wi + h >= uint32_t(S::kSets)) ok = warp_wait(empty + ps % S::kXStages, (ps / S::kXStages) & 1, a.status) && ok;
+          // the TMEM slot is free when the step kSlots before has been read
+          const uint32_t ps = 2 * wi + h - S::kSlots;
+          if (2 * wi + h >= uint32_t(S::kSlots)) ok = warp_wait(empty + ps % S::kXStages, (ps / S::kXStages) & 1, a.status) && ok;
           if (!ok) break;
           tmem_fence_after();
-          if (h == 0) {
+          if (h == 0 && (!S::kWide || set == 0)) {
             const __half2 dd = as_half2(head.x);
             dring[(wi & 3) * 128 + row] = Q6 ? make_float2(d_now, 0.f) : make_float2(__low2float(dd), -__high2float(dd));
-          } else if (!Q6) {
+          } else if (!Q6 && h == 1 && (!S::kWide || set == 1)) {
             // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
             const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
             auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
@@ -508,8 +517,8 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           // Q4_K: the four scales of the step; Q6_K: the step is one half of the block
           const uint32_t scales = h == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
 #pragma unroll 1
-          for (int cc = 0; cc < 2; ++cc) {                // 64 columns
-            const uint32_t dst = tl + cc * 32;
+          for (int cc = S::kWide ? set : 0; cc < (S::kWide ? set + 1 : 2); ++cc) {       // 64 columns
+            const uint32_t dst = tl + (S::kWide ? h * 64 : 0) + cc * 32;
             const uint32_t at = raw + (Q6 ? 128 + h * 32 : 16 + (h * 2 + cc) * 32);
             const uint4 w0 = lds128(at), w1 = lds128(at + 16);        // Q4_K: codes; Q6_K: upper bits
             const uint32_t scw = scales >> (16 * cc);
@@ -563,7 +572,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(full + (2 * wi + h) % S::kXStages);
-            mbar_arrive(wempty + ws);
+            if (!S::kWide || h == 1) mbar_arrive(wempty + ws);
           }
         }
         if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
@@ -571,30 +580,30 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     }
     if (!ok) abort_flag = 1;
   } else {
-    if (NT == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if (S::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kRegPromote));
     // ---- promotion and store ---------------------------------------------------------------------------------------------
-    constexpr int kFirst = 4 + 4 * S::kSets;
-    const int row = (warp - kFirst) * 32 + lane;
-    const uint32_t tl = uint32_t((warp - kFirst) * 32) << 16;
+    constexpr int kFirst = 4 + 4 * S::kSets, kHalf = NT / (S::kPromote / 4);       // rows of x per warp
+    const int quarter = warp & 3, row = quarter * 32 + lane, c0 = ((warp - kFirst) >> 2) * kHalf;
+    const uint32_t tl = (uint32_t(quarter * 32) << 16) + c0;
+    float* scale = xsc[warp - kFirst];
     uint32_t wi = 0;
     bool ok = true;
     GgTile t;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
       locate(tile, t);
-      // scales of the tile's rows
-      float* scale = xsc[warp - kFirst];
+      const int rows = min(t.rows - c0, kHalf);            // of this warp's; may be none
       __syncwarp();
 #pragma unroll
-      for (int q = 0; q < NT / 32; ++q) {
+      for (int q = 0; q < kHalf / 32; ++q) {
         const int r = q * 32 + lane;
-        const float v = r < t.rows ? __ldg(a.xscale + t.first + r) : 0.f;
-        if (v < 0.f && warp == kFirst) atomicOr(a.status, kStatusBadRoute);
+        const float v = r < rows ? __ldcg(a.xscale + t.first + c0 + r) : 0.f;
+        if (v < 0.f && quarter == 0) atomicOr(a.status, kStatusBadRoute);
         scale[r] = fabsf(v);
       }
       __syncwarp();
-      unsigned long long acc[NT / 2];                    // pairs of float32 sums
+      unsigned long long acc[kHalf / 2];                   // pairs of float32 sums
 #pragma unroll
-      for (int c = 0; c < NT / 2; ++c) acc[c] = 0ull;
+      for (int c = 0; c < kHalf / 2; ++c) acc[c] = 0ull;
 #pragma unroll 1
       for (int b = 0; b < a.nblk; ++b, ++wi) {
         const uint32_t buf = wi & 1;
@@ -602,21 +611,27 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (!warp_wait(bar, kOwnDone || S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1, a.status)) { ok = false; break; }
         tmem_fence_after();
         const float2 d = dring[(wi & 3) * 128 + row];     // {d, -dmin}
-        const unsigned long long dd = pack2(d.x, d.x), dm = pack2(d.y, d.y);
+        auto add = [&](uint32_t from, float f) {          // acc += f * columns
+          const unsigned long long ff = pack2(f, f);
 #pragma unroll
-        for (int c = 0; c < NT; c += 32) {
-          if (c < t.rows) {
-            uint32_t v[32];
-            tmem_ld32(tmem + tl + buf * NT + c, v);
+          for (int c = 0; c < kHalf; c += 32) {
+            if (c < rows) {
+              uint32_t v[32];
+              tmem_ld32(from + c, v);
 #pragma unroll
-            for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dd, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
-            if (!Q6) {
-              tmem_ld32(tmem_min + tl + (S::kMinBufs == 2 ? buf * NT : 0u) + c, v);
-#pragma unroll
-              for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(dm, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
+              for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(ff, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
             }
           }
+        };
+        if (!Q6) {
+          add(tmem_min + tl + (S::kMinBufs == 2 ? buf * NT : 0u), d.y);
+          if (S::kMinBufs == 1) {
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&mfree);
+          }
         }
+        add(tmem + tl + buf * NT, d.x);
         if (b + 1 < a.nblk) {
           tmem_fence_before();
           __syncwarp();
@@ -625,11 +640,11 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       }
       if (!ok) break;
       // The sums go through the buffer just read, which is not handed back yet: a loop of few instructions stores them (128 stores
-      // in a row would come through the instruction cache anew for every tile). A warp writes 32 neighbours of an output row.
+      // in a row would come through the instruction cache anew for every tile).
       const uint32_t last = (wi - 1) & 1, stage = tmem + tl + last * NT;
 #pragma unroll
-      for (int c = 0; c < NT; c += 16) {
-        if (c < t.rows) {
+      for (int c = 0; c < kHalf; c += 16) {
+        if (c < rows) {
           uint32_t v[16];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -641,37 +656,33 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         }
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      // 16 output rows at a time: this warp's 32 columns of them through shared memory, out in pieces of 16 bytes
-      constexpr int kPieces = sizeof(OUT) * 2;            // per row
-      OUT* mine = reinterpret_cast<OUT*>(smem + S::kOffStore + (warp - kFirst) * 16 * 128);
-      const int col = t.n0 + (warp - kFirst) * 32;
-      OUT* base = static_cast<OUT*>(a.out) + size_t(t.first) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
+      // a few output rows at a time: this warp's 32 columns of them through shared memory, out in pieces of 16 bytes
+      constexpr int kAtOnce = 32 / int(sizeof(OUT)), kPieces = int(sizeof(OUT)) * 2;     // rows; pieces per row
+      OUT* mine = reinterpret_cast<OUT*>(smem + S::kOffStore + (warp - kFirst) * 1024);
+      const int col = t.n0 + quarter * 32;
+      OUT* base = static_cast<OUT*>(a.out) + size_t(t.first + c0) * size_t(a.ldo) + size_t(t.mat) * a.n + col;
       const bool whole = a.aligned && col + 32 <= a.n;
 #pragma unroll 1
-      for (int c = 0; c < t.rows; c += 16) {
+      for (int c = 0; c < rows; c += 16) {
         uint32_t v[16];
         tmem_ld16(stage + c, v);
-        const float4* f = reinterpret_cast<const float4*>(scale + c);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 s4 = f[q];
-          mine[(4 * q) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q]) * s4.x);
-          mine[(4 * q + 1) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q + 1]) * s4.y);
-          mine[(4 * q + 2) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q + 2]) * s4.z);
-          mine[(4 * q + 3) * 32 + lane] = from_float<OUT>(__uint_as_float(v[4 * q + 3]) * s4.w);
-        }
-        __syncwarp();
-        if (whole) {
+        for (int g = 0; g < 16; g += kAtOnce) {
 #pragma unroll
-          for (int i = lane; i < 16 * kPieces; i += 32) {
-            const int r = i / kPieces, part = i % kPieces;
-            if (c + r < t.rows)
-              reinterpret_cast<uint4*>(base + size_t(c + r) * size_t(a.ldo))[part] = reinterpret_cast<const uint4*>(mine + r * 32)[part];
+          for (int q = 0; q < kAtOnce; ++q) mine[q * 32 + lane] = from_float<OUT>(__uint_as_float(v[g + q]) * scale[c + g + q]);
+          __syncwarp();
+          if (whole) {
+#pragma unroll
+            for (int i = lane; i < 64; i += 32) {
+              const int r = i / kPieces, part = i % kPieces;
+              if (c + g + r < rows)
+                reinterpret_cast<uint4*>(base + size_t(c + g + r) * size_t(a.ldo))[part] = reinterpret_cast<const uint4*>(mine + r * 32)[part];
+            }
+          } else if (col + lane < a.n) {
+            for (int r = 0; r < kAtOnce && c + g + r < rows; ++r) base[size_t(c + g + r) * size_t(a.ldo) + lane] = mine[r * 32 + lane];
           }
-        } else if (col + lane < a.n) {
-          for (int r = 0; r < 16 && c + r < t.rows; ++r) base[size_t(c + r) * size_t(a.ldo) + lane] = mine[r * 32 + lane];
+          __syncwarp();
         }
-        __syncwarp();
       }
       tmem_fence_before();
       __syncwarp();

@@ -23,19 +23,21 @@ inline int row_source_vec(const void* x, int ty, long long ld, int k, int swiglu
 }
 inline size_t row_type_bytes(int ty) { return ty == DARASK_GGML_F32 ? 4 : ty == DARASK_GGML_F16 || ty == DARASK_GGML_BF16 ? 2 : 0; }
 
+// Loads pass L1 by here and in the kernels behind: nothing says that a launch which starts while its predecessor drains finds L1
+// cleared of lines that have been rewritten since.
 DEVI float load_elem(const void* p, int ty, size_t i) {
-  if (ty == DARASK_GGML_F32) return __ldg(static_cast<const float*>(p) + i);
-  const unsigned short u = __ldg(static_cast<const unsigned short*>(p) + i);
+  if (ty == DARASK_GGML_F32) return __ldcg(static_cast<const float*>(p) + i);
+  const unsigned short u = __ldcg(static_cast<const unsigned short*>(p) + i);
   return ty == DARASK_GGML_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float(uint32_t(u) << 16);
 }
 // elements i .. i + 3, i a multiple of four on an aligned base
 DEVI void load_elem4(const void* p, int ty, size_t i, float (&v)[4]) {
   if (ty == DARASK_GGML_F32) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
+    const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
     v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
     return;
   }
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i));
+  const uint2 u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i));
   if (ty == DARASK_GGML_F16) {
     v[0] = half_lo(u.x); v[1] = half_hi(u.x); v[2] = half_lo(u.y); v[3] = half_hi(u.y);
   } else {
