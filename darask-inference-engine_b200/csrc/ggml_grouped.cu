@@ -45,6 +45,13 @@ static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, c
   return launch_pdl(kernel, dim3(sm_count()), dim3(S::kThreads), size_t(S::kSmem), st, m[0], m[1], m[2], m[3], m[4], m[5], a);
 }
 
+template <int KIND>
+static cudaError_t launch_rows(const GgRowsArgs& r, int parts, bool sums, cudaStream_t st) {
+  const auto kernel = parts == 2 ? (sums ? ggml_rows_kernel<KIND, true, true> : ggml_rows_kernel<KIND, true, false>)
+                                 : (sums ? ggml_rows_kernel<KIND, false, true> : ggml_rows_kernel<KIND, false, false>);
+  return launch_pdl(kernel, dim3(unsigned(r.rows)), dim3(kGgRowThreads), 0, st, r);
+}
+
 // f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
 template <bool Q6, int NT>
 static cudaError_t launch_by_type(int out_ty, int nx, const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
@@ -104,9 +111,11 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
       !byte_map(m + 4, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !byte_map(m + 5, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 128, 32, CU_TENSOR_MAP_SWIZZLE_32B))
     return cudaErrorInvalidValue;
-  const auto rows_kernel = nx == 2 ? (q6 ? ggml_rows_kernel<true, false> : ggml_rows_kernel<true, true>)
-                                   : (q6 ? ggml_rows_kernel<false, false> : ggml_rows_kernel<false, true>);
-  if ((e = launch_pdl(rows_kernel, dim3(unsigned(d->rows)), dim3(kGgRowThreads), 0, st, r))) return e;
+  const int kind = d->swiglu || r.src.vec < (d->x_ty == DARASK_GGML_F32 ? 1 : 2) || d->ldx % (d->x_ty == DARASK_GGML_F32 ? 4 : 8)
+                       ? 0 : d->x_ty == DARASK_GGML_F32 ? 1 : d->x_ty == DARASK_GGML_F16 ? 2 : 3;
+  if ((e = kind == 0 ? launch_rows<0>(r, nx, !q6, st) : kind == 1 ? launch_rows<1>(r, nx, !q6, st) : kind == 2 ? launch_rows<2>(r, nx, !q6, st)
+                                                                                              : launch_rows<3>(r, nx, !q6, st)))
+    return e;
   GgArgs a = {};
   a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);

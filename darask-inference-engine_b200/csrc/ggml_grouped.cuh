@@ -39,11 +39,11 @@ struct GgArgs {
 // NT: rows of x per tile, NX: f16 parts of a row of x, NA: f16 terms of a Q6_K integer. A step is 128 columns of k.
 template <bool Q6, int NT, int NX, int NA>
 struct GgShape {
-  // TMEM holds the weights of kSlots steps. Few rows: one set of four expander warps per slot, the sets hide their latencies from
-  // each other. Many rows leave TMEM for two slots, which two sets fill together (half a step each): a slot is filled, handed over,
-  // multiplied and handed back in turn, and that turn sets the pace.
+  // TMEM holds the weights of kSets steps, and a set of four expander warps belongs to each slot. Few rows leave room for four slots,
+  // whose sets hide their latencies from each other; 128 rows leave two (there, sets that fill each step together took 439 us where
+  // these take 423, and four promotion warps instead of eight 466: 32768 rows, 128 groups of 2 x 768 x 2048).
   static constexpr bool kWide = NT > 32;
-  static constexpr int kSlots = kWide ? 2 : NA == 2 ? 3 : 4, kSets = kWide ? 2 : kSlots;
+  static constexpr int kSets = kWide ? 2 : NA == 2 ? 3 : 4;
   static constexpr int kPromote = kWide ? 8 : 4;         // warps that promote and store: two per quarter of the weight rows, half of x each
   static constexpr int kThreads = 128 * (1 + kSets) + 32 * kPromote;
   // wide: registers of the roles, the expanders and the promotion; their sum is what the block is launched with (640 x 96)
@@ -56,7 +56,7 @@ struct GgShape {
   static constexpr int kSums = Q6 ? 0 : NT * 32;         // NT rows x 16 f16: the sums of eight groups of 32 columns, high and low parts
   static constexpr int kXStage = NX * kPart + kSums;     // Q4_K: the sums travel with the second step of a block
   static constexpr int kXStages = kWide && NX == 2 ? 2 : 4;
-  static constexpr int kMins = Q6 ? 0 : kSlots / 2;       // 128 rows x 32 bytes each
+  static constexpr int kMins = Q6 ? 0 : kSets / 2;       // 128 rows x 32 bytes each
   static constexpr int kOffMin = kXStages * kXStage;
   static constexpr int kOffRaw = kOffMin + kMins * 4096;
   static constexpr int kStore = kPromote * 1024;         // per warp 16 output rows x 32 columns (8 rows of float32)
@@ -69,8 +69,8 @@ struct GgShape {
   static constexpr int kSmem = 1024 + kOffStore + kTail;
   // TMEM columns: two main buffers, one or two of min products, the weights, their second terms
   static constexpr int kMinBufs = Q6 ? 0 : kWide ? 1 : 2;
-  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSlots;
-  static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSlots : 0) <= 512, "rings must fit");
+  static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSets;
+  static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSets : 0) <= 512, "rings must fit");
 };
 
 // ---- rows of x -> f16 parts --------------------------------------------------------------------------------------------
@@ -87,24 +87,30 @@ struct GgRowsArgs {
 };
 constexpr int kGgRowThreads = 128;
 constexpr int kGgRowHeld = 4;                            // groups of eight columns a thread keeps in registers (k <= 4096); longer rows are read twice
-DEVI void rows_load8(const RowSource& s, long long row, int c, float (&v)[8]) {
-  if (s.vec == 2 && s.ty != DARASK_GGML_F32 && !s.swiglu) {          // 16-byte aligned 16-bit rows: one load
-    const uint4 u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(s.x) + size_t(row) * size_t(s.ld) + c));
+// KIND: 0 any rows (four elements at a time, strides and SwiGLU as they come); 1 float32, 2 f16, 3 bf16 rows on 16-byte boundaries
+template <int KIND>
+DEVI void rows_load8(const RowSource& s, const void* at, long long row, int c, float (&v)[8]) {
+  if (KIND == 0) {
+    float a[4], b[4];
+    row_source_load4(s, row, c, a);
+    row_source_load4(s, row, c + 4, b);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+  } else if (KIND == 1) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(at) + c);
+    const float4 a = __ldcg(p), b = __ldcg(p + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(at) + c));
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      v[2 * q] = s.ty == DARASK_GGML_F16 ? half_lo(w[q]) : __uint_as_float(w[q] << 16);
-      v[2 * q + 1] = s.ty == DARASK_GGML_F16 ? half_hi(w[q]) : __uint_as_float(w[q] & 0xffff0000u);
+      v[2 * q] = KIND == 2 ? half_lo(w[q]) : __uint_as_float(w[q] << 16);
+      v[2 * q + 1] = KIND == 2 ? half_hi(w[q]) : __uint_as_float(w[q] & 0xffff0000u);
     }
-    return;
   }
-  float a[4], b[4];
-  row_source_load4(s, row, c, a);
-  row_source_load4(s, row, c + 4, b);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
 }
-template <bool PARTS, bool SUMS>
+template <int KIND, bool PARTS, bool SUMS>
 __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsArgs a) {
   __shared__ uint32_t red[kGgRowThreads / 32];
   pdl_wait();
@@ -114,6 +120,8 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   long long row = i;
   if (a.assignments) row = __ldcg(a.assignments + i) / unsigned(a.topk);
   const bool exists = row < a.x_rows;
+  const void* at = KIND == 1 ? static_cast<const void*>(static_cast<const float*>(a.src.x) + row * a.src.ld)
+                             : static_cast<const void*>(static_cast<const unsigned short*>(a.src.x) + row * a.src.ld);      // KIND 0: unused
   float held[kGgRowHeld][8];
   uint32_t top = 0;
   auto scan = [&](const float (&v)[8]) {
@@ -123,18 +131,15 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
 #pragma unroll
   for (int j = 0; j < kGgRowHeld; ++j) {
     const int c = (j * kGgRowThreads + threadIdx.x) * 8;
-    if (exists && c < k) rows_load8(a.src, row, c, held[j]);
-    else {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) held[j][q] = 0.f;
+    if (exists && c < k) {
+      rows_load8<KIND>(a.src, at, row, c, held[j]);
+      scan(held[j]);
     }
   }
-#pragma unroll
-  for (int j = 0; j < kGgRowHeld; ++j) scan(held[j]);
   if (exists)
     for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 8; c < k; c += kGgRowThreads * 8) {
       float v[8];
-      rows_load8(a.src, row, c, v);
+      rows_load8<KIND>(a.src, at, row, c, v);
       scan(v);
     }
   top = __reduce_max_sync(0xffffffffu, top);
@@ -154,7 +159,7 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
     float s = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      v[q] = live ? v[q] * down : 0.f;
+      v[q] = live ? v[q] * down : 0.f;         // (a row that does not exist was never loaded)
       s += v[q];
     }
 #pragma unroll
@@ -191,7 +196,7 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
     float v[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = 0.f;
-    if (live) rows_load8(a.src, row, c, v);
+    if (live) rows_load8<KIND>(a.src, at, row, c, v);
     put(c, v);
   }
 }
@@ -267,7 +272,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
   int* ends = reinterpret_cast<int*>(smem + S::kOffEnds);                   // [groups + 1] cumulative tile counts
   // A step (128 columns of k) has one "full" barrier, on which its tile of x and its expander warps count, and one "empty"
-  // barrier, on which the tensor core reports it read: the loader, the expanders (kSlots steps on) and, at the end of a block of
+  // barrier, on which the tensor core reports it read: the loader, the expanders (kSets steps on) and, at the end of a block of
   // 256 columns, the promotion all wait for that one. Waits and commits are what the MMA warp spends its time on.
   // With two stages and nothing but the buffers between them (Q6_K) the tensor core could report the next block before a late warp
   // has looked for this one, so the promotion has barriers of its own there.
@@ -280,7 +285,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < S::kRawStages; ++s) { mbar_init(wfull + s, 1); mbar_init(wempty + s, 8); }
-    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, S::kWide ? 9 : 5); mbar_init(empty + s, 1); }
+    for (int s = 0; s < S::kXStages; ++s) { mbar_init(full + s, 5); mbar_init(empty + s, 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(tempty + s, S::kPromote); mbar_init(done + s, 1); }
     mbar_init(&mfree, S::kPromote);
     mbar_fence_init();
@@ -428,8 +433,8 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           // stage of the first step and its parity: two or four stages
           const uint32_t x0 = S::kXStages == 4 ? buf * 2 : 0u, ph = S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1;
           // TMEM slots of the two steps
-          const uint32_t a0 = slot, a1 = slot + 1 == S::kSlots ? 0u : slot + 1;
-          slot = a1 + 1 == S::kSlots ? 0u : a1 + 1;
+          const uint32_t a0 = slot, a1 = slot + 1 == S::kSets ? 0u : slot + 1;
+          slot = a1 + 1 == S::kSets ? 0u : a1 + 1;
           // the buffers are free: the block before the last has been promoted
           if (wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
           ok = warp_wait(full + x0, ph, a.status) && ok;
@@ -466,7 +471,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     if (S::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegExpand));
     // ---- expanders: four warps, one for each quarter of the TMEM lanes, take every kSets-th step --------------------------------
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + (S::kWide ? 0 : set * 64);       // narrow: the set's TMEM slot
+    const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + set * 64;       // the set's TMEM slot
     const uint32_t magic = opaque(0x64006400u);      // 1024 in both halves
     int ws = 0, turn = 0;                // raw stage, set whose step comes next
     uint32_t wph = 0, wi = 0;
@@ -487,24 +492,22 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (Q6 && b + 1 < a.nblk) d_next = __half2float(__ldcg(dq + b + 1));
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {                     // the block's two steps
-          if (!S::kWide) {
-            const bool mine = turn == set;
-            if (++turn == S::kSets) turn = 0;
-            if (!mine) continue;
-          }
+          const bool mine = turn == set;
+          if (++turn == S::kSets) turn = 0;
+          if (!mine) continue;
           ok = warp_wait(wfull + ws, wph, a.status);
           const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
           // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
           const uint4 head = lds128(raw + (Q6 ? 192 : 0));
-          // the TMEM slot is free when the step kSlots before has been read
-          const uint32_t ps = 2 * wi + h - S::kSlots;
-          if (2 * wi + h >= uint32_t(S::kSlots)) ok = warp_wait(empty + ps % S::kXStages, (ps / S::kXStages) & 1, a.status) && ok;
+          // the TMEM slot is free when the step kSets before has been read
+          const uint32_t ps = 2 * wi + h - S::kSets;
+          if (2 * wi + h >= uint32_t(S::kSets)) ok = warp_wait(empty + ps % S::kXStages, (ps / S::kXStages) & 1, a.status) && ok;
           if (!ok) break;
           tmem_fence_after();
-          if (h == 0 && (!S::kWide || set == 0)) {
+          if (h == 0) {
             const __half2 dd = as_half2(head.x);
             dring[(wi & 3) * 128 + row] = Q6 ? make_float2(d_now, 0.f) : make_float2(__low2float(dd), -__high2float(dd));
-          } else if (!Q6 && h == 1 && (!S::kWide || set == 1)) {
+          } else if (!Q6) {
             // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
             const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
             auto pair = [](uint32_t w, int sel) { return as_word(__hsub2(as_half2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(1024.f))); };
@@ -517,8 +520,8 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           // Q4_K: the four scales of the step; Q6_K: the step is one half of the block
           const uint32_t scales = h == 0 ? head.y & 0x3f3f3f3fu : (head.w & 0x0f0f0f0fu) | ((head.y >> 2) & 0x30303030u);
 #pragma unroll 1
-          for (int cc = S::kWide ? set : 0; cc < (S::kWide ? set + 1 : 2); ++cc) {       // 64 columns
-            const uint32_t dst = tl + (S::kWide ? h * 64 : 0) + cc * 32;
+          for (int cc = 0; cc < 2; ++cc) {                // 64 columns
+            const uint32_t dst = tl + cc * 32;
             const uint32_t at = raw + (Q6 ? 128 + h * 32 : 16 + (h * 2 + cc) * 32);
             const uint4 w0 = lds128(at), w1 = lds128(at + 16);        // Q4_K: codes; Q6_K: upper bits
             const uint32_t scw = scales >> (16 * cc);
@@ -572,7 +575,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(full + (2 * wi + h) % S::kXStages);
-            if (!S::kWide || h == 1) mbar_arrive(wempty + ws);
+            mbar_arrive(wempty + ws);
           }
         }
         if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
@@ -601,9 +604,9 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         scale[r] = fabsf(v);
       }
       __syncwarp();
-      unsigned long long acc[kHalf / 2];                   // pairs of float32 sums
+      float acc[kHalf];
 #pragma unroll
-      for (int c = 0; c < kHalf / 2; ++c) acc[c] = 0ull;
+      for (int c = 0; c < kHalf; ++c) acc[c] = 0.f;
 #pragma unroll 1
       for (int b = 0; b < a.nblk; ++b, ++wi) {
         const uint32_t buf = wi & 1;
@@ -612,14 +615,13 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         tmem_fence_after();
         const float2 d = dring[(wi & 3) * 128 + row];     // {d, -dmin}
         auto add = [&](uint32_t from, float f) {          // acc += f * columns
-          const unsigned long long ff = pack2(f, f);
 #pragma unroll
           for (int c = 0; c < kHalf; c += 32) {
             if (c < rows) {
               uint32_t v[32];
               tmem_ld32(from + c, v);
 #pragma unroll
-              for (int q = 0; q < 16; ++q) acc[c / 2 + q] = fma2(ff, pack2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), acc[c / 2 + q]);
+              for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(f, __uint_as_float(v[q]), acc[c + q]);
             }
           }
         };
@@ -647,11 +649,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (c < rows) {
           uint32_t v[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 y = unpack2(acc[c / 2 + j]);
-            v[2 * j] = __float_as_uint(y.x);
-            v[2 * j + 1] = __float_as_uint(y.y);
-          }
+          for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(acc[c + j]);
           tmem_st16(stage + c, v);
         }
       }
