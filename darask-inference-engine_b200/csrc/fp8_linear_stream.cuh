@@ -203,13 +203,9 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
     const uint32_t tl = tmem + (uint32_t((warp - 4) * 32) << 16);
     for (int i = 0; i < kbs; ++i) {
       const int buf = i % kFsBufs, g = i / kFsGroup;
-      int ok = 1;
-      if (lane == 0) {
-        ok = pipe_wait(tfull + buf, (i / kFsBufs) & 1, a.status) ? 1 : 0;
-        if (ok && !FUSED && i % kFsGroup == 0) ok = pipe_wait(ffull + (g & 1), (g >> 1) & 1, a.status) ? 1 : 0;
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok || abort_flag) { abort_flag = 1; break; }
+      bool ok = warp_wait(tfull + buf, (i / kFsBufs) & 1, a.status);
+      if (!FUSED && i % kFsGroup == 0) ok = warp_wait(ffull + (g & 1), (g >> 1) & 1, a.status) && ok;
+      if (!ok) { abort_flag = 1; break; }
       tmem_fence_after();
       const float4* f = reinterpret_cast<const float4*>(factors + (FUSED ? i : (g & 1) * kFsGroup + i % kFsGroup) * NT);
       if (NT == 16) {

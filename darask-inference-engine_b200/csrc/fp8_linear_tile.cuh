@@ -164,13 +164,9 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       for (int c = 0; c < 128; ++c) acc[c] = 0.f;
       for (int kb = 0; kb < a.kb; ++kb, ++it) {
         const int buf = it & 1, slot = fg & 1;
-        int got = 1;
-        if (lane == 0) {
-          if (kb % kFtGroup == 0) got = pipe_wait(ffull + slot, (fg >> 1) & 1, a.status) ? 1 : 0;
-          if (got) got = pipe_wait(tfull + buf, (it >> 1) & 1, a.status) ? 1 : 0;
-        }
-        got = __shfl_sync(0xffffffffu, got, 0);
-        if (!got) { abort_flag = 1; ok = false; break; }
+        if (kb % kFtGroup == 0) ok = warp_wait(ffull + slot, (fg >> 1) & 1, a.status);
+        ok = warp_wait(tfull + buf, (it >> 1) & 1, a.status) && ok;
+        if (!ok) { abort_flag = 1; break; }
         tmem_fence_after();
         const float f = fx[(slot * kFtGroup + kb % kFtGroup) * 128 + row] * fw[(slot * kFtGroup + kb % kFtGroup) * 2 + half];
         uint32_t v[64];

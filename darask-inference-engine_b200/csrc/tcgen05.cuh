@@ -170,8 +170,10 @@ DEVI uint32_t cluster_map(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-DEVI void mbar_arrive_cluster(uint32_t addr) {      // barrier anywhere in the cluster, address from cluster_map
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+// Barrier anywhere in the cluster, address from cluster_map. It hands over TMEM, which tcgen05.fence orders: a release at the scope of
+// the cluster would wait here for everything this thread has in flight (400 to 2000 cycles).
+DEVI void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 DEVI float ld_cluster_f32(uint32_t addr) {
   float v;
