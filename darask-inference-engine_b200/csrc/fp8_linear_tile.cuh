@@ -45,9 +45,18 @@ DEVI void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, ui
 DEVI void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
 }
-DEVI void umma_commit_pair(uint64_t* bar) {                       // arrives on the barrier at this offset in both blocks
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(smem_u32(bar)), "h"(uint16_t(3)) : "memory");
+DEVI void umma_commit_pair(uint64_t* bar, uint32_t go) {          // arrives on the barrier at this offset in both blocks
+  asm volatile(
+      "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
+      "@g tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+      ::"r"(smem_u32(bar)), "h"(uint16_t(3)), "r"(go) : "memory");
+}
+DEVI void umma_f8_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t accumulate, uint32_t go) {      // M256 N256 K32
+  constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(256 >> 3) << 17) | (uint32_t(256 >> 4) << 24);
+  asm volatile(
+      "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %5, 0;\n\t"
+      "@g tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(da), "l"(db), "r"(kIdesc), "r"(accumulate), "r"(go) : "memory");
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFtThreads, 1)
@@ -61,7 +70,7 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   __shared__ uint64_t full[kFtStages], empty[kFtStages], tfull[2], tempty[2], ffull[2], fempty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -84,42 +93,58 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0 && lane == 0) {
-      int it = 0;
-      for (int tile = first; tile < total && !abort_flag; tile += step) {
+    // (the lanes of warps 0 and 1 stay together: operands of the copies and of tcgen05.mma live in uniform registers)
+    if (warp == 0) {
+      const uint32_t go = elect_lane();
+      const uint32_t full0 = cluster_map(smem_u32(full), 0), ring0 = smem_u32(ring);
+      int s = 0, used = 0;               // stage; stages filled so far (up to the first round)
+      uint32_t ph = 1;                   // parity of the "empty" phase
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += step) {
         const int r0 = (tile % a.tiles_m) * 256 + int(rank) * 128, w0 = (tile / a.tiles_m) * 256 + int(rank) * 128;
-        for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int s = it % kFtStages;
-          if (it >= kFtStages && !pipe_wait(empty + s, ((it / kFtStages) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-          const uint32_t dst = smem_u32(ring + s * kFtStageBytes), bar = cluster_map(smem_u32(full + s), 0);
-          if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * kFtStageBytes);
-          tma_load_pair(dst, &map_x, kb * 128, r0, bar);
-          tma_load_pair(dst + 128 * 128, &map_w, kb * 128, w0, bar);
+#pragma unroll 1
+        for (int kb = 0; kb < a.kb; ++kb) {
+          if (used == kFtStages) ok = warp_wait(empty + s, ph, a.status);
+          else ++used;
+          if (!ok) break;
+          if (go) {
+            const uint32_t dst = ring0 + s * kFtStageBytes, bar = full0 + s * 8;
+            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * kFtStageBytes);
+            tma_load_pair(dst, &map_x, kb * 128, r0, bar);
+            tma_load_pair(dst + 128 * 128, &map_w, kb * 128, w0, bar);
+          }
+          if (++s == kFtStages) { s = 0; ph ^= 1; }
         }
       }
-      // after a timeout the copies in flight land before the pair ends
-      if (abort_flag && rank == 0)
-        for (int i = it > kFtStages ? it - kFtStages : 0; i < it; ++i) pipe_wait(full + i % kFtStages, (i / kFtStages) & 1, a.status);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-      constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(256 >> 3) << 17) | (uint32_t(256 >> 4) << 24);
-      int it = 0;
-      for (int tile = first; tile < total && !abort_flag; tile += step) {
-        for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int s = it % kFtStages, buf = it & 1;
-          if (it >= 2 && !pipe_wait(tempty + buf, ((it >> 1) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-          if (!pipe_wait(full + s, (it / kFtStages) & 1, a.status)) { abort_flag = 1; break; }
-          tmem_fence_after();
-          const uint32_t sx = smem_u32(ring + s * kFtStageBytes);
-          const uint64_t dx = umma_desc_k128(sx), dw = umma_desc_k128(sx + 128 * 128);
+      if (!ok) {                         // after a timeout the copies in flight land before the pair ends
+        abort_flag = 1;
+        if (rank == 0)
+          for (int i = 0; i < used; ++i) pipe_wait(full + i, i < s ? ph ^ 1 : ph, a.status);
+      }
+    } else if (warp == 1) {
+      if (rank == 0) {
+        const uint32_t go = elect_lane();
+        const uint64_t d0 = umma_desc_k128(smem_u32(ring));
+        int s = 0;
+        uint32_t ph = 0, it = 0;
+        bool ok = true;
+        for (int tile = first; tile < total && ok; tile += step) {
+#pragma unroll 1
+          for (int kb = 0; kb < a.kb; ++kb, ++it) {
+            const uint32_t buf = it & 1;
+            if (it >= 2) ok = warp_wait(tempty + buf, ((it >> 1) & 1) ^ 1, a.status);
+            ok = warp_wait(full + s, ph, a.status) && ok;
+            if (!ok) break;
+            tmem_fence_after();
+            const uint64_t dx = d0 + uint32_t(s * (kFtStageBytes >> 4)), dw = dx + (128 * 128 >> 4);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            asm volatile(
-                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                ::"r"(tmem + buf * 256), "l"(dx + 2 * q), "l"(dw + 2 * q), "r"(kIdesc), "r"(q ? 1u : 0u) : "memory");
-          umma_commit_pair(empty + s);
-          umma_commit_pair(tfull + buf);
+            for (int q = 0; q < 4; ++q) umma_f8_pair(tmem + buf * 256, dx + 2 * q, dw + 2 * q, q ? 1u : 0u, go);
+            umma_commit_pair(empty + s, go);
+            umma_commit_pair(tfull + buf, go);
+            if (++s == kFtStages) { s = 0; ph ^= 1; }
+          }
         }
+        if (!ok) abort_flag = 1;
       }
     } else if (warp >= 2) {
       const int ft = threadIdx.x - 64;

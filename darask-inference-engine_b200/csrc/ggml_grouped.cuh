@@ -244,11 +244,6 @@ DEVI void umma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint
       "@g tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
 }
-DEVI void umma_commit_if(uint64_t* bar, uint32_t go) {
-  asm volatile(
-      "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %1, 0;\n\t"
-      "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(go) : "memory");
-}
 // K-major operand tile, rows of 32 bytes, 32-byte swizzle, 8-row groups 256 bytes apart
 DEVI uint64_t umma_desc_k32(uint32_t smem_addr) {
   return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(256 >> 4) << 32) | (1ull << 46) | (6ull << 61);

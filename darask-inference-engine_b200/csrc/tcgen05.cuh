@@ -155,6 +155,13 @@ DEVI uint32_t elect_lane() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one;
 }
+// commits by the lane with `go` set
+DEVI void umma_commit_if(uint64_t* bar, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %1, 0;\n\t"
+      "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(go) : "memory");
+}
+
 // ---- clusters --------------------------------------------------------------------------------------------------------
 DEVI uint32_t cluster_rank() {
   uint32_t r;
