@@ -210,6 +210,15 @@ def float_type(dtype) -> int | None:
     return _FLOAT_TYPES.get(dtype)
 
 
+def current_stream(device_index: int) -> int:
+    """cudaStream_t of the current stream of a device."""
+    import torch
+    try:
+        return torch._C._cuda_getCurrentRawStream(device_index)      # what torch.cuda.current_stream(...).cuda_stream holds, without the object
+    except AttributeError:
+        return torch.cuda.current_stream(device_index).cuda_stream
+
+
 def row_stride(t) -> int:
     """Elements from row to row of a 2D tensor, or -1 when its columns are strided or its rows overlap. A single row has
     whatever stride; the kernels want at least its length, in steps of 16."""

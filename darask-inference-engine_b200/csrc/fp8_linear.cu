@@ -10,6 +10,20 @@
 namespace dmoe {
 
 static __device__ unsigned g_fp8_linear_status;
+// its address, looked up once per device
+static cudaError_t status_word(unsigned** p) {
+  static unsigned* known[64] = {};
+  const int dev = current_device_slot();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  if (!known[dev]) {
+    void* q = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&q, g_fp8_linear_status);
+    if (e != cudaSuccess) return e;
+    known[dev] = static_cast<unsigned*>(q);
+  }
+  *p = known[dev];
+  return cudaSuccess;
+}
 
 // One warp per row and 128 columns, four columns per lane: scale = absmax / 448 (1 for zeros), code = e4m3(x * (1 / scale)),
 // every step rounded to float32. A group with an infinity or a NaN gets the scale NaN, so that the row's products say so.
@@ -119,8 +133,8 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
   if (!linear_ok(d)) return cudaErrorInvalidValue;
   if (d->m == 0) return cudaSuccess;
   const int kb = (d->k + 127) / 128;
-  void* status = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&status, g_fp8_linear_status);
+  unsigned* status = nullptr;
+  cudaError_t e = status_word(&status);
   if (e != cudaSuccess) return e;
   const bool codes = d->x_ty == DARASK_E4M3;
   const LinearPlan p = linear_plan(d->m, d->n, kb, codes);
@@ -129,7 +143,7 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
   a.ws = d->w_scales; a.ld_ws = d->ld_ws;
   a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo;
   a.tiles_n = (d->n + 127) / 128;
-  a.status = static_cast<unsigned*>(status);
+  a.status = status;
   a.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, codes ? 0 : row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
   const uint8_t* xc = static_cast<const uint8_t*>(d->x);
   unsigned long long pitch = d->ldx, cols = d->k;
@@ -159,8 +173,8 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
 
 extern "C" int darask_fp8_linear_status(unsigned* host_status, cudaStream_t st) {
   if (!host_status) return cudaErrorInvalidValue;
-  void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, g_fp8_linear_status);
+  unsigned* p = nullptr;
+  cudaError_t e = status_word(&p);
   if (!e) e = cudaMemcpyAsync(host_status, p, 4, cudaMemcpyDeviceToHost, st);
   if (!e) e = cudaMemsetAsync(p, 0, 4, st);
   return e ? e : cudaStreamSynchronize(st);

@@ -7,7 +7,7 @@
 //   warp 1      tcgen05.mma, four per block of k, into one of four TMEM buffers of NT columns
 //   warps 2-3   the factors sx * sw of the blocks, eight blocks of k at a time, two groups ahead of their use
 //   warps 4-7   tcgen05.ld of the block's partial tile (thread = one weight row), times the factors, added in registers
-// FUSED: x comes as float rows; before the loop all warps but 0 and 1 quantize this block's part of x straight into the
+// FUSED: x comes as float rows; before the loop all warps but 0 quantize this block's part of x straight into the
 // swizzled operand tiles, which stay in shared memory (16 rows, at most kFsResident blocks of k): one launch in all.
 #pragma once
 #include <cuda_fp8.h>
@@ -19,6 +19,7 @@ namespace dmoe {
 constexpr int kFsThreads = 256;
 constexpr int kFsResident = 32;              // blocks of k a FUSED block holds of x
 constexpr int kFsGroup = 8;                  // blocks of k whose factors travel together
+constexpr int kFsFlight = 6;                 // groups of x a warp has in flight while it quantizes
 constexpr int kFsBufs = 4;                   // TMEM buffers
 
 struct FsArgs {
@@ -68,6 +69,39 @@ DEVI float fp8_group(const float (&v)[4], uint32_t* codes) {
   return scale;
 }
 
+// Block `rank` adds and stores every SPLITS-th row of x of the cluster's tile: a warp per row, four weight rows per lane, eight pieces
+// from other blocks in flight; added in rank order.
+template <int SPLITS, int NT>
+DEVI void fs_join(const FsArgs& a, float* part, uint32_t rank, int n0, int t0) {
+  constexpr int U = 8 / SPLITS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = n0 + lane * 4;
+  uint32_t from[SPLITS];
+#pragma unroll
+  for (int s = 0; s < SPLITS; ++s) from[s] = cluster_map(smem_u32(part) + lane * 16, s);
+  for (int c0 = int(rank) + warp * SPLITS; c0 < NT && t0 + c0 < a.m; c0 += 8 * SPLITS * U) {
+    float4 v[U][SPLITS];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < SPLITS; ++s) {
+        const int c = c0 + u * 8 * SPLITS;
+        if (c < NT) v[u][s] = ld_cluster_f32x4(from[s] + c * 512);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 8 * SPLITS;
+      if (c >= NT || t0 + c >= a.m) break;
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < SPLITS; ++s) { y[0] += v[u][s].x; y[1] += v[u][s].y; y[2] += v[u][s].z; y[3] += v[u][s].w; }
+      const size_t at = size_t(t0 + c) * size_t(a.ldo) + col;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (col + q < a.n) store_elem(a.out, a.out_ty, at + q, y[q]);
+    }
+  }
+}
+
 template <int NT, bool FUSED>
 __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                        const __grid_constant__ CUtensorMap map_x, const FsArgs a) {
@@ -80,7 +114,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
   __shared__ uint64_t full[kStages], empty[kStages], tfull[kFsBufs], tempty[kFsBufs], ffull[2], fempty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const uint32_t rank = cluster_rank();
@@ -109,27 +143,29 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
     // the first weight tiles travel while x is quantized (thread 0 has initialised the barriers that it uses here)
     if (threadIdx.x == 0)
       for (int i = 0; i < kStages && i < kbs; ++i) load_stage(i);
-    if (warp >= 2) {
-      // group = (block of k, row); rows past m: zero codes and factors
-      const int groups = kbs * 16;
-      for (int g0 = (warp - 2); g0 < groups; g0 += 6 * 4) {
-        float v[4][4];
+    if (warp >= 1) {
+      // group = (block of k, row), a handful per warp in flight; rows past m stay as they are: what they give is never stored
+      const int groups = kbs * a.m;
+      const float* ws = a.ws + size_t(n0 / 128) * size_t(a.ld_ws) + kb0;
+      for (int g0 = warp - 1; g0 < groups; g0 += 7 * kFsFlight) {
+        float v[kFsFlight][4], w[kFsFlight];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int g = g0 + 6 * u, row = g & 15;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
-          if (g < groups && row < a.m) row_source_load4(a.src, row, (kb0 + (g >> 4)) * 128 + lane * 4, v[u]);
+        for (int u = 0; u < kFsFlight; ++u) {
+          const int g = g0 + 7 * u, b = g / a.m;
+          if (g < groups) {
+            row_source_load4(a.src, g - b * a.m, (kb0 + b) * 128 + lane * 4, v[u]);
+            w[u] = __ldcg(ws + b);
+          }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int g = g0 + 6 * u, b = g >> 4, row = g & 15;
+        for (int u = 0; u < kFsFlight; ++u) {
+          const int g = g0 + 7 * u, b = g / a.m, row = g - b * a.m;
           if (g >= groups) break;
           uint32_t codes;
           const float scale = fp8_group(v[u], &codes);
           // 128-byte rows, 16-byte pieces swizzled by the row in its group of eight
           *reinterpret_cast<uint32_t*>(xres + size_t(b) * 2048 + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = codes;
-          if (lane == 0) factors[b * 16 + row] = row < a.m ? scale * __ldcg(a.ws + size_t(n0 / 128) * size_t(a.ld_ws) + kb0 + b) : 0.f;
+          if (lane == 0) factors[b * 16 + row] = scale * w[u];
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -156,23 +192,26 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
         for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) pipe_wait(full + i % kStages, (i / kStages) & 1, a.status);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      for (int i = 0; i < kbs && !abort_flag; ++i) {
-        const int s = i % kStages, buf = i % kFsBufs;
-        if (i >= kFsBufs && !pipe_wait(tempty + buf, ((i / kFsBufs) & 1) ^ 1, a.status)) { abort_flag = 1; break; }
-        if (!pipe_wait(full + s, (i / kStages) & 1, a.status)) { abort_flag = 1; break; }
-        tmem_fence_after();
-        const uint32_t sw = smem_u32(ring + s * kStageBytes);
-        const uint64_t dw = umma_desc_k128(sw), dx = umma_desc_k128(FUSED ? smem_u32(xres + size_t(i) * 2048) : sw + 128 * 128);
+    // (the lanes stay together: operands of tcgen05.mma live in uniform registers)
+    const uint32_t go = elect_lane();
+    const uint64_t d0 = umma_desc_k128(smem_u32(ring)), dres = umma_desc_k128(smem_u32(xres));
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < kbs; ++i) {
+      const int s = i % kStages, buf = i % kFsBufs;
+      if (i >= kFsBufs) ok = warp_wait(tempty + buf, ((i / kFsBufs) & 1) ^ 1, a.status);
+      ok = warp_wait(full + s, (i / kStages) & 1, a.status) && ok;
+      if (!ok) { abort_flag = 1; break; }
+      tmem_fence_after();
+      const uint64_t dw = d0 + uint32_t(s * (kStageBytes >> 4)), dx = FUSED ? dres + uint32_t(i * (2048 >> 4)) : dw + (128 * 128 >> 4);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          asm volatile(
-              "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-              ::"r"(tmem + buf * NT), "l"(dw + 2 * q), "l"(dx + 2 * q), "r"(kIdesc), "r"(q ? 1u : 0u), "r"(0u) : "memory");
-        umma_commit(empty + s);
-        umma_commit(tfull + buf);
-      }
+      for (int q = 0; q < 4; ++q)
+        asm volatile(
+            "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %5, 0;\n\t"
+            "@g tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(tmem + buf * NT), "l"(dw + 2 * q), "l"(dx + 2 * q), "r"(kIdesc), "r"(q ? 1u : 0u), "r"(go) : "memory");
+      umma_commit_if(empty + s, go);
+      umma_commit_if(tfull + buf, go);
     }
   } else if (warp < 4) {
     if (!FUSED) {
@@ -258,13 +297,9 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
       for (int c = 0; c < NT; ++c) part[c * 128 + row] = acc[c];
     }
     cluster_sync();
-    // block `rank` joins every splits-th row of x
-    const int half = threadIdx.x >> 7, r = threadIdx.x & 127;
-    for (int c = int(rank) + half * int(splits); c < NT && t0 + c < a.m; c += 2 * int(splits)) {
-      float v = 0.f;
-      for (uint32_t s = 0; s < splits; ++s) v += ld_cluster_f32(cluster_map(smem_u32(part + c * 128 + r), s));
-      if (n0 + r < a.n) store_elem(a.out, a.out_ty, size_t(t0 + c) * size_t(a.ldo) + n0 + r, v);
-    }
+    if (splits == 2) fs_join<2, NT>(a, part, rank, n0, t0);
+    else if (splits == 4) fs_join<4, NT>(a, part, rank, n0, t0);
+    else fs_join<8, NT>(a, part, rank, n0, t0);
     cluster_sync();                                                // nobody leaves while its tile is being read
   }
   tmem_fence_before();

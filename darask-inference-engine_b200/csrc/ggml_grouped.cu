@@ -8,6 +8,20 @@
 namespace dmoe {
 
 static __device__ unsigned g_ggml_grouped_status;
+// its address, looked up once per device
+static cudaError_t status_word(unsigned** p) {
+  static unsigned* known[64] = {};
+  const int dev = current_device_slot();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  if (!known[dev]) {
+    void* q = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&q, g_ggml_grouped_status);
+    if (e != cudaSuccess) return e;
+    known[dev] = static_cast<unsigned*>(q);
+  }
+  *p = known[dev];
+  return cudaSuccess;
+}
 
 static int ggml_row_bytes(int ty, int k) {
   return ty == DARASK_GGML_Q4_K ? k / 256 * 144 : ty == DARASK_GGML_Q6_K ? k / 256 * 208 + (2 * (k / 256) + 15) / 16 * 16 : 0;
@@ -89,8 +103,8 @@ static bool grouped_ok(const DaraskGgmlGrouped* d) {
 extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t st) {
   if (!grouped_ok(d)) return cudaErrorInvalidValue;
   if (d->rows == 0) return cudaSuccess;
-  void* status = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&status, g_ggml_grouped_status);
+  unsigned* status = nullptr;
+  cudaError_t e = status_word(&status);
   if (e) return e;
   const bool q6 = d->w_ty == DARASK_GGML_Q6_K;
   const int parts = row_parts(d->x_ty, d->swiglu), row_bytes = ggml_row_bytes(d->w_ty, d->k), nblk = d->k / 256;
@@ -122,7 +136,7 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo;
   const size_t ob = row_type_bytes(d->out_ty);
   a.aligned = reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->ldo * ob % 16 == 0 && (!d->w_up || d->n * ob % 16 == 0);
-  a.status = static_cast<unsigned*>(status);
+  a.status = status;
   // narrow tiles while the groups have few rows on average: the weights' bytes pace the product then
   const bool narrow = d->rows <= 32ll * d->groups;
   if (q6) return narrow ? launch_by_type<true, 32>(d->out_ty, nx, m, a, st) : launch_by_type<true, 128>(d->out_ty, nx, m, a, st);
@@ -131,8 +145,8 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
 
 extern "C" int darask_ggml_grouped_status(unsigned* host_status, cudaStream_t st) {
   if (!host_status) return cudaErrorInvalidValue;
-  void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, g_ggml_grouped_status);
+  unsigned* p = nullptr;
+  cudaError_t e = status_word(&p);
   if (!e) e = cudaMemcpyAsync(host_status, p, 4, cudaMemcpyDeviceToHost, st);
   if (!e) e = cudaMemsetAsync(p, 0, 4, st);
   return e ? e : cudaStreamSynchronize(st);

@@ -62,7 +62,7 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
                                                   x_scales.shape[1] < kb)):
         raise ValueError(f"codes come with x_scales float32 [{m}, {kb}], float rows without")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or (torch.bfloat16 if codes else x.dtype), device=x.device)
+        out = x.new_empty((m, n), dtype=out_dtype or (torch.bfloat16 if codes else x.dtype))
     elif tuple(out.shape) != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be [{m}, {n}]")
     out_ty = _lib.float_type(out.dtype)
@@ -84,10 +84,10 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
             return linear(x, w, w_scales, x_scales, swiglu, None, out)
     lib = _lib.lib()
     nbytes = lib.darask_fp8_linear_workspace_bytes(m, n, k, ty)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     d = _lib.DaraskFp8Linear(m, n, k, xp, ty, ldx, x_scales.data_ptr() if codes else None, ldxs, 1 if swiglu else 0, wp, ldw,
                              w_scales.data_ptr(), ldws, out.data_ptr(), out_ty, ldo, scratch.data_ptr() if nbytes else None, nbytes)
-    _lib.check(lib.darask_fp8_linear(ctypes.byref(d), torch.cuda.current_stream().cuda_stream), "darask_fp8_linear")
+    _lib.check(lib.darask_fp8_linear(ctypes.byref(d), _lib.current_stream(dev)), "darask_fp8_linear")
     return out
 
 

@@ -57,7 +57,7 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
         rows = assignments.numel()
     width = n * len(data)
     if out is None:
-        out = torch.empty((rows, width), dtype=out_dtype or x.dtype, device=x.device)
+        out = x.new_empty((rows, width), dtype=out_dtype or x.dtype)
     elif tuple(out.shape) != (rows, width) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be [{rows}, {width}]")
     out_ty = _lib.float_type(out.dtype)
@@ -74,12 +74,12 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
             return grouped_gemm(x, ranges, weight, up, assignments, topk, swiglu, None, out)
     lib = _lib.lib()
     nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty, 1 if swiglu else 0)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    scratch = x.new_empty(nbytes, dtype=torch.uint8)
     d = _lib.DaraskGgmlGrouped(groups, n, k, rows, ranges.data_ptr(), x.data_ptr(), ty, ldx, x.shape[0],
                                assignments.data_ptr() if assignments is not None else None, topk, 1 if swiglu else 0,
                                data[0].data_ptr(), data[1].data_ptr() if up is not None else None, weight.ty,
                                out.data_ptr(), out_ty, ldo, scratch.data_ptr(), nbytes)
-    _lib.check(lib.darask_ggml_grouped_gemm(ctypes.byref(d), torch.cuda.current_stream().cuda_stream), "darask_ggml_grouped_gemm")
+    _lib.check(lib.darask_ggml_grouped_gemm(ctypes.byref(d), _lib.current_stream(dev)), "darask_ggml_grouped_gemm")
     return out
 
 
