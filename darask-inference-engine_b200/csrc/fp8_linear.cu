@@ -41,20 +41,43 @@ __global__ void __launch_bounds__(256) fp8_linear_quant_kernel(const RowSource s
   reinterpret_cast<uint32_t*>(codes)[w * 32 + lane] = out;
 }
 
-// What a call runs. `fused` (rows quantized in the product's launch) depends on m and k alone, as the workspace does.
+// What a call runs. `fused` (rows quantized in the product's launch) depends on m and k alone, as the workspace does: one launch less
+// (4.9 against 5.0 us on the device for 6 rows of 2048 x 2048, 9.2 against 7.8 for 8 of 4096 x 4096, and 4 us less on the host).
 struct LinearPlan { int nt, splits; bool fused, tile; };
-static bool linear_fused(int m, int kb, bool codes) { return !codes && m <= 16 && kb <= 8 * kFsResident; }
+static bool linear_small(int m, int kb) { return m <= 8 && kb <= 8 * kFsResident; }
+// Rows of x per tile, blocks per cluster and kind of kernel by the time they are expected to take, in ns. The weights are fitted to a
+// sweep over 17 to 1024 rows of matrices from 1024 x 1536 to 8192 x 4096: a 128-column block of k takes 310, 390, 510 or 780 ns with
+// 16, 32, 64 or 128 rows (1.3 times as long where two blocks share an SM), joining S parts 450 S (1 + NT / 64), a 256 x 256 tile of the
+// pair kernel 550 ns per block of k and 900 more to start. (4096 x 4096, 256 rows: 128 rows in two parts 18.7 us, 32 rows undivided
+// 19.6, pairs 22.0; 512 rows: pairs 23.2, 128 rows 30.5.)
 static LinearPlan linear_plan(int m, int n, int kb, bool codes) {
-  LinearPlan p;
-  const int sms = sm_count();
-  p.fused = linear_fused(m, kb, codes);
-  // 256 x 256 tiles once they occupy half of the pairs of SMs
-  p.tile = m > 128 && (long long)((n + 255) / 256) * ((m + 255) / 256) * 4 >= sms;
-  p.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-  const long long tiles = (long long)((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
-  p.splits = 1;
-  while (p.splits < 8 && p.splits * 2 <= kb && (tiles * p.splits * 2 <= sms || (p.fused && (kb + p.splits - 1) / p.splits > kFsResident)))
-    p.splits *= 2;
+  LinearPlan p = {};
+  const long long sms = sm_count() > 1 ? sm_count() : 148;
+  const long long tiles_n = (n + 127) / 128;
+  if (linear_small(m, kb)) {             // codes are divided the same way: they give the same bits as the rows they came from
+    p.fused = !codes;
+    p.nt = 16;
+    p.splits = 1;
+    while (p.splits < 8 && p.splits * 2 <= kb && (tiles_n * p.splits * 2 <= 2 * sms || (kb + p.splits - 1) / p.splits > kFsResident)) p.splits *= 2;
+    return p;
+  }
+  long long best = -1;
+  for (int nt = 16, unit = 0; nt <= 128; nt *= 2, ++unit) {
+    static const int kUnit[4] = {310, 390, 510, 780};
+    if (nt > 16 && nt / 2 >= m) break;                 // no wider than the rows need
+    const long long tiles = tiles_n * ((m + nt - 1) / nt);
+    for (int splits = 1; splits <= 8 && splits <= kb; splits *= 2) {
+      const long long blocks = tiles * splits, slots = nt <= 32 ? 2 * sms : sms, kbs = (kb + splits - 1) / splits;
+      long long cost = (blocks + slots - 1) / slots * kbs * kUnit[unit];
+      if (blocks > sms && nt <= 32) cost = cost * 13 / 10;
+      if (splits > 1) cost += 450ll * splits * (64 + nt) / 64;
+      if (best < 0 || cost < best) { best = cost; p.nt = nt; p.splits = splits; }
+    }
+  }
+  if (m > 128) {
+    const long long tiles = (long long)((n + 255) / 256) * ((m + 255) / 256), pairs = sms / 2;
+    p.tile = 900 + (tiles + pairs - 1) / pairs * kb * 550 < best;
+  }
   return p;
 }
 
@@ -109,7 +132,7 @@ using namespace dmoe;
 extern "C" size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_ty) {
   if (m < 1 || n < 1 || k < 1 || x_ty == DARASK_E4M3) return 0;
   const size_t kb = (size_t(k) + 127) / 128;
-  if (linear_fused(m, int(kb), false)) return 0;
+  if (linear_small(m, int(kb))) return 0;
   return round_up(size_t(m) * kb * 128, 256) + round_up(size_t(m) * kb * 4, 256);
 }
 
