@@ -70,7 +70,7 @@ class DaraskFp8Linear(ctypes.Structure):
         ("m", c_int), ("n", c_int), ("k", c_int),
         ("x", c_void_p), ("x_ty", c_int), ("ldx", c_longlong), ("x_scales", c_void_p), ("ld_xs", c_longlong), ("swiglu", c_int),
         ("w", c_void_p), ("ldw", c_longlong), ("w_scales", c_void_p), ("ld_ws", c_longlong),
-        ("out", c_void_p), ("out_ty", c_int), ("ldo", c_longlong), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("out", c_void_p), ("out_ty", c_int), ("ldo", c_longlong), ("add", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
@@ -167,6 +167,8 @@ _SIGNATURES = {
     "kogarashi_moe_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "kogarashi_moe_workspace_init": (c_int, [c_void_p, c_size_t, c_void_p]),
     "kogarashi_moe_layer": (c_int, [ctypes.POINTER(KogarashiMoe), c_void_p]),
+    "kogarashi_moe_prefill_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "kogarashi_moe_prefill": (c_int, [ctypes.POINTER(KogarashiMoe), c_int, c_void_p]),
     "kogarashi_moe_set_single_launch": (c_int, [c_int]),
     "kogarashi_moe_static_scratch_bytes": (c_size_t, []),
     "kogarashi_moe_layer_static": (c_int, [ctypes.POINTER(KogarashiMoe), c_void_p]),

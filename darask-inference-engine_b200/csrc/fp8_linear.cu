@@ -107,8 +107,8 @@ static cudaError_t launch_tile(const DaraskFp8Linear* d, const FsArgs& s, const 
   const bool aligned = reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->ldo * es % 16 == 0 && d->n * es % 16 == 0;
   FtArgs a = {};
   a.m = d->m; a.n = d->n; a.kb = s.kb; a.xs = s.xs; a.ld_xs = s.ld_xs; a.ws = s.ws; a.ld_ws = s.ld_ws;
-  a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo; a.status = s.status;
-  a.tma_store = aligned && byte_map(&mo, d->out, d->m, d->n * es, d->ldo * es, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B, unsigned(es));
+  a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo; a.add = d->add; a.status = s.status;
+  a.tma_store = aligned && !d->add && byte_map(&mo, d->out, d->m, d->n * es, d->ldo * es, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B, unsigned(es));
   if (!a.tma_store) mo = mx;            // not used
   a.tiles_m = (d->m + 255) / 256; a.tiles_n = (d->n + 255) / 256;
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffll) return cudaErrorInvalidValue;
@@ -140,7 +140,7 @@ static bool linear_ok(const DaraskFp8Linear* d) {
   if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->m > (1 << 24) || d->n > (1 << 24) || d->k > (1 << 20)) return false;
   if (!d->w || !d->w_scales || reinterpret_cast<uintptr_t>(d->w) % 16 || d->ldw % 16 || d->ldw < d->k) return false;
   const long long kb = (d->k + 127) / 128;
-  if (d->ld_ws < kb || !row_type_bytes(d->out_ty) || d->ldo < d->n) return false;
+  if (d->ld_ws < kb || !row_type_bytes(d->out_ty) || d->ldo < d->n || (d->add && d->out_ty != DARASK_GGML_F32)) return false;
   if (d->m == 0) return true;
   if (!d->x || !d->out || reinterpret_cast<uintptr_t>(d->out) % row_type_bytes(d->out_ty)) return false;
   if (d->x_ty == DARASK_E4M3)
@@ -165,6 +165,7 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
   a.m = d->m; a.n = d->n; a.kb = kb;
   a.ws = d->w_scales; a.ld_ws = d->ld_ws;
   a.out = d->out; a.out_ty = d->out_ty; a.ldo = d->ldo;
+  a.add = d->add;
   a.tiles_n = (d->n + 127) / 128;
   a.status = status;
   a.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, codes ? 0 : row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};

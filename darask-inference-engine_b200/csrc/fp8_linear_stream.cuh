@@ -32,6 +32,7 @@ struct FsArgs {
   void* out;
   int out_ty;
   long long ldo;
+  int add;                                   // on top of what out holds
   int tiles_n;                               // ceil(n/128)
   unsigned* status;
 };
@@ -97,7 +98,7 @@ DEVI void fs_join(const FsArgs& a, float* part, uint32_t rank, int n0, int t0) {
       const size_t at = size_t(t0 + c) * size_t(a.ldo) + col;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (col + q < a.n) store_elem(a.out, a.out_ty, at + q, y[q]);
+        if (col + q < a.n) store_elem(a.out, a.out_ty, at + q, y[q], a.add);
     }
   }
 }
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_linear_strea
     if (warp >= 4 && col < a.n) {
 #pragma unroll
       for (int c = 0; c < NT; ++c)
-        if (t0 + c < a.m) store_elem(a.out, a.out_ty, size_t(t0 + c) * size_t(a.ldo) + col, acc[c]);
+        if (t0 + c < a.m) store_elem(a.out, a.out_ty, size_t(t0 + c) * size_t(a.ldo) + col, acc[c], a.add);
     }
   } else {
     float* part = reinterpret_cast<float*>(ring);                  // [NT][128]: every copy into the ring has been read

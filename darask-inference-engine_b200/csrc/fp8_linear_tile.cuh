@@ -33,6 +33,7 @@ struct FtArgs {
   void* out;
   int out_ty;
   long long ldo;
+  int add;                    // on top of what out holds (not with tma_store)
   int tma_store;              // the output's rows can be written by TMA
   int tiles_m, tiles_n;       // of 256
   unsigned* status;
@@ -231,7 +232,7 @@ fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             for (int c = lane; c < per && col + c < a.n; c += 32) {
               const uint8_t* src = mine + r * 128 + (((c * es >> 4) ^ (r & 7)) << 4) + ((c * es) & 15);
               const size_t at = size_t(r0 + r) * size_t(a.ldo) + size_t(col + c);
-              if (es == 4) static_cast<float*>(a.out)[at] = *reinterpret_cast<const float*>(src);
+              if (es == 4) store_elem(a.out, a.out_ty, at, *reinterpret_cast<const float*>(src), a.add);
               else static_cast<unsigned short*>(a.out)[at] = *reinterpret_cast<const unsigned short*>(src);
             }
           __syncwarp();

@@ -207,6 +207,110 @@ static cudaError_t launch_fused(const FusedArgs& a, int smem_bytes, cudaStream_t
                    : launch_pdl(k4, dim3(sm_count()), dim3(kFusedThreads), size_t(smem_bytes), st, a);
 }
 
+// ---- the layer for prompts: expert products grouped by expert (ggml_grouped.cu) ---------------------------------------
+// logits[t][row] = W[row] . x[t] (+ bias): 64 tokens x 64 router rows per block, 4 x 4 per thread, float32 throughout. Row E is the
+// shared expert's gate, which goes to `extra_out`.
+struct PrefillRouterArgs {
+  const void* w; const void* extra; const float* bias; const float* x;
+  float* logits; float* extra_out;
+  int hidden, experts, tokens, first;                  // first: first row (experts: only the gate)
+};
+template <typename WT>
+__global__ void __launch_bounds__(256) prefill_router_kernel(const PrefillRouterArgs a) {
+  __shared__ float xt[32][68], wt[32][68];             // [k][token], [k][row]
+  pdl_wait();
+  pdl_launch();
+  const int t0 = blockIdx.x * 64, r0 = a.first + blockIdx.y * 64, rows = a.experts + (a.extra ? 1 : 0);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4] = {};
+  for (int k0 = 0; k0 < a.hidden; k0 += 32) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < 64 * 32; e += 256) {
+      const int i = e >> 5, k = e & 31;
+      xt[k][i] = t0 + i < a.tokens ? __ldcg(a.x + size_t(t0 + i) * a.hidden + k0 + k) : 0.f;
+      const int r = r0 + i;
+      wt[k][i] = r < a.experts ? to_f32(static_cast<const WT*>(a.w)[size_t(r) * a.hidden + k0 + k])
+                 : r < rows    ? to_f32(static_cast<const WT*>(a.extra)[k0 + k]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const float4 p = *reinterpret_cast<const float4*>(&xt[k][ty * 4]), q = *reinterpret_cast<const float4*>(&wt[k][tx * 4]);
+      const float pv[4] = {p.x, p.y, p.z, p.w}, qv[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(pv[i], qv[j], acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = t0 + ty * 4 + i, r = r0 + tx * 4 + j;
+      if (t >= a.tokens || r >= rows) continue;
+      if (r == a.experts) a.extra_out[t] = acc[i][j];
+      else a.logits[size_t(t) * a.experts + r] = acc[i][j] + (a.bias ? a.bias[r] : 0.f);
+    }
+}
+// position[assignment] = dispatch row, and the one range of the shared expert
+__global__ void __launch_bounds__(256) prefill_position_kernel(const unsigned* assignments, const int* counters, unsigned* position, unsigned* shared_range,
+                                                               unsigned tokens) {
+  pdl_wait();
+  pdl_launch();
+  const unsigned i = blockIdx.x * 256 + threadIdx.x;
+  if (i == 0) { shared_range[0] = tokens; shared_range[1] = 0; }
+  if (i < unsigned(__ldcg(counters + 1))) position[__ldcg(assignments + i)] = i;
+}
+// x[t][i] += sum_s p[t][s] y[position[t][s]][i] + sigmoid(sg[t]) ysh[t][i], in the order of kogarashi_combine_kernel; a dropped route has no row
+__global__ void __launch_bounds__(256) prefill_combine_kernel(float* x, const float* y, const float* ysh, const float* prob, const unsigned* position,
+                                                              const float* sg, int hidden, int topk, unsigned rows) {
+  pdl_wait();
+  pdl_launch();
+  const int i = blockIdx.y * 256 + threadIdx.x, t = blockIdx.x;
+  if (i >= hidden) return;
+  float v = 0.f;
+  for (int s = 0; s < topk; ++s) {
+    const unsigned p = __ldcg(position + size_t(t) * topk + s);
+    if (p < rows) v = fmaf(__ldcg(prob + size_t(t) * topk + s), __ldcg(y + size_t(p) * hidden + i), v);
+  }
+  if (ysh) v += sigmoid_precise(__ldcg(sg + t)) * __ldcg(ysh + size_t(t) * hidden + i);
+  x[size_t(t) * hidden + i] += v;
+}
+
+// The words in front lie where `carve` has them, so that kogarashi_moe_status finds the status word.
+struct PrefillWs {
+  int* counters; unsigned* status; int* active; unsigned* ranges; unsigned* shared_range; unsigned* assignments; unsigned* position; int* perm;
+  float* sg; float* gu; float* y; float* ysh; void* products; size_t products_bytes, bytes;
+};
+static PrefillWs carve_prefill(void* base, int hidden, int inter, int experts, int topk, int tokens) {
+  PrefillWs w;
+  uint8_t* p = static_cast<uint8_t*>(base);
+  size_t off = 0;
+  auto take = [&](size_t bytes) { uint8_t* q = p ? p + off : nullptr; off = align_up(off + bytes, 256); return q; };
+  const size_t routes = size_t(tokens) * topk;
+  take(256);
+  w.counters = reinterpret_cast<int*>(take(16));
+  take(4);
+  w.status = reinterpret_cast<unsigned*>(take(4));
+  w.shared_range = reinterpret_cast<unsigned*>(take(8));
+  w.active = reinterpret_cast<int*>(take(size_t(experts) * 4));
+  w.ranges = reinterpret_cast<unsigned*>(take(size_t(experts) * 8));
+  w.assignments = reinterpret_cast<unsigned*>(take(routes * 4));
+  w.position = reinterpret_cast<unsigned*>(take(routes * 4));
+  w.perm = reinterpret_cast<int*>(take(darask_moe_permute_scratch_bytes(tokens, topk, experts)));
+  w.sg = reinterpret_cast<float*>(take(size_t(tokens) * 4));
+  w.gu = reinterpret_cast<float*>(take(routes * 2 * inter * 4));
+  w.y = reinterpret_cast<float*>(take(routes * hidden * 4));
+  w.ysh = reinterpret_cast<float*>(take(size_t(tokens) * hidden * 4));
+  const size_t up = darask_ggml_grouped_workspace_bytes((long long)routes, hidden, DARASK_GGML_F32, 0);
+  const size_t down = darask_ggml_grouped_workspace_bytes((long long)routes, inter, DARASK_GGML_F32, 1);
+  w.products_bytes = up > down ? up : down;
+  w.products = take(w.products_bytes);
+  w.bytes = off;
+  return w;
+}
+
 static thread_local bool g_force_staged = false;    // host-thread-local: take the staged launches for one token too
 
 }  // namespace dmoe
@@ -327,6 +431,61 @@ extern "C" int kogarashi_moe_layer(const KogarashiMoe* d, cudaStream_t st) {
   // 4. combine
   return launch_pdl(kogarashi_combine_kernel, dim3((H + 255) / 256, T), dim3(256), 0, st, d->x, (const float*)w.y,
                     (const float*)d->prob, (const float*)w.sg, H, K, T, shared ? 1 : 0);
+}
+
+extern "C" size_t kogarashi_moe_prefill_workspace_bytes(int hidden, int inter, int experts, int topk, int tokens) {
+  if (hidden < 256 || hidden % 256 || inter < 256 || inter % 256 || experts < 1 || topk < 1 || tokens < 1) return 0;
+  return carve_prefill(nullptr, hidden, inter, experts, topk, tokens).bytes;
+}
+
+extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cudaStream_t st) {
+  if (!descriptor_ok(d) || !d->workspace || reinterpret_cast<uintptr_t>(d->workspace) % 256) return cudaErrorInvalidValue;
+  const int H = d->hidden, F = d->inter, E = d->experts, K = d->topk, T = d->tokens;
+  if ((long long)T * K > (1ll << 27) || d->workspace_bytes < kogarashi_moe_prefill_workspace_bytes(H, F, E, K, T)) return cudaErrorInvalidValue;
+  const bool shared = d->sh_gate_w != nullptr;
+  const PrefillWs w = carve_prefill(d->workspace, H, F, E, K, T);
+  const long long routes = (long long)T * K;
+  cudaError_t e = cudaMemsetAsync(d->workspace, 0, 1280, st);           // counters, status
+  // a route that the permutation drops has no row: its position stays out of range
+  if (!e) e = cudaMemsetAsync(w.position, 0xff, size_t(routes) * 4, st);
+  if (!e && d->norm_w)
+    e = launch_pdl(kogarashi_entry_kernel, dim3(T), dim3(256), size_t(0), st, d->x, d->attn_out, d->norm_w, d->n, H, d->norm_eps);
+  if (e) return e;
+  // 1. router projection (or the shared gate alone), top-k, permutation
+  const int first = logits_given ? E : 0, rows = E + (shared ? 1 : 0) - first;
+  if (rows > 0) {
+    const PrefillRouterArgs r{d->router_w, shared ? d->sh_inp_w : nullptr, d->router_bias, d->n, d->logits, w.sg, H, E, T, first};
+    const dim3 grid((T + 63) / 64, (rows + 63) / 64);
+    if (d->router_ty == DARASK_GGML_F32) e = launch_pdl(prefill_router_kernel<float>, grid, dim3(256), 0, st, r);
+    else if (d->router_ty == DARASK_GGML_BF16) e = launch_pdl(prefill_router_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, r);
+    else e = launch_pdl(prefill_router_kernel<__half>, grid, dim3(256), 0, st, r);
+    if (e) return e;
+  }
+  if ((e = (cudaError_t)darask_route_topk(DARASK_ROUTE_KOGARASHI, d->logits, E, E, K, T, nullptr, 1.f, d->ids, d->prob, nullptr, st))) return e;
+  if ((e = (cudaError_t)darask_moe_permute_large(d->ids, T, K, E, w.assignments, w.ranges, w.active, w.counters, w.status, w.perm,
+                                                 darask_moe_permute_scratch_bytes(T, K, E), st))) return e;
+  if ((e = launch_pdl(prefill_position_kernel, dim3(unsigned((routes + 255) / 256)), dim3(256), 0, st, (const unsigned*)w.assignments,
+                      (const int*)w.counters, w.position, w.shared_range, unsigned(T)))) return e;
+  // 2. gate | up of every route, SwiGLU and down; the same for the shared expert, one group of all tokens
+  DaraskGgmlGrouped g = {};
+  auto products = [&](int groups, long long count, const unsigned* ranges, const unsigned* assignments, const void* gate, const void* up, const void* down,
+                      float* out) -> cudaError_t {
+    g = DaraskGgmlGrouped{};
+    g.groups = groups; g.n = F; g.k = H; g.rows = count; g.ranges = ranges;
+    g.x = d->n; g.x_ty = DARASK_GGML_F32; g.ldx = H; g.x_rows = T; g.assignments = assignments; g.topk = K;
+    g.w = gate; g.w_up = up; g.w_ty = d->gate_ty;
+    g.out = w.gu; g.out_ty = DARASK_GGML_F32; g.ldo = 2ll * F; g.workspace = w.products; g.workspace_bytes = w.products_bytes;
+    const int r = darask_ggml_grouped_gemm(&g, st);
+    if (r) return (cudaError_t)r;
+    g.n = H; g.k = F; g.x = w.gu; g.ldx = 2ll * F; g.x_rows = count; g.assignments = nullptr; g.swiglu = 1;
+    g.w = down; g.w_up = nullptr; g.w_ty = d->down_ty; g.out = out; g.ldo = H;
+    return (cudaError_t)darask_ggml_grouped_gemm(&g, st);
+  };
+  if ((e = products(E, routes, w.ranges, w.assignments, d->gate_w, d->up_w, d->down_w, w.y))) return e;
+  if (shared && (e = products(1, T, w.shared_range, nullptr, d->sh_gate_w, d->sh_up_w, d->sh_down_w, w.ysh))) return e;
+  // 3. combine into the residual stream
+  return launch_pdl(prefill_combine_kernel, dim3(T, (H + 255) / 256), dim3(256), 0, st, d->x, (const float*)w.y, shared ? (const float*)w.ysh : (const float*)nullptr,
+                    (const float*)d->prob, (const unsigned*)w.position, (const float*)w.sg, H, K, unsigned(routes));
 }
 
 // ---- stand-alone pieces (also used by the parity tests) ------------------------------------------

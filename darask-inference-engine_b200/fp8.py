@@ -39,12 +39,12 @@ def grouped_gemm(a_codes, a_scales, ranges, w0, sw0, w1=None, sw1=None, quantize
     return (out, scales) if mode == 2 else out
 
 
-def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None):
+def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None, add=False):
     """Dense product in block-scaled FP8, x [m, k] -> [m, n].  w uint8 (e4m3 codes) [n, k], w_scales float32 [ceil(n/128), >= ceil(k/128)]
     (``quantize.fp8_block``).  x float32, float16 or bfloat16 is quantized by the call with one scale per row and 128 columns; with
     `swiglu` its rows hold gate | up ([m, 2k]) and silu(gate) * up is quantized.  x uint8 holds e4m3 codes, with x_scales float32
     [m, >= ceil(k/128)] (``quantize.fp8_act``).  Sums are float32; `out_dtype` (float32, float16, bfloat16) defaults to x's type, or
-    bfloat16 for codes.  Rows may be strided; rows of w and of codes start on 16-byte boundaries.  Any m, including 0; k as w has it.
+    bfloat16 for codes.  With `add` the product is added to what a float32 `out` holds.  Rows may be strided; rows of w and of codes start on 16-byte boundaries.  Any m, including 0; k as w has it.
     Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
     if w.dim() != 2 or w.dtype is not torch.uint8 or w_scales.dim() != 2 or w_scales.dtype is not torch.float32:
         raise ValueError("w must be uint8 [n, k] and w_scales float32 [n blocks, k blocks]")
@@ -61,6 +61,8 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
     if codes is (x_scales is None) or (codes and (x_scales.dim() != 2 or x_scales.dtype is not torch.float32 or x_scales.shape[0] != m or
                                                   x_scales.shape[1] < kb)):
         raise ValueError(f"codes come with x_scales float32 [{m}, {kb}], float rows without")
+    if add and (out is None or out.dtype is not torch.float32):
+        raise ValueError("add needs a float32 out to add to")
     if out is None:
         out = x.new_empty((m, n), dtype=out_dtype or (torch.bfloat16 if codes else x.dtype))
     elif tuple(out.shape) != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
@@ -81,12 +83,12 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
         return out
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return linear(x, w, w_scales, x_scales, swiglu, None, out)
+            return linear(x, w, w_scales, x_scales, swiglu, None, out, add)
     lib = _lib.lib()
     nbytes = lib.darask_fp8_linear_workspace_bytes(m, n, k, ty)
     scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     d = _lib.DaraskFp8Linear(m, n, k, xp, ty, ldx, x_scales.data_ptr() if codes else None, ldxs, 1 if swiglu else 0, wp, ldw,
-                             w_scales.data_ptr(), ldws, out.data_ptr(), out_ty, ldo, scratch.data_ptr() if nbytes else None, nbytes)
+                             w_scales.data_ptr(), ldws, out.data_ptr(), out_ty, ldo, 1 if add else 0, scratch.data_ptr() if nbytes else None, nbytes)
     _lib.check(lib.darask_fp8_linear(ctypes.byref(d), _lib.current_stream(dev)), "darask_fp8_linear")
     return out
 
@@ -109,9 +111,24 @@ class Fp8MoeLayer:
         self.ids = torch.empty(max_tokens, topk, dtype=torch.int32, device=self.device)
         self.prob = torch.empty(max_tokens, topk, dtype=torch.float32, device=self.device)
         self.w = {}
+        self.shared = None
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
+
+    def load_shared(self, gate, up, down) -> None:
+        """An always-on shared expert in the same format, added to the routed sum (hayate cu/glm53/decode.cu:55-59): gate and up
+        (payload uint8 [F, H], scales float32 [F/128, H/128]), down (payload [H, F], scales [H/128, F/128]); F a multiple of 128 of
+        its own.  Its products are the dense ones of `linear`: gate | up in one, SwiGLU and the quantizer in front of down."""
+        f = gate[0].shape[0]
+        if f < 128 or f % 128:
+            raise ValueError("the shared expert's intermediate width must be a multiple of 128")
+        for name, (p, s), (n, k) in (("gate", gate, (f, self.hidden)), ("up", up, (f, self.hidden)), ("down", down, (self.hidden, f))):
+            if tuple(p.shape) != (n, k) or tuple(s.shape) != (n // 128, k // 128):
+                raise ValueError(f"shared {name}: expected payload [{n},{k}] and scales [{n // 128},{k // 128}]")
+        put = lambda t, ty: t.to(self.device, ty).contiguous()
+        self.shared = (put(torch.cat([gate[0], up[0]]), torch.uint8), put(torch.cat([gate[1], up[1]]), torch.float32),
+                       put(down[0], torch.uint8), put(down[1], torch.float32))
 
     def load(self, name: str, payload: torch.Tensor, scales: torch.Tensor) -> None:
         """name in gate|up|down; payload uint8 [E, n, k]; scales float32 [E, n/128, k/128]."""
@@ -121,7 +138,7 @@ class Fp8MoeLayer:
         self.w[name] = (payload.to(self.device, torch.uint8).contiguous(), scales.to(self.device, torch.float32).contiguous())
 
     def forward(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
-        """x bf16 [T,H], logits float32 [T,E] -> float32 [T,H] (the routed experts' weighted sum)."""
+        """x bf16 [T,H], logits float32 [T,E] -> float32 [T,H] (the routed experts' weighted sum, and the shared expert if loaded)."""
         t = x.shape[0]
         if t > self.max_tokens or x.dtype != torch.bfloat16 or logits.dtype != torch.float32 or not x.is_contiguous() or not logits.is_contiguous():
             raise ValueError("x must be contiguous bf16 [T<=max_tokens,H], logits contiguous float32 [T,E]")
@@ -135,6 +152,9 @@ class Fp8MoeLayer:
         d.out, d.ids, d.prob = out.data_ptr(), self.ids.data_ptr(), self.prob.data_ptr()
         d.workspace, d.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
         _lib.check(_lib.lib().darask_fp8_moe_layer(ctypes.byref(d), self._stream()), "darask_fp8_moe_layer")
+        if self.shared is not None:
+            gu_w, gu_s, down_w, down_s = self.shared
+            linear(linear(x, gu_w, gu_s, out_dtype=torch.float32), down_w, down_s, swiglu=True, out=out, add=True)
         return out
 
     def status(self) -> int:

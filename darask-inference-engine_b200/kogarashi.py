@@ -143,8 +143,16 @@ class KogarashiMoeLayer:
             raise ValueError("token count / shape")
         if x.dtype != torch.float32 or n.dtype != torch.float32 or not x.is_contiguous() or not n.is_contiguous():
             raise ValueError("x and n must be contiguous float32")
+        d = self._descriptor(x, n, attn_out, norm_w, eps)
+        d.logits, d.ids, d.prob = self.logits.data_ptr(), self.ids.data_ptr(), self.prob.data_ptr()
+        d.workspace, d.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        _lib.check(_lib.lib().kogarashi_moe_layer(ctypes.byref(d), self._stream()), "kogarashi_moe_layer")
+        return x
+
+    def _descriptor(self, x, n, attn_out, norm_w, eps):
+        """The call's descriptor but for its routes and its workspace."""
         d = _lib.KogarashiMoe()
-        d.hidden, d.inter, d.experts, d.topk, d.tokens = self.hidden, self.inter, self.experts, self.topk, t
+        d.hidden, d.inter, d.experts, d.topk, d.tokens = self.hidden, self.inter, self.experts, self.topk, n.shape[0]
         d.router_w, d.router_ty = self._w("ffn_gate_inp.weight")
         d.router_bias = self.router_bias.data_ptr() if self.router_bias is not None else None
         d.gate_w, d.gate_ty = self._w("ffn_gate_exps.weight")
@@ -162,10 +170,33 @@ class KogarashiMoeLayer:
             d.attn_out = attn_out.data_ptr() if attn_out is not None else None
         elif attn_out is not None:
             raise ValueError("attn_out needs norm_w")
-        d.logits, d.ids, d.prob = self.logits.data_ptr(), self.ids.data_ptr(), self.prob.data_ptr()
-        d.workspace, d.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
-        _lib.check(_lib.lib().kogarashi_moe_layer(ctypes.byref(d), self._stream()), "kogarashi_moe_layer")
-        return x
+        return d
+
+    def prefill(self, x: torch.Tensor, n: torch.Tensor, logits: torch.Tensor | None = None, attn_out: torch.Tensor | None = None,
+                norm_w: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+        """`forward` for prompts and large batches (any number of tokens, `max_tokens` or not): the expert products run grouped by
+        expert (`grouped_gemm`) instead of in passes of eight tokens.  `logits` float32 [T, E]: routes by these instead of projecting
+        them.  Scratch and routes belong to the call; returns x (updated in place), ids int32 [T, k], prob float32 [T, k]."""
+        t = n.shape[0]
+        if t < 1 or n.shape != x.shape or n.shape[1] != self.hidden:
+            raise ValueError("token count / shape")
+        if x.dtype != torch.float32 or n.dtype != torch.float32 or not x.is_contiguous() or not n.is_contiguous():
+            raise ValueError("x and n must be contiguous float32")
+        if logits is not None and (logits.dtype != torch.float32 or tuple(logits.shape) != (t, self.experts) or not logits.is_contiguous()):
+            raise ValueError("logits must be contiguous float32 [T, E]")
+        lib = _lib.lib()
+        d = self._descriptor(x, n, attn_out, norm_w, eps)
+        given = logits is not None
+        if not given:
+            logits = x.new_empty((t, self.experts))
+        ids, prob = x.new_empty((t, self.topk), dtype=torch.int32), x.new_empty((t, self.topk))
+        d.logits, d.ids, d.prob = logits.data_ptr(), ids.data_ptr(), prob.data_ptr()
+        nbytes = lib.kogarashi_moe_prefill_workspace_bytes(self.hidden, self.inter, self.experts, self.topk, t)
+        scratch = x.new_empty(nbytes, dtype=torch.uint8)
+        d.workspace, d.workspace_bytes = scratch.data_ptr(), nbytes
+        with torch.cuda.device(self.device):
+            _lib.check(lib.kogarashi_moe_prefill(ctypes.byref(d), 1 if given else 0, self._stream()), "kogarashi_moe_prefill")
+        return x, ids, prob
 
     def forward_host(self, x_host: torch.Tensor, n_host: torch.Tensor, out_host: torch.Tensor | None = None) -> torch.Tensor:
         """The layer for activations that live in host memory: x [T,H] and n [T,H] float32 on the CPU in, the updated

@@ -128,6 +128,13 @@ size_t kogarashi_moe_workspace_bytes(int hidden, int inter, int experts, int top
  * CTAs of the one-token launch hand values to each other: a workspace that was never cleared may hold a stale tag) */
 int kogarashi_moe_workspace_init(void* workspace, size_t bytes, darask_stream_t stream);
 int kogarashi_moe_layer(const KogarashiMoe* desc /* host */, darask_stream_t stream);
+/* The same layer for prompts and large batches: the same descriptor and results (routing from the same logits, sums in another
+ * order), the expert products through darask_ggml_grouped_gemm instead of passes of eight tokens.  `workspace` holds
+ * kogarashi_moe_prefill_workspace_bytes(...) bytes, 256-byte aligned, needs no initialisation and belongs to the call;
+ * kogarashi_moe_status reads its status word.  logits_given != 0: desc->logits holds the logits (router_bias included) and the
+ * router projection is left out; the shared expert's gate is projected all the same. */
+size_t kogarashi_moe_prefill_workspace_bytes(int hidden, int inter, int experts, int topk, int tokens);
+int kogarashi_moe_prefill(const KogarashiMoe* desc /* host */, int logits_given, darask_stream_t stream);
 /* One token with an F32 router and Q4_K gate/up runs as ONE persistent launch (router rows, top-k in every CTA,
  * gate/up, down and combine; the CTAs hand logits, products and rows to each other as tagged words with bounded
  * polling, the weight stream running through); other shapes take four launches.  enabled = 0 makes the calling host thread take the four launches for one token as well
@@ -390,6 +397,7 @@ int darask_fp8_ep_sum(float* out, const float* zr, int ranks, int tokens, int tc
  *            DARASK_E4M3: e4m3 codes with x_scales [m][ld_xs] (16-byte aligned rows).
  *   swiglu   float x only: rows hold gate | up (2k columns) and silu(gate) * up, in float32, is quantized.
  *   w        e4m3 [n][ldw], 16-byte aligned rows; w_scales float32 [ceil(n/128)][ld_ws], ld_ws >= ceil(k/128).
+ *   add      != 0 (float32 out only): the product is added to what out holds.
  *   ld*      row strides in elements.  out must not overlap an input.
  *   workspace  darask_fp8_linear_workspace_bytes(m, n, k, x_ty) bytes, 256-byte aligned (0 bytes: may be NULL), not shared by
  *            calls that can overlap; nothing has to be initialised and nothing is kept between calls.
@@ -403,7 +411,7 @@ typedef struct {
   int swiglu;
   const void* w; long long ldw;
   const float* w_scales; long long ld_ws;
-  void* out; int out_ty; long long ldo;
+  void* out; int out_ty; long long ldo; int add;
   void* workspace; size_t workspace_bytes;
 } DaraskFp8Linear;
 size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_ty);
