@@ -61,9 +61,11 @@ static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, c
 
 template <int KIND>
 static cudaError_t launch_rows(const GgRowsArgs& r, int parts, bool sums, cudaStream_t st) {
-  const auto kernel = parts == 2 ? (sums ? ggml_rows_kernel<KIND, true, true> : ggml_rows_kernel<KIND, true, false>)
-                                 : (sums ? ggml_rows_kernel<KIND, false, true> : ggml_rows_kernel<KIND, false, false>);
-  return launch_pdl(kernel, dim3(unsigned(r.rows)), dim3(kGgRowThreads), 0, st, r);
+  auto kernel = sums ? ggml_rows_kernel<KIND, false, true> : ggml_rows_kernel<KIND, false, false>;
+  if constexpr (KIND != 2 && KIND != 3)                  // plain 16-bit rows have one part
+    if (parts == 2) kernel = sums ? ggml_rows_kernel<KIND, true, true> : ggml_rows_kernel<KIND, true, false>;
+  const size_t smem = size_t(r.src.k < kGgRowHeld ? r.src.k : kGgRowHeld) * sizeof(float);
+  return launch_pdl(kernel, dim3(unsigned(r.rows)), dim3(kGgRowThreads), smem, st, r);
 }
 
 // f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
@@ -91,8 +93,8 @@ static bool grouped_ok(const DaraskGgmlGrouped* d) {
   const size_t eb = row_type_bytes(d->x_ty), ob = row_type_bytes(d->out_ty);
   if (!eb || !ob || d->ldx < (d->swiglu ? 2ll : 1ll) * d->k || d->ldo < (d->w_up ? 2ll : 1ll) * d->n) return false;
   if (d->assignments && d->topk < 1) return false;
-  // tiles of 128 rows x 128 columns are counted in 32 bits
-  if ((d->rows / 128 + d->groups) * ((d->n + 127) / 128) * 2 > 0x7fffffffll) return false;
+  // the tiles of one matrix or two are counted in 32 bits
+  if ((d->rows / (d->rows <= 32ll * d->groups ? 32 : 128) + d->groups) * ((d->n + 127) / 128) * (d->w_up ? 2 : 1) >= kGgMaxTiles) return false;
   if (d->rows == 0) return true;
   if (!d->ranges || !d->out || reinterpret_cast<uintptr_t>(d->out) % ob) return false;
   if (d->x_rows > 0 && (!d->x || reinterpret_cast<uintptr_t>(d->x) % eb)) return false;
@@ -125,11 +127,19 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
       !byte_map(m + 4, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !byte_map(m + 5, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 128, 32, CU_TENSOR_MAP_SWIZZLE_32B))
     return cudaErrorInvalidValue;
-  const int kind = d->swiglu || r.src.vec < (d->x_ty == DARASK_GGML_F32 ? 1 : 2) || d->ldx % (d->x_ty == DARASK_GGML_F32 ? 4 : 8)
-                       ? 0 : d->x_ty == DARASK_GGML_F32 ? 1 : d->x_ty == DARASK_GGML_F16 ? 2 : 3;
-  if ((e = kind == 0 ? launch_rows<0>(r, nx, !q6, st) : kind == 1 ? launch_rows<1>(r, nx, !q6, st) : kind == 2 ? launch_rows<2>(r, nx, !q6, st)
-                                                                                              : launch_rows<3>(r, nx, !q6, st)))
-    return e;
+  // eight columns at a time where the rows allow it
+  const bool whole = r.src.vec >= (d->x_ty == DARASK_GGML_F32 ? 1 : 2) && d->ldx % (d->x_ty == DARASK_GGML_F32 ? 4 : 8) == 0;
+  const int kind = !whole ? 0 : (d->x_ty == DARASK_GGML_F32 ? 1 : d->x_ty == DARASK_GGML_F16 ? 2 : 3) + (d->swiglu ? 3 : 0);
+  switch (kind) {
+    case 0: e = launch_rows<0>(r, nx, !q6, st); break;
+    case 1: e = launch_rows<1>(r, nx, !q6, st); break;
+    case 2: e = launch_rows<2>(r, nx, !q6, st); break;
+    case 3: e = launch_rows<3>(r, nx, !q6, st); break;
+    case 4: e = launch_rows<4>(r, nx, !q6, st); break;
+    case 5: e = launch_rows<5>(r, nx, !q6, st); break;
+    default: e = launch_rows<6>(r, nx, !q6, st);
+  }
+  if (e) return e;
   GgArgs a = {};
   a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);

@@ -23,6 +23,7 @@
 namespace dmoe {
 
 constexpr int kGgMaxGroups = 1024;
+constexpr int kGgMaxTiles = 1 << 30;                     // a call whose ranges do not overlap has fewer; two of them still add up in 32 bits
 
 struct GgArgs {
   const unsigned* ranges;                                // [groups][2]
@@ -86,17 +87,26 @@ struct GgRowsArgs {
   float* scale;                                          // [rows]
 };
 constexpr int kGgRowThreads = 128;
-constexpr int kGgRowHeld = 4;                            // groups of eight columns a thread keeps in registers (k <= 4096); longer rows are read twice
-// KIND: 0 any rows (four elements at a time, strides and SwiGLU as they come); 1 float32, 2 f16, 3 bf16 rows on 16-byte boundaries
+constexpr int kGgRowHeld = 4096;                         // columns that stay in shared memory between the passes; what is behind them is read twice
+// KIND: 0 any rows (four elements at a time, strides and SwiGLU as they come); rows on 16-byte boundaries: 1 float32, 2 f16, 3 bf16;
+// 4, 5, 6 the same three as gate | up halves. One loop of few registers for all: held in registers, rows of 2048 bf16 left room for
+// eight blocks per SM, and the code of unrolled SwiGLU products came through the instruction cache anew for every block (32768 rows:
+// 2048 bf16 53 us instead of 65, 2 x 768 float32 50 instead of 83).
 template <int KIND>
 DEVI void rows_load8(const RowSource& s, const void* at, long long row, int c, float (&v)[8]) {
-  if (KIND == 0) {
+  if constexpr (KIND == 0) {
     float a[4], b[4];
     row_source_load4(s, row, c, a);
     row_source_load4(s, row, c + 4, b);
 #pragma unroll
     for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
-  } else if (KIND == 1) {
+  } else if constexpr (KIND >= 4) {
+    float u[8];
+    rows_load8<KIND - 3>(s, at, row, c, v);
+    rows_load8<KIND - 3>(s, at, row, c + s.k, u);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = silu_mul(v[q], u[q]);
+  } else if constexpr (KIND == 1) {
     const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(at) + c);
     const float4 a = __ldcg(p), b = __ldcg(p + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -112,6 +122,8 @@ DEVI void rows_load8(const RowSource& s, const void* at, long long row, int c, f
 }
 template <int KIND, bool PARTS, bool SUMS>
 __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsArgs a) {
+  constexpr int kUnroll = KIND == 0 || KIND >= 4 ? 1 : 2;
+  extern __shared__ __align__(16) float row_smem[];      // [min(k, kGgRowHeld)]
   __shared__ uint32_t red[kGgRowThreads / 32];
   pdl_wait();
   pdl_launch();
@@ -120,28 +132,24 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
   long long row = i;
   if (a.assignments) row = __ldcg(a.assignments + i) / unsigned(a.topk);
   const bool exists = row < a.x_rows;
-  const void* at = KIND == 1 ? static_cast<const void*>(static_cast<const float*>(a.src.x) + row * a.src.ld)
-                             : static_cast<const void*>(static_cast<const unsigned short*>(a.src.x) + row * a.src.ld);      // KIND 0: unused
-  float held[kGgRowHeld][8];
+  const void* at = static_cast<const uint8_t*>(a.src.x) + row * a.src.ld * (KIND == 1 || KIND == 4 ? 4 : 2);       // KIND 0: unused
   uint32_t top = 0;
   auto scan = [&](const float (&v)[8]) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
   };
-#pragma unroll
-  for (int j = 0; j < kGgRowHeld; ++j) {
-    const int c = (j * kGgRowThreads + threadIdx.x) * 8;
-    if (exists && c < k) {
-      rows_load8<KIND>(a.src, at, row, c, held[j]);
-      scan(held[j]);
-    }
-  }
-  if (exists)
-    for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 8; c < k; c += kGgRowThreads * 8) {
+  if (exists) {
+#pragma unroll kUnroll
+    for (int c = threadIdx.x * 8; c < k; c += kGgRowThreads * 8) {
       float v[8];
       rows_load8<KIND>(a.src, at, row, c, v);
       scan(v);
+      if (c < kGgRowHeld) {
+        *reinterpret_cast<float4*>(row_smem + c) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(row_smem + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
     }
+  }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
@@ -187,16 +195,15 @@ __global__ void __launch_bounds__(kGgRowThreads) ggml_rows_kernel(const GgRowsAr
       }
     }
   };
-#pragma unroll
-  for (int j = 0; j < kGgRowHeld; ++j) {
-    const int c = (j * kGgRowThreads + threadIdx.x) * 8;
-    if (c < k) put(c, held[j]);
-  }
-  for (int c = (kGgRowHeld * kGgRowThreads + threadIdx.x) * 8; c < k; c += kGgRowThreads * 8) {
-    float v[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = 0.f;
-    if (live) rows_load8<KIND>(a.src, at, row, c, v);
+#pragma unroll 1
+  for (int c = threadIdx.x * 8; c < k; c += kGgRowThreads * 8) {         // what this thread has left there itself
+    float v[8] = {};
+    if (live && c < kGgRowHeld) {
+      const float4 p = *reinterpret_cast<const float4*>(row_smem + c), q = *reinterpret_cast<const float4*>(row_smem + c + 4);
+      v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+    } else if (live) {
+      rows_load8<KIND>(a.src, at, row, c, v);
+    }
     put(c, v);
   }
 }
@@ -303,15 +310,20 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   }
   __syncthreads();
   if (warp == 0) {                       // inclusive scan, consecutive groups per lane
+    // ranges that overlap can count more tiles than rows hold: the sum stops at kGgMaxTiles, groups behind it get none
     const int per = (a.groups + 31) / 32;
     int sum = 0;
-    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) sum += ends[g]; }
+    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) sum = min(sum + ends[g], kGgMaxTiles); }
     int run = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += t; }
-    int off = run - sum;
-    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) { off += ends[g]; ends[g] = off; } }
-    if (lane == 31) ends[a.groups] = run;
+    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run = min(run + t, kGgMaxTiles); }
+    int off = __shfl_up_sync(0xffffffffu, run, 1);
+    if (lane == 0) off = 0;
+    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) { off = min(off + ends[g], kGgMaxTiles); ends[g] = off; } }
+    if (lane == 31) {
+      ends[a.groups] = run;
+      if (run == kGgMaxTiles && blockIdx.x == 0) atomicOr(a.status, kStatusBadRoute);
+    }
   }
   tmem_fence_before();
   __syncthreads();

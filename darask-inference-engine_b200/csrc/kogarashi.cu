@@ -10,7 +10,9 @@
 #include "stream_launch.cuh"
 #include "gemv_launch.cuh"
 #include "decode_fused.cuh"
+#include "row_source.cuh"
 #include <cstdio>
+#include <type_traits>
 
 namespace dmoe {
 
@@ -208,50 +210,82 @@ static cudaError_t launch_fused(const FusedArgs& a, int smem_bytes, cudaStream_t
 }
 
 // ---- the layer for prompts: expert products grouped by expert (ggml_grouped.cu) ---------------------------------------
-// logits[t][row] = W[row] . x[t] (+ bias): 64 tokens x 64 router rows per block, 4 x 4 per thread, float32 throughout. Row E is the
-// shared expert's gate, which goes to `extra_out`.
+// logits[t][row] = W[row] . x[t] (+ bias), float32 throughout. Row E is the shared expert's gate, which goes to `extra_out`. A block
+// takes 32 tokens x 32 router rows, its eight warps every eighth 16 columns of k each (so that few tokens, few blocks, still read
+// with many loads in flight), 4 x 8 sums per lane, joined in the order of the warps.
 struct PrefillRouterArgs {
   const void* w; const void* extra; const float* bias; const float* x;
   float* logits; float* extra_out;
   int hidden, experts, tokens, first;                  // first: first row (experts: only the gate)
+  int vec;                                             // every four elements start on a boundary of four
 };
 template <typename WT>
 __global__ void __launch_bounds__(256) prefill_router_kernel(const PrefillRouterArgs a) {
-  __shared__ float xt[32][68], wt[32][68];             // [k][token], [k][row]
+  constexpr int kPitch = 36, kTile = 16 * kPitch;      // [k][token or row]: four at a time, two lanes per bank on the way in
+  __shared__ __align__(16) float tiles[8][2][kTile];
   pdl_wait();
   pdl_launch();
-  const int t0 = blockIdx.x * 64, r0 = a.first + blockIdx.y * 64, rows = a.experts + (a.extra ? 1 : 0);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < a.hidden; k0 += 32) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < 64 * 32; e += 256) {
-      const int i = e >> 5, k = e & 31;
-      xt[k][i] = t0 + i < a.tokens ? __ldcg(a.x + size_t(t0 + i) * a.hidden + k0 + k) : 0.f;
-      const int r = r0 + i;
-      wt[k][i] = r < a.experts ? to_f32(static_cast<const WT*>(a.w)[size_t(r) * a.hidden + k0 + k])
-                 : r < rows    ? to_f32(static_cast<const WT*>(a.extra)[k0 + k]) : 0.f;
-    }
-    __syncthreads();
+  constexpr int kWTy = sizeof(WT) == 4 ? DARASK_GGML_F32 : std::is_same<WT, __half>::value ? DARASK_GGML_F16 : DARASK_GGML_BF16;
+  const int t0 = blockIdx.x * 32, r0 = a.first + blockIdx.y * 32, rows = a.experts + (a.extra ? 1 : 0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = (lane & 3) * 4;
+  float xr[4][4], wr[4][4], acc[4][8] = {};
+  auto get4 = [&](const void* p, int ty, size_t at, float (&v)[4]) {
+    if (a.vec) return load_elem4(p, ty, at, v);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const float4 p = *reinterpret_cast<const float4*>(&xt[k][ty * 4]), q = *reinterpret_cast<const float4*>(&wt[k][tx * 4]);
-      const float pv[4] = {p.x, p.y, p.z, p.w}, qv[4] = {q.x, q.y, q.z, q.w};
+    for (int j = 0; j < 4; ++j) v[j] = load_elem(p, ty, at + j);
+  };
+  auto fetch = [&](int k0) {                           // 16 columns of 32 tokens and 32 rows, four lanes per row
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int o = i * 8 + (lane >> 2), r = r0 + o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xr[i][j] = wr[i][j] = 0.f;
+      if (t0 + o < a.tokens) get4(a.x, DARASK_GGML_F32, size_t(t0 + o) * a.hidden + k0 + part, xr[i]);
+      if (r < a.experts) get4(a.w, kWTy, size_t(r) * a.hidden + k0 + part, wr[i]);
+      else if (r < rows) get4(a.extra, kWTy, size_t(k0 + part), wr[i]);
+    }
+  };
+  float *xt = tiles[warp][0], *wt = tiles[warp][1];
+  const int tx = (lane & 3) * 8, ty = (lane >> 2) * 4;
+  fetch(warp * 16);
+  for (int k0 = warp * 16; k0 < a.hidden; k0 += 128) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        xt[(part + j) * kPitch + i * 8 + (lane >> 2)] = xr[i][j];
+        wt[(part + j) * kPitch + i * 8 + (lane >> 2)] = wr[i][j];
+      }
+    __syncwarp();
+    if (k0 + 128 < a.hidden) fetch(k0 + 128);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float4 p = *reinterpret_cast<const float4*>(xt + k * kPitch + ty);
+      const float4 q = *reinterpret_cast<const float4*>(wt + k * kPitch + tx), u = *reinterpret_cast<const float4*>(wt + k * kPitch + tx + 4);
+      const float pv[4] = {p.x, p.y, p.z, p.w}, qv[8] = {q.x, q.y, q.z, q.w, u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(pv[i], qv[j], acc[i][j]);
+        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(pv[i], qv[j], acc[i][j]);
     }
   }
+  __syncthreads();
+  float* mine = &tiles[0][0][0] + warp * 1024;         // [token][row] of this warp
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + ty * 4 + i, r = r0 + tx * 4 + j;
-      if (t >= a.tokens || r >= rows) continue;
-      if (r == a.experts) a.extra_out[t] = acc[i][j];
-      else a.logits[size_t(t) * a.experts + r] = acc[i][j] + (a.bias ? a.bias[r] : 0.f);
-    }
+    for (int j = 0; j < 8; ++j) mine[(ty + i) * 32 + tx + j] = acc[i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 1024; e += 256) {
+    const int t = t0 + (e >> 5), r = r0 + (e & 31);
+    if (t >= a.tokens || r >= rows) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += (&tiles[0][0][0])[q * 1024 + e];
+    if (r == a.experts) a.extra_out[t] = v;
+    else a.logits[size_t(t) * a.experts + r] = v + (a.bias ? a.bias[r] : 0.f);
+  }
 }
 // position[assignment] = dispatch row, and the one range of the shared expert
 __global__ void __launch_bounds__(256) prefill_position_kernel(const unsigned* assignments, const int* counters, unsigned* position, unsigned* shared_range,
@@ -263,19 +297,43 @@ __global__ void __launch_bounds__(256) prefill_position_kernel(const unsigned* a
   if (i < unsigned(__ldcg(counters + 1))) position[__ldcg(assignments + i)] = i;
 }
 // x[t][i] += sum_s p[t][s] y[position[t][s]][i] + sigmoid(sg[t]) ysh[t][i], in the order of kogarashi_combine_kernel; a dropped route has no row
-__global__ void __launch_bounds__(256) prefill_combine_kernel(float* x, const float* y, const float* ysh, const float* prob, const unsigned* position,
+// A thread has COLS columns, so that a route's row is read with few and independent loads.
+template <int COLS>
+__global__ void __launch_bounds__(128) prefill_combine_kernel(float* x, const float* y, const float* ysh, const float* prob, const unsigned* position,
                                                               const float* sg, int hidden, int topk, unsigned rows) {
+  __shared__ unsigned at[32];
+  __shared__ float p[32];
   pdl_wait();
   pdl_launch();
-  const int i = blockIdx.y * 256 + threadIdx.x, t = blockIdx.x;
-  if (i >= hidden) return;
-  float v = 0.f;
-  for (int s = 0; s < topk; ++s) {
-    const unsigned p = __ldcg(position + size_t(t) * topk + s);
-    if (p < rows) v = fmaf(__ldcg(prob + size_t(t) * topk + s), __ldcg(y + size_t(p) * hidden + i), v);
+  const int i = (blockIdx.y * 128 + threadIdx.x) * COLS, t = blockIdx.x;
+  if (threadIdx.x < topk) {
+    at[threadIdx.x] = __ldcg(position + size_t(t) * topk + threadIdx.x);
+    p[threadIdx.x] = __ldcg(prob + size_t(t) * topk + threadIdx.x);
   }
-  if (ysh) v += sigmoid_precise(__ldcg(sg + t)) * __ldcg(ysh + size_t(t) * hidden + i);
-  x[size_t(t) * hidden + i] += v;
+  __syncthreads();
+  if (i >= hidden) return;
+  using V = typename std::conditional<COLS == 4, float4, float>::type;
+  union Row { V v; float f[COLS]; };
+  Row sum = {}, own;
+  own.v = *reinterpret_cast<const V*>(x + size_t(t) * hidden + i);
+#pragma unroll 8
+  for (int s = 0; s < topk; ++s) {
+    if (at[s] >= rows) continue;
+    Row r;
+    r.v = __ldcg(reinterpret_cast<const V*>(y + size_t(at[s]) * hidden + i));
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) sum.f[c] = fmaf(p[s], r.f[c], sum.f[c]);
+  }
+  if (ysh) {
+    Row r;
+    r.v = __ldcg(reinterpret_cast<const V*>(ysh + size_t(t) * hidden + i));
+    const float g = sigmoid_precise(__ldcg(sg + t));
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) sum.f[c] += g * r.f[c];
+  }
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) own.f[c] += sum.f[c];
+  *reinterpret_cast<V*>(x + size_t(t) * hidden + i) = own.v;
 }
 
 // The words in front lie where `carve` has them, so that kogarashi_moe_status finds the status word.
@@ -454,8 +512,9 @@ extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cu
   // 1. router projection (or the shared gate alone), top-k, permutation
   const int first = logits_given ? E : 0, rows = E + (shared ? 1 : 0) - first;
   if (rows > 0) {
-    const PrefillRouterArgs r{d->router_w, shared ? d->sh_inp_w : nullptr, d->router_bias, d->n, d->logits, w.sg, H, E, T, first};
-    const dim3 grid((T + 63) / 64, (rows + 63) / 64);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(d->router_w) | (shared ? reinterpret_cast<uintptr_t>(d->sh_inp_w) : 0) | reinterpret_cast<uintptr_t>(d->n);
+    const PrefillRouterArgs r{d->router_w, shared ? d->sh_inp_w : nullptr, d->router_bias, d->n, d->logits, w.sg, H, E, T, first, at % 16 == 0};
+    const dim3 grid((T + 31) / 32, (rows + 31) / 32);
     if (d->router_ty == DARASK_GGML_F32) e = launch_pdl(prefill_router_kernel<float>, grid, dim3(256), 0, st, r);
     else if (d->router_ty == DARASK_GGML_BF16) e = launch_pdl(prefill_router_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, r);
     else e = launch_pdl(prefill_router_kernel<__half>, grid, dim3(256), 0, st, r);
@@ -484,8 +543,10 @@ extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cu
   if ((e = products(E, routes, w.ranges, w.assignments, d->gate_w, d->up_w, d->down_w, w.y))) return e;
   if (shared && (e = products(1, T, w.shared_range, nullptr, d->sh_gate_w, d->sh_up_w, d->sh_down_w, w.ysh))) return e;
   // 3. combine into the residual stream
-  return launch_pdl(prefill_combine_kernel, dim3(T, (H + 255) / 256), dim3(256), 0, st, d->x, (const float*)w.y, shared ? (const float*)w.ysh : (const float*)nullptr,
-                    (const float*)d->prob, (const unsigned*)w.position, (const float*)w.sg, H, K, unsigned(routes));
+  const bool four = reinterpret_cast<uintptr_t>(d->x) % 16 == 0;
+  return launch_pdl(four ? prefill_combine_kernel<4> : prefill_combine_kernel<1>, dim3(T, (H + (four ? 511 : 127)) / (four ? 512 : 128)), dim3(128), 0, st, d->x,
+                    (const float*)w.y, shared ? (const float*)w.ysh : (const float*)nullptr, (const float*)d->prob, (const unsigned*)w.position,
+                    (const float*)w.sg, H, K, unsigned(routes));
 }
 
 // ---- stand-alone pieces (also used by the parity tests) ------------------------------------------

@@ -61,22 +61,6 @@ template <int COLS>
 DEVI void tmem_free(uint32_t base) {            // the warp that allocated
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(uint32_t(COLS)) : "memory");
 }
-// Two float32 sums at a time: {a.lo * b.lo + c.lo, a.hi * b.hi + c.hi}, each rounded once
-DEVI unsigned long long pack2(float lo, float hi) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-DEVI float2 unpack2(unsigned long long v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-DEVI unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // 32 columns of this warp's 32 TMEM lanes -> registers, complete on return
 DEVI void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
