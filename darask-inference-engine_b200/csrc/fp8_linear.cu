@@ -138,13 +138,13 @@ extern "C" size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_t
 
 static bool linear_ok(const DaraskFp8Linear* d) {
   if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->m > (1 << 24) || d->n > (1 << 24) || d->k > (1 << 20)) return false;
-  if (!d->w || !d->w_scales || reinterpret_cast<uintptr_t>(d->w) % 16 || d->ldw % 16 || d->ldw < d->k) return false;
+  if (!d->w || !d->w_scales || reinterpret_cast<uintptr_t>(d->w_scales) % 4 || reinterpret_cast<uintptr_t>(d->w) % 16 || d->ldw % 16 || d->ldw < d->k) return false;
   const long long kb = (d->k + 127) / 128;
   if (d->ld_ws < kb || !row_type_bytes(d->out_ty) || d->ldo < d->n || (d->add && d->out_ty != DARASK_GGML_F32)) return false;
   if (d->m == 0) return true;
   if (!d->x || !d->out || reinterpret_cast<uintptr_t>(d->out) % row_type_bytes(d->out_ty)) return false;
   if (d->x_ty == DARASK_E4M3)
-    return d->x_scales && d->ld_xs >= kb && !d->swiglu && reinterpret_cast<uintptr_t>(d->x) % 16 == 0 && d->ldx % 16 == 0 && d->ldx >= d->k;
+    return d->x_scales && reinterpret_cast<uintptr_t>(d->x_scales) % 4 == 0 && d->ld_xs >= kb && !d->swiglu && reinterpret_cast<uintptr_t>(d->x) % 16 == 0 && d->ldx % 16 == 0 && d->ldx >= d->k;
   const size_t eb = row_type_bytes(d->x_ty);
   if (!eb || d->x_scales || reinterpret_cast<uintptr_t>(d->x) % eb || d->ldx < (d->swiglu ? 2ll : 1ll) * d->k) return false;
   const size_t need = darask_fp8_linear_workspace_bytes(d->m, d->n, d->k, d->x_ty);

@@ -86,17 +86,22 @@ extern "C" size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int
   return carve(nullptr, rows, k, row_parts(x_ty, swiglu)).bytes;
 }
 
+// Few rows per group, narrow tiles: the weights' bytes pace the product then.
+static bool grouped_narrow(const DaraskGgmlGrouped* d) { return d->rows <= 32ll * d->groups; }
+// one more than the tiles of ranges that do not overlap
+static long long grouped_tile_cap(const DaraskGgmlGrouped* d) {
+  return (d->rows / (grouped_narrow(d) ? 32 : 128) + d->groups) * ((d->n + 127) / 128) * (d->w_up ? 2 : 1) + 1;
+}
 static bool grouped_ok(const DaraskGgmlGrouped* d) {
   if (!d || d->groups < 1 || d->groups > 1024 || d->n < 1 || d->n > (1 << 20) || d->k < 256 || d->k > (1 << 16) || d->k % 256) return false;
   if (d->rows < 0 || d->rows > (1ll << 27) || d->x_rows < 0 || d->x_rows > (1ll << 31) - 1) return false;
   if (!d->w || reinterpret_cast<uintptr_t>(d->w) % 16 || reinterpret_cast<uintptr_t>(d->w_up) % 16 || !ggml_row_bytes(d->w_ty, d->k)) return false;
   const size_t eb = row_type_bytes(d->x_ty), ob = row_type_bytes(d->out_ty);
   if (!eb || !ob || d->ldx < (d->swiglu ? 2ll : 1ll) * d->k || d->ldo < (d->w_up ? 2ll : 1ll) * d->n) return false;
-  if (d->assignments && d->topk < 1) return false;
-  // the tiles of one matrix or two are counted in 32 bits
-  if ((d->rows / (d->rows <= 32ll * d->groups ? 32 : 128) + d->groups) * ((d->n + 127) / 128) * (d->w_up ? 2 : 1) >= kGgMaxTiles) return false;
+  if (d->assignments && (d->topk < 1 || reinterpret_cast<uintptr_t>(d->assignments) % 4)) return false;
+  if (grouped_tile_cap(d) >= 1ll << 30) return false;      // tiles are counted in 32 bits, two counts added
   if (d->rows == 0) return true;
-  if (!d->ranges || !d->out || reinterpret_cast<uintptr_t>(d->out) % ob) return false;
+  if (!d->ranges || reinterpret_cast<uintptr_t>(d->ranges) % 4 || !d->out || reinterpret_cast<uintptr_t>(d->out) % ob) return false;
   if (d->x_rows > 0 && (!d->x || reinterpret_cast<uintptr_t>(d->x) % eb)) return false;
   return d->workspace && reinterpret_cast<uintptr_t>(d->workspace) % 256 == 0 &&
          d->workspace_bytes >= darask_ggml_grouped_workspace_bytes(d->rows, d->k, d->x_ty, d->swiglu);
@@ -143,12 +148,11 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   GgArgs a = {};
   a.ranges = d->ranges; a.groups = d->groups; a.n = d->n; a.nblk = nblk; a.mats = d->w_up ? 2 : 1; a.row_bytes = row_bytes; a.rows = d->rows;
   a.w[0] = static_cast<const uint8_t*>(d->w); a.w[1] = static_cast<const uint8_t*>(d->w_up);
-  a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo;
+  a.xscale = ws.scale; a.out = d->out; a.ldo = d->ldo; a.tile_cap = int(grouped_tile_cap(d));
   const size_t ob = row_type_bytes(d->out_ty);
   a.aligned = reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->ldo * ob % 16 == 0 && (!d->w_up || d->n * ob % 16 == 0);
   a.status = status;
-  // narrow tiles while the groups have few rows on average: the weights' bytes pace the product then
-  const bool narrow = d->rows <= 32ll * d->groups;
+  const bool narrow = grouped_narrow(d);
   if (q6) return narrow ? launch_by_type<true, 32>(d->out_ty, nx, m, a, st) : launch_by_type<true, 128>(d->out_ty, nx, m, a, st);
   return narrow ? launch_by_type<false, 32>(d->out_ty, nx, m, a, st) : launch_by_type<false, 128>(d->out_ty, nx, m, a, st);
 }

@@ -23,7 +23,6 @@
 namespace dmoe {
 
 constexpr int kGgMaxGroups = 1024;
-constexpr int kGgMaxTiles = 1 << 30;                     // a call whose ranges do not overlap has fewer; two of them still add up in 32 bits
 
 struct GgArgs {
   const unsigned* ranges;                                // [groups][2]
@@ -33,6 +32,7 @@ struct GgArgs {
   const float* xscale;                                   // [rows] powers of two; negative: row(i) does not exist
   void* out;
   long long ldo;
+  int tile_cap;                                          // more tiles than ranges that do not overlap can have, below 2^30
   int aligned;                                           // 16-byte pieces of the output's rows start on 16-byte boundaries
   unsigned* status;
 };
@@ -310,19 +310,19 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   }
   __syncthreads();
   if (warp == 0) {                       // inclusive scan, consecutive groups per lane
-    // ranges that overlap can count more tiles than rows hold: the sum stops at kGgMaxTiles, groups behind it get none
+    // ranges that overlap can count more tiles than the rows hold: the sum stops at tile_cap, groups behind it get none
     const int per = (a.groups + 31) / 32;
     int sum = 0;
-    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) sum = min(sum + ends[g], kGgMaxTiles); }
+    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) sum = min(sum + ends[g], a.tile_cap); }
     int run = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run = min(run + t, kGgMaxTiles); }
+    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run = min(run + t, a.tile_cap); }
     int off = __shfl_up_sync(0xffffffffu, run, 1);
     if (lane == 0) off = 0;
-    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) { off = min(off + ends[g], kGgMaxTiles); ends[g] = off; } }
+    for (int i = 0; i < per; ++i) { const int g = lane * per + i; if (g < a.groups) { off = min(off + ends[g], a.tile_cap); ends[g] = off; } }
     if (lane == 31) {
       ends[a.groups] = run;
-      if (run == kGgMaxTiles && blockIdx.x == 0) atomicOr(a.status, kStatusBadRoute);
+      if (run == a.tile_cap && blockIdx.x == 0) atomicOr(a.status, kStatusBadRoute);
     }
   }
   tmem_fence_before();

@@ -501,6 +501,12 @@ extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cu
   const int H = d->hidden, F = d->inter, E = d->experts, K = d->topk, T = d->tokens;
   if ((long long)T * K > (1ll << 27) || d->workspace_bytes < kogarashi_moe_prefill_workspace_bytes(H, F, E, K, T)) return cudaErrorInvalidValue;
   const bool shared = d->sh_gate_w != nullptr;
+  // what the products would refuse is refused before anything is enqueued
+  uintptr_t at = reinterpret_cast<uintptr_t>(d->gate_w) | reinterpret_cast<uintptr_t>(d->up_w) | reinterpret_cast<uintptr_t>(d->down_w);
+  if (shared) at |= reinterpret_cast<uintptr_t>(d->sh_gate_w) | reinterpret_cast<uintptr_t>(d->sh_up_w) | reinterpret_cast<uintptr_t>(d->sh_down_w);
+  const uintptr_t words = reinterpret_cast<uintptr_t>(d->n) | reinterpret_cast<uintptr_t>(d->x) | reinterpret_cast<uintptr_t>(d->logits) |
+                          reinterpret_cast<uintptr_t>(d->ids) | reinterpret_cast<uintptr_t>(d->prob);
+  if (at % 16 || words % 4 || H > (1 << 16) || F > (1 << 16)) return cudaErrorInvalidValue;
   const PrefillWs w = carve_prefill(d->workspace, H, F, E, K, T);
   const long long routes = (long long)T * K;
   cudaError_t e = cudaMemsetAsync(d->workspace, 0, 1280, st);           // counters, status
@@ -512,8 +518,8 @@ extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cu
   // 1. router projection (or the shared gate alone), top-k, permutation
   const int first = logits_given ? E : 0, rows = E + (shared ? 1 : 0) - first;
   if (rows > 0) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(d->router_w) | (shared ? reinterpret_cast<uintptr_t>(d->sh_inp_w) : 0) | reinterpret_cast<uintptr_t>(d->n);
-    const PrefillRouterArgs r{d->router_w, shared ? d->sh_inp_w : nullptr, d->router_bias, d->n, d->logits, w.sg, H, E, T, first, at % 16 == 0};
+    const uintptr_t rat = reinterpret_cast<uintptr_t>(d->router_w) | (shared ? reinterpret_cast<uintptr_t>(d->sh_inp_w) : 0) | reinterpret_cast<uintptr_t>(d->n);
+    const PrefillRouterArgs r{d->router_w, shared ? d->sh_inp_w : nullptr, d->router_bias, d->n, d->logits, w.sg, H, E, T, first, rat % 16 == 0};
     const dim3 grid((T + 31) / 32, (rows + 31) / 32);
     if (d->router_ty == DARASK_GGML_F32) e = launch_pdl(prefill_router_kernel<float>, grid, dim3(256), 0, st, r);
     else if (d->router_ty == DARASK_GGML_BF16) e = launch_pdl(prefill_router_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, r);

@@ -44,7 +44,8 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
     (``quantize.fp8_block``).  x float32, float16 or bfloat16 is quantized by the call with one scale per row and 128 columns; with
     `swiglu` its rows hold gate | up ([m, 2k]) and silu(gate) * up is quantized.  x uint8 holds e4m3 codes, with x_scales float32
     [m, >= ceil(k/128)] (``quantize.fp8_act``).  Sums are float32; `out_dtype` (float32, float16, bfloat16) defaults to x's type, or
-    bfloat16 for codes.  With `add` the product is added to what a float32 `out` holds.  Rows may be strided; rows of w and of codes start on 16-byte boundaries.  Any m, including 0; k as w has it.
+    bfloat16 for codes.  With `add` the product is added to what a float32 `out` holds.  `out` must not overlap an input.  Rows
+    may be strided; rows of w and of codes start on 16-byte boundaries.  Any m, including 0; k as w has it.
     Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
     if w.dim() != 2 or w.dtype is not torch.uint8 or w_scales.dim() != 2 or w_scales.dtype is not torch.float32:
         raise ValueError("w must be uint8 [n, k] and w_scales float32 [n blocks, k blocks]")

@@ -34,8 +34,8 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
     with `up`, a second one of the same shape, out holds both products side by side ([rows, 2n]).  ranges int32 [groups, 2] =
     {rows, offset}.  x float32, float16 or bfloat16 [*, k]; dispatch row i reads x row assignments[i] // topk (int32, on the
     device), or row i without assignments.  With `swiglu` the rows of x hold gate | up ([*, 2k]) and silu(gate) * up is multiplied.
-    Sums are float32; `out_dtype` defaults to x's type.  Rows outside every range are left as they were (uninitialised when
-    `out` is not given).  Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
+    Sums are float32; `out_dtype` defaults to x's type.  Ranges do not overlap, `out` overlaps no input.  Rows outside every range
+    are left as they were (uninitialised when `out` is not given).  Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
     k, n, groups = weight.k, weight.rows, weight.ne[2] if len(weight.ne) > 2 else 1
     if weight.ty not in (GGML_Q4_K, GGML_Q6_K) or k < 256 or k % 256 or n < 1 or not 1 <= groups <= 1024:
         raise ValueError("weight must be Q4_K or Q6_K [k % 256 == 0, n, groups <= 1024]")
@@ -184,6 +184,8 @@ class KogarashiMoeLayer:
             raise ValueError("x and n must be contiguous float32")
         if logits is not None and (logits.dtype != torch.float32 or tuple(logits.shape) != (t, self.experts) or not logits.is_contiguous()):
             raise ValueError("logits must be contiguous float32 [T, E]")
+        if any(v is not None and v.get_device() != self.workspace.get_device() for v in (x, n, logits, attn_out, norm_w)):
+            raise ValueError("tensors must be on the layer's device")
         lib = _lib.lib()
         d = self._descriptor(x, n, attn_out, norm_w, eps)
         given = logits is not None

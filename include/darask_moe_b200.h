@@ -130,8 +130,8 @@ int kogarashi_moe_workspace_init(void* workspace, size_t bytes, darask_stream_t 
 int kogarashi_moe_layer(const KogarashiMoe* desc /* host */, darask_stream_t stream);
 /* The same layer for prompts and large batches: the same descriptor and results (routing from the same logits, sums in another
  * order), the expert products through darask_ggml_grouped_gemm instead of passes of eight tokens.  `workspace` holds
- * kogarashi_moe_prefill_workspace_bytes(...) bytes, 256-byte aligned, needs no initialisation and belongs to the call;
- * kogarashi_moe_status reads its status word.  logits_given != 0: desc->logits holds the logits (router_bias included) and the
+ * kogarashi_moe_prefill_workspace_bytes(...) bytes, 256-byte aligned, needs no initialisation and belongs to the call (never the
+ * one that kogarashi_moe_layer runs in, which keeps words between calls); kogarashi_moe_status reads its status word.  logits_given != 0: desc->logits holds the logits (router_bias included) and the
  * router projection is left out; the shared expert's gate is projected all the same. */
 size_t kogarashi_moe_prefill_workspace_bytes(int hidden, int inter, int experts, int topk, int tokens);
 int kogarashi_moe_prefill(const KogarashiMoe* desc /* host */, int logits_given, darask_stream_t stream);
@@ -425,10 +425,12 @@ int darask_fp8_linear_status(unsigned* host_status /* host */, darask_stream_t s
  *            with w_up, out rows hold x . w | x . w_up (2n columns).  k % 256 == 0, k <= 65536, groups <= 1024.
  *   x        float32 / f16 / bf16 rows, x_rows of them; row(i) = assignments[i] / topk, or i without assignments.
  *   swiglu   rows of x hold gate | up (2k columns) and silu(gate) * up is multiplied (the down product).
- *   out      [rows][ldo]; rows outside every range are left as they were.
+ *   out      [rows][ldo], overlapping no input; rows outside every range are left as they were, ranges do not overlap (a row in
+ *            two of them holds either product).
  * Sums in float32; weights enter as exact integers (Q4_K, Q6_K: block scale times an integer), float32 rows as two f16
  * parts (22 bits), f16 and bf16 rows as they are, with one power of two per row taken out first.  An infinity or a NaN in a row
- * makes the row's outputs NaN.  A range that leaves [0, rows) is cut and a row(i) >= x_rows reads as zeros; both set
+ * makes the row's outputs NaN.  A range that leaves [0, rows) is cut, a row(i) >= x_rows reads as zeros, and of overlapping ranges
+ * that hold many times `rows` the last ones may be left out; each sets
  * DARASK_STATUS_BAD_ROUTE in the device's status word (darask_ggml_grouped_status, as darask_fp8_linear_status).
  * workspace: darask_ggml_grouped_workspace_bytes(rows, k, x_ty, swiglu) bytes, 256-byte aligned, as for darask_fp8_linear. */
 typedef struct {

@@ -212,3 +212,17 @@ def test_no_rows():
     out = torch.full((5, 128), 2.0, device="cuda")
     D.kogarashi.grouped_gemm(x, ranges_of([0] * 4), w, out=out)            # rows, but none in a range
     assert bool((out == 2).all())
+
+
+def test_ranges_that_all_hold_every_row():
+    """Far more tiles than the rows have: some are left out and reported, the call ends, rows past the ranges stay."""
+    import darask_inference_engine_b200 as D
+    g, rows, n, k = 64, 600, 130, 256
+    w, _, _ = weight(11, Q4, g, n, k)
+    x = torch.randn(rows, k, device="cuda")
+    D.kogarashi.grouped_status()
+    r = torch.tensor([[rows - 1, 0]] * g, dtype=torch.int32, device="cuda")
+    out = torch.full((rows, n), 7.0, device="cuda")
+    D.kogarashi.grouped_gemm(x, r, w, out=out)
+    assert D.kogarashi.grouped_status() == 2
+    assert bool((out[-1] == 7.0).all())

@@ -109,3 +109,45 @@ def test_python_refusals_of_the_grouped_product():
                        (dict(assignments=torch.zeros(5, dtype=torch.int32), topk=0), "assignments"), (dict(out=torch.zeros(5, 63)), "out must"), (dict(), "CUDA device")):
         with pytest.raises(ValueError, match=match):
             D.kogarashi.grouped_gemm(**{**dict(x=x, ranges=r, weight=good), **bad})
+
+
+@no_gpu
+@pytest.mark.parametrize("entry,make,bad", [("darask_fp8_linear", linear, [dict(w_scales=FAKE + 2), dict(x_ty=100, ldx=304, x_scales=FAKE + 1, ld_xs=3)]),
+                                            ("darask_ggml_grouped_gemm", grouped, [dict(ranges=FAKE + 2), dict(assignments=FAKE + 1)])], ids=["linear", "grouped"])
+def test_scales_and_index_lists_off_their_words_are_refused(entry, make, bad):
+    import darask_inference_engine_b200 as D
+    for change in bad:
+        assert getattr(D._lib.lib(), entry)(ctypes.byref(make(**change)), None) == INVALID, change
+
+
+@no_gpu
+def test_more_tiles_than_the_kernel_counts_are_refused():
+    import darask_inference_engine_b200 as D
+    d = grouped(groups=1024, n=1 << 20, rows=1 << 25, x_rows=1 << 25, w_up=FAKE, ldo=2 << 20, workspace_bytes=1 << 50)
+    assert D._lib.lib().darask_ggml_grouped_gemm(ctypes.byref(d), None) == INVALID
+
+
+def prefill(**kw):
+    import darask_inference_engine_b200 as D
+    d = D._lib.KogarashiMoe()
+    d.hidden, d.inter, d.experts, d.topk, d.tokens = 512, 256, 8, 2, 5
+    for name in ("router_w", "gate_w", "up_w", "down_w", "n", "x", "logits", "ids", "prob", "workspace"):
+        setattr(d, name, FAKE)
+    d.router_ty, d.gate_ty, d.up_ty, d.down_ty = 0, 12, 12, 14
+    for k, v in kw.items():
+        setattr(d, k, v)
+    d.workspace_bytes = kw.get("workspace_bytes", D._lib.lib().kogarashi_moe_prefill_workspace_bytes(d.hidden, d.inter, d.experts, d.topk, d.tokens))
+    return d
+
+
+@no_gpu
+def test_the_prompt_layer_refuses_before_anything_is_enqueued():
+    import darask_inference_engine_b200 as D
+    call = D._lib.lib().kogarashi_moe_prefill
+    assert call(None, 0, None) == INVALID
+    assert call(ctypes.byref(prefill()), 0, None) != INVALID              # passes, and ends in the missing driver
+    shared = dict(sh_gate_w=FAKE, sh_up_w=FAKE, sh_down_w=FAKE, sh_inp_w=FAKE)
+    for change in (dict(gate_w=FAKE + 8), dict(up_w=FAKE + 4), dict(down_w=FAKE + 8), dict(shared, sh_down_w=FAKE + 8), dict(n=FAKE + 2), dict(logits=FAKE + 1),
+                   dict(ids=FAKE + 2), dict(hidden=65536 + 256), dict(inter=65536 + 256), dict(workspace=FAKE + 16), dict(workspace_bytes=64), dict(tokens=0),
+                   dict(tokens=1 << 27), dict(topk=9), dict(gate_ty=0, up_ty=0), dict(down_ty=30), dict(shared, sh_up_w=0)):
+        assert call(ctypes.byref(prefill(**change)), 0, None) == INVALID, change

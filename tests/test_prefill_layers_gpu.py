@@ -171,3 +171,25 @@ def test_the_operators_together_in_a_graph():
         block()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(x, want)
+
+
+def test_prefill_refuses_tensors_that_are_elsewhere():
+    layer, acts = W.kogarashi_layer(9, hidden=256, inter=256, experts=4, topk=2, tokens=3, shared=False, pool=4)
+    m, _ = run_kogarashi(layer, acts)
+    x = torch.zeros(3, 256, device="cuda")
+    for bad in (dict(x=x.cpu(), n=x), dict(x=x, n=x.cpu()), dict(x=x, n=x.clone(), logits=torch.zeros(3, 4)),
+                dict(x=x, n=x.clone(), norm_w=torch.ones(256)), dict(x=x, n=x.clone(), norm_w=x[0].clone(), attn_out=torch.zeros(3, 256))):
+        with pytest.raises(ValueError):
+            m.prefill(**bad)
+
+
+@pytest.mark.parametrize("tokens", [1, 33, 70])
+def test_prefill_of_rows_on_any_word(tokens):
+    """x, n and the router four bytes off: the same bits as on 16-byte boundaries."""
+    layer, acts = W.kogarashi_layer(21, hidden=512, inter=256, experts=40, topk=3, tokens=tokens, shared=True, pool=8)
+    m, _ = run_kogarashi(layer, acts)
+    off = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+    x, n = torch.from_numpy(acts["x"].copy()).cuda(), torch.from_numpy(acts["n"].copy()).cuda()
+    y, ids, prob = m.prefill(x.clone(), n)
+    y2, ids2, prob2 = m.prefill(off(x), off(n))
+    assert torch.equal(y, y2) and torch.equal(ids, ids2) and torch.equal(prob, prob2)
