@@ -57,6 +57,17 @@ struct GgShape {
   static constexpr int kSums = Q6 ? 0 : NT * 32;         // NT rows x 16 f16: the sums of eight groups of 32 columns, high and low parts
   static constexpr int kXStage = NX * kPart + kSums;     // Q4_K: the sums travel with the second step of a block
   static constexpr int kXStages = kWide && NX == 2 ? 2 : 4;
+  // Partial products per block. The tensor core cuts the sum of every 16 columns to the accumulator's 24 bits, toward zero, so that the
+  // error grows with the number of sums and does not average out. Integers times bf16 or f16 hardly have bits to lose (3e-7 of the result
+  // over 256 columns); two parts do: multiplied into one accumulator in turn they lost 1.5e-6 (Q4_K; Q6_K 8e-7). So there the small
+  // products come first and every step has an accumulator of its own (PREC).
+  // Partial products per block of 256 columns. The tensor core cuts the sum of every 16 columns to the accumulator's 24 bits, toward
+  // zero, so that the error grows with the number of sums and does not average out; products of two parts have bits to lose. In turn in
+  // one accumulator they lost 1.5e-6 of the result (Q4_K, whose codes have no sign and largely cancel against the mins) and 8e-7 (Q6_K).
+  // The small products go first (Q6_K: 6e-7; an accumulator per step would bring 2e-7, but 513 us where this takes 449: 32768 rows, 128
+  // groups of 2048 x 768), and Q4_K has an accumulator of its own for every step as well (4e-7 for 4 % of the time).
+  static constexpr int kSteps = Q6 ? 1 : NX;
+  static_assert(kSteps == 2 || kXStages == 4 || Q6, "the promotion takes the stage of a block's second step from its buffer");
   static constexpr int kMins = Q6 ? 0 : kSets / 2;       // 128 rows x 32 bytes each
   static constexpr int kOffMin = kXStages * kXStage;
   static constexpr int kOffRaw = kOffMin + kMins * 4096;
@@ -436,14 +447,15 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         const uint32_t idesc = __shfl_sync(0xffffffffu, (1u << 4) | (uint32_t((t.rows + 15) / 16 * 2) << 17) | (uint32_t(128 >> 4) << 24), 0);
 #pragma unroll 1
         for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
-          const uint32_t buf = wi & 1, d = tmem + buf * NT;
+          const uint32_t buf = wi & 1;
           // stage of the first step and its parity: two or four stages
           const uint32_t x0 = S::kXStages == 4 ? buf * 2 : 0u, ph = S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1;
           // TMEM slots of the two steps
           const uint32_t a0 = slot, a1 = slot + 1 == S::kSets ? 0u : slot + 1;
           slot = a1 + 1 == S::kSets ? 0u : a1 + 1;
           // the buffers are free: the block before the last has been promoted
-          if (wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+          if (S::kSteps == 1 && wi >= 2) ok = warp_wait(tempty + buf, ((wi >> 1) & 1) ^ 1, a.status);
+          if (S::kSteps == 2 && wi >= 1) ok = warp_wait(tempty, (wi & 1) ^ 1, a.status);
           ok = warp_wait(full + x0, ph, a.status) && ok;
           if (!ok) break;
           tmem_fence_after();
@@ -452,19 +464,26 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             if (step == 1) {
               // one buffer of mins: the promotion of the last block has read it
               if (S::kMinBufs == 1 && wi >= 1) ok = warp_wait(&mfree, (wi - 1) & 1, a.status);
+              if (S::kSteps == 2 && wi >= 1) ok = warp_wait(tempty + 1, (wi & 1) ^ 1, a.status) && ok;
               ok = warp_wait(full + x0 + 1, ph, a.status) && ok;
               if (!ok) break;
               tmem_fence_after();
             }
             const uint64_t dx = dx0 + (x0 + step) * uint32_t(S::kXStage >> 4);
             const uint32_t at = tmem_a + (step ? a1 : a0) * 64, a2 = tmem_a2 + (step ? a1 : a0) * 64;
+            const uint32_t d = tmem + (S::kSteps == 2 ? uint32_t(step) : buf) * NT;
+            const uint32_t first = S::kSteps == 2 || step == 0 ? 0u : 1u;
+            auto box = [&](int q) -> uint64_t { return (q >> 2) * (S::kBox >> 4) + 2 * (q & 3); };      // 16 columns of k
+            if (NX == 2) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {                    // 16 columns of k
-              const uint64_t box = (q >> 2) * (S::kBox >> 4) + 2 * (q & 3);
-              umma_f16_ts(d, at + q * 8, dx + box, idesc, step | q ? 1u : 0u, go);
-              if (NX == 2) umma_f16_ts(d, at + q * 8, dx + (S::kPart >> 4) + box, idesc, 1u, go);
-              if (NA == 2) umma_f16_ts(d, a2 + q * 8, dx + box, idesc, 1u, go);
+              for (int q = 0; q < 8; ++q) umma_f16_ts(d, at + q * 8, dx + (S::kPart >> 4) + box(q), idesc, q ? 1u : first, go);
             }
+            if (NA == 2) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) umma_f16_ts(d, a2 + q * 8, dx + box(q), idesc, NX == 2 || q ? 1u : first, go);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) umma_f16_ts(d, at + q * 8, dx + box(q), idesc, NX == 2 || NA == 2 || q ? 1u : first, go);
             if (!Q6 && step == 1)                            // sums times mins
               umma_f16_ss(tmem_min + (S::kMinBufs == 2 ? buf * NT : 0u), dmin + (S::kMins == 2 ? buf * (4096u >> 4) : 0u), dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);
             umma_commit_if(empty + x0 + step, go);
@@ -596,7 +615,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     const int quarter = warp & 3, row = quarter * 32 + lane, c0 = ((warp - kFirst) >> 2) * kHalf;
     const uint32_t tl = (uint32_t(quarter * 32) << 16) + c0;
     float* scale = xsc[warp - kFirst];
-    uint32_t wi = 0;
+    uint32_t wi = 0, pi = 0;             // blocks of 256 columns and partial products so far
     bool ok = true;
     GgTile t;
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
@@ -616,41 +635,46 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int c = 0; c < kHalf; ++c) acc[c] = 0.f;
 #pragma unroll 1
       for (int b = 0; b < a.nblk; ++b, ++wi) {
-        const uint32_t buf = wi & 1;
-        uint64_t* bar = kOwnDone ? done + buf : empty + (S::kXStages == 4 ? buf * 2 + 1 : 1);
-        if (!warp_wait(bar, kOwnDone || S::kXStages == 4 ? (wi >> 1) & 1 : wi & 1, a.status)) { ok = false; break; }
-        tmem_fence_after();
-        const float2 d = dring[(wi & 3) * 128 + row];     // {d, -dmin}
-        auto add = [&](uint32_t from, float f) {          // acc += f * columns
+#pragma unroll 1
+        for (int u = 0; u < S::kSteps; ++u, ++pi) {
+          const uint32_t buf = pi & 1;
+          uint64_t* bar = kOwnDone ? done + buf : empty + (S::kSteps == 2 ? pi % S::kXStages : buf * 2 + 1);
+          const uint32_t ph = S::kSteps == 2 ? pi / S::kXStages : pi >> 1;
+          if (!warp_wait(bar, ph & 1, a.status)) { ok = false; break; }
+          tmem_fence_after();
+          const float2 d = dring[(wi & 3) * 128 + row];   // {d, -dmin}
+          auto add = [&](uint32_t from, float f) {        // acc += f * columns
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 32) {
-            if (c < rows) {
-              uint32_t v[32];
-              tmem_ld32(from + c, v);
+            for (int c = 0; c < kHalf; c += 32) {
+              if (c < rows) {
+                uint32_t v[32];
+                tmem_ld32(from + c, v);
 #pragma unroll
-              for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(f, __uint_as_float(v[q]), acc[c + q]);
+                for (int q = 0; q < 32; ++q) acc[c + q] = fmaf(f, __uint_as_float(v[q]), acc[c + q]);
+              }
+            }
+          };
+          if (!Q6 && u == S::kSteps - 1) {
+            add(tmem_min + tl + (S::kMinBufs == 2 ? (wi & 1) * NT : 0u), d.y);
+            if (S::kMinBufs == 1) {
+              tmem_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&mfree);
             }
           }
-        };
-        if (!Q6) {
-          add(tmem_min + tl + (S::kMinBufs == 2 ? buf * NT : 0u), d.y);
-          if (S::kMinBufs == 1) {
+          add(tmem + tl + buf * NT, d.x);
+          if (b + 1 < a.nblk || u + 1 < S::kSteps) {
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&mfree);
+            if (lane == 0) mbar_arrive(tempty + buf);
           }
         }
-        add(tmem + tl + buf * NT, d.x);
-        if (b + 1 < a.nblk) {
-          tmem_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(tempty + buf);
-        }
+        if (!ok) break;
       }
       if (!ok) break;
       // The sums go through the buffer just read, which is not handed back yet: a loop of few instructions stores them (128 stores
       // in a row would come through the instruction cache anew for every tile).
-      const uint32_t last = (wi - 1) & 1, stage = tmem + tl + last * NT;
+      const uint32_t last = (pi - 1) & 1, stage = tmem + tl + last * NT;
 #pragma unroll
       for (int c = 0; c < kHalf; c += 16) {
         if (c < rows) {
