@@ -11,11 +11,15 @@
 // rows cost a narrow tile (N a multiple of 16). The weight operand is written straight into TMEM (tcgen05.st), where
 // tcgen05.mma reads it: it costs shared memory neither space nor bandwidth.
 //   warps 0, 2    TMA: rows of x and their sums per 128 columns; packed weight rows (128 x 144 or 208 bytes) per 256 columns
-//   warp 1        tcgen05.mma kind::f16; per 256 columns one accumulator buffer of two
-//   warps 4-11    expanders: thread = one weight row; codes -> integers in f16 -> TMEM, 128 columns of k in each of two slots
-//   warps 12-15   promotion (thread = one weight row): acc += d * main - dmin * min, and the store at the end of a tile
-// TMEM: two main buffers of 128 columns, 128 columns for Q4_K's min products or Q6_K's second terms, 128 for the slots.
+//   warp 1        tcgen05.mma kind::f16 into one of two accumulators
+//   then          two to four sets of four expander warps: thread = one weight row; codes -> integers in f16 -> TMEM, a step of 128
+//                 columns of k in the set's slot
+//   the last 4-8  promotion (thread = one weight row): acc += d * main - dmin * min, and the store at the end of a tile
+// TMEM: two accumulators of NT columns, Q4_K's min products, the slots, Q6_K's second terms.
 // Persistent: tiles are dealt out in steps of the grid, the row tiles of a group's weight tile next to each other.
+// Bound: instructions and their latencies. A tile's 256 columns cost about 5000 warp instructions (2.1 per cycle), most of them the
+// expanders', whatever its rows: 32768 rows over 128 groups of 2 x 768 x 2048 Q4_K (bf16) take 430 us, 352 when the groups are even and
+// fill their tiles (585 TFLOP/s), 2048 rows over 256 groups of 2 x 1024 x 2048 232 us (2.6 TB/s).
 #pragma once
 #include "row_source.cuh"
 #include "tcgen05.cuh"
