@@ -347,8 +347,12 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   const int total = ends[a.groups];
   // a warp's tiles come in ascending order: the search for the group goes on from the last one
   auto locate = [&](int tile, GgTile& t) {
-    int g = t.group;
-    while (tile >= ends[g]) ++g;
+    int g = t.group;                     // (ends[groups] is above every tile, what lies behind it is not looked at)
+    for (;;) {                           // 32 groups at a time
+      const uint32_t found = __ballot_sync(0xffffffffu, g + lane <= a.groups && tile < ends[min(g + lane, a.groups)]);
+      if (found) { g += __ffs(found) - 1; break; }
+      g += 32;
+    }
     const int local = tile - (g ? ends[g - 1] : 0);
     t.group = g;
     const int r = group_rows(g, &t.first);
@@ -503,29 +507,23 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     const int set = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t((warp & 3) * 32) << 16) + set * 64;       // the set's TMEM slot
     const uint32_t magic = opaque(0x64006400u);      // 1024 in both halves
-    int ws = 0, turn = 0;                // raw stage, set whose step comes next
-    uint32_t wph = 0, wi = 0;
+    uint32_t wi0 = 0;                    // blocks of 256 columns before the tile
     bool ok = true;
     GgTile t;
-    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, wi0 += a.nblk) {
       locate(tile, t);
       const __half* dq = nullptr;        // Q6_K: the row's block scales
-      float d_next = 0.f;
       if (Q6) {
         const int r = t.n0 + row < a.n ? t.n0 + row : a.n - 1;
         dq = reinterpret_cast<const __half*>(a.w[t.mat] + (size_t(t.group) * a.n + r) * a.row_bytes + size_t(a.nblk) * 208);
-        d_next = __half2float(__ldcg(dq));
       }
+      // steps of the tile whose number, counted from the first tile on, is `set` modulo kSets
 #pragma unroll 1
-      for (int b = 0; b < a.nblk && ok; ++b, ++wi) {
-        const float d_now = d_next;
-        if (Q6 && b + 1 < a.nblk) d_next = __half2float(__ldcg(dq + b + 1));
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {                     // the block's two steps
-          const bool mine = turn == set;
-          if (++turn == S::kSets) turn = 0;
-          if (!mine) continue;
-          ok = warp_wait(wfull + ws, wph, a.status);
+      for (uint32_t own = (set + 2u * S::kSets - (2u * wi0) % S::kSets) % S::kSets; own < 2u * a.nblk; own += S::kSets) {
+          const uint32_t b = own >> 1, h = own & 1, wi = wi0 + b, ws = wi % S::kRawStages;
+          __half d_now = {};
+          if (Q6 && h == 0) d_now = __ldcg(dq + b);
+          ok = warp_wait(wfull + ws, (wi / S::kRawStages) & 1, a.status);
           const uint32_t raw = smem_u32(smem + S::kOffRaw + ws * S::kRawStage) + row * S::kRawBytes;
           // Q4_K: d, dmin, 6-bit scales and mins; Q6_K: the sixteen int8 scales
           const uint4 head = lds128(raw + (Q6 ? 192 : 0));
@@ -536,7 +534,7 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           tmem_fence_after();
           if (h == 0) {
             const __half2 dd = as_half2(head.x);
-            dring[(wi & 3) * 128 + row] = Q6 ? make_float2(d_now, 0.f) : make_float2(__low2float(dd), -__high2float(dd));
+            dring[(wi & 3) * 128 + row] = Q6 ? make_float2(__half2float(d_now), 0.f) : make_float2(__low2float(dd), -__high2float(dd));
           } else if (!Q6) {
             // m_0 .. m_7 twice (for the high and the low parts of the sums): 32 bytes, the same whatever the swizzle
             const uint32_t m0 = head.z & 0x3f3f3f3fu, m1 = ((head.w >> 4) & 0x0f0f0f0fu) | ((head.z >> 2) & 0x30303030u);
@@ -607,8 +605,6 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             mbar_arrive(full + (2 * wi + h) % S::kXStages);
             mbar_arrive(wempty + ws);
           }
-        }
-        if (++ws == S::kRawStages) { ws = 0; wph ^= 1; }
       }
     }
     if (!ok) abort_flag = 1;
