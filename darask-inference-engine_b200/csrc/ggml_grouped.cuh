@@ -68,7 +68,7 @@ struct GgShape {
   // Partial products per block of 256 columns. The tensor core cuts the sum of every 16 columns to the accumulator's 24 bits, toward
   // zero, so that the error grows with the number of sums and does not average out; products of two parts have bits to lose. In turn in
   // one accumulator they lost 1.5e-6 of the result (Q4_K, whose codes have no sign and largely cancel against the mins) and 8e-7 (Q6_K).
-  // The small products go first (Q6_K: 6e-7; an accumulator per step would bring 2e-7, but 513 us where this takes 449: 32768 rows, 128
+  // The small products go first (Q6_K: 6e-7; an accumulator per step would bring 2e-7, but took 513 us where this took 449: 32768 rows, 128
   // groups of 2048 x 768), and Q4_K has an accumulator of its own for every step as well (4e-7 for 4 % of the time).
   static constexpr int kSteps = Q6 ? 1 : NX;
   static_assert(kSteps == 2 || kXStages == 4 || Q6, "the promotion takes the stage of a block's second step from its buffer");
@@ -253,12 +253,22 @@ DEVI uint4 lds128(uint32_t addr) {
   return v;
 }
 
-// d = a (TMEM) x b (shared memory) in f16, float32 accumulation; issued by the lane with `go` set
-DEVI void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t go) {
+// d = a (TMEM) x b (shared memory) in f16, float32 accumulation; issued by the lane with `go` set. The eight products of a step, 64
+// columns of k per box of b, in one piece with one predicate: fewer instructions for the one warp that issues (Q6_K down 447 -> 435 us).
+DEVI void umma_f16_ts_step(uint32_t d, uint32_t a_tmem, uint64_t box0, uint64_t box1, uint32_t idesc, uint32_t accumulate, uint32_t go) {
   asm volatile(
-      "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %5, 0;\n\t"
-      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
+      "{\n\t.reg .pred p, g, one;\n\t.reg .b32 t;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 g, %6, 0;\n\tsetp.eq.b32 one, 0, 0;\n\t"
+      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %4, p;\n\t"
+      "add.u32 t, %1, 8;\n\tadd.s64 b, %2, 2;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], b, %4, one;\n\t"
+      "add.u32 t, %1, 16;\n\tadd.s64 b, %2, 4;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], b, %4, one;\n\t"
+      "add.u32 t, %1, 24;\n\tadd.s64 b, %2, 6;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], b, %4, one;\n\t"
+      "add.u32 t, %1, 32;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], %3, %4, one;\n\t"
+      "add.u32 t, %1, 40;\n\tadd.s64 b, %3, 2;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], b, %4, one;\n\t"
+      "add.u32 t, %1, 48;\n\tadd.s64 b, %3, 4;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], b, %4, one;\n\t"
+      "add.u32 t, %1, 56;\n\tadd.s64 b, %3, 6;\n\t@g tcgen05.mma.cta_group::1.kind::f16 [%0], [t], b, %4, one;\n\t"
+      "}"
+      ::"r"(d), "r"(a_tmem), "l"(box0), "l"(box1), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
 }
 DEVI void umma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t go) {
   asm volatile(
@@ -481,17 +491,10 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             const uint32_t at = tmem_a + (step ? a1 : a0) * 64, a2 = tmem_a2 + (step ? a1 : a0) * 64;
             const uint32_t d = tmem + (S::kSteps == 2 ? uint32_t(step) : buf) * NT;
             const uint32_t first = S::kSteps == 2 || step == 0 ? 0u : 1u;
-            auto box = [&](int q) -> uint64_t { return (q >> 2) * (S::kBox >> 4) + 2 * (q & 3); };      // 16 columns of k
-            if (NX == 2) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) umma_f16_ts(d, at + q * 8, dx + (S::kPart >> 4) + box(q), idesc, q ? 1u : first, go);
-            }
-            if (NA == 2) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) umma_f16_ts(d, a2 + q * 8, dx + box(q), idesc, NX == 2 || q ? 1u : first, go);
-            }
-#pragma unroll
-            for (int q = 0; q < 8; ++q) umma_f16_ts(d, at + q * 8, dx + box(q), idesc, NX == 2 || NA == 2 || q ? 1u : first, go);
+            const uint64_t dx1 = dx + (S::kBox >> 4), dl = dx + (S::kPart >> 4), dl1 = dl + (S::kBox >> 4);
+            if (NX == 2) umma_f16_ts_step(d, at, dl, dl1, idesc, first, go);
+            if (NA == 2) umma_f16_ts_step(d, a2, dx, dx1, idesc, NX == 2 ? 1u : first, go);
+            umma_f16_ts_step(d, at, dx, dx1, idesc, NX == 2 || NA == 2 ? 1u : first, go);
             if (!Q6 && step == 1)                            // sums times mins
               umma_f16_ss(tmem_min + (S::kMinBufs == 2 ? buf * NT : 0u), dmin + (S::kMins == 2 ? buf * (4096u >> 4) : 0u), dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);
             umma_commit_if(empty + x0 + step, go);
