@@ -193,3 +193,36 @@ def test_prefill_of_rows_on_any_word(tokens):
     y, ids, prob = m.prefill(x.clone(), n)
     y2, ids2, prob2 = m.prefill(off(x), off(n))
     assert torch.equal(y, y2) and torch.equal(ids, ids2) and torch.equal(prob, prob2)
+
+
+@pytest.mark.parametrize("dtype,ty", [(torch.bfloat16, 30), (torch.float16, 1)])
+def test_prefill_with_a_router_of_16_bits(dtype, ty):
+    """A 16-bit router and the same numbers in float32: the same bits."""
+    import darask_inference_engine_b200 as D
+    layer, acts = W.kogarashi_layer(23, hidden=512, inter=256, experts=40, topk=3, tokens=45, shared=True, pool=8)
+    m, _ = run_kogarashi(layer, acts)
+    runs = []
+    router = torch.from_numpy(layer.router).cuda().to(dtype)
+    gate = m.weights["ffn_gate_inp_shexp.weight"].data.view(torch.float32).to(dtype)
+    for cast, kind in ((torch.float32, 0), (dtype, ty)):
+        m.weights["ffn_gate_inp.weight"] = D.kogarashi.Weight(router.to(cast).contiguous().view(torch.uint8).view(-1), kind, 512, 40, (512, 40))
+        m.weights["ffn_gate_inp_shexp.weight"] = D.kogarashi.Weight(gate.to(cast).contiguous().view(torch.uint8).view(-1), kind, 512, 1, (512, 1))
+        runs.append(m.prefill(torch.from_numpy(acts["x"].copy()).cuda(), torch.from_numpy(acts["n"]).cuda()))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_two_prompts_at_once_through_one_layer():
+    """Scratch and routes belong to the call: prompts of different lengths on two streams, again and again, give the bits of one alone."""
+    layer, acts = W.kogarashi_layer(24, hidden=512, inter=256, experts=16, topk=4, tokens=150, shared=True, pool=8)
+    m, _ = run_kogarashi(layer, acts)
+    x, n = torch.from_numpy(acts["x"].copy()).cuda(), torch.from_numpy(acts["n"].copy()).cuda()
+    parts = [(x[:150], n[:150]), (x[:37], n[:37].flip(0).contiguous())]
+    alone = [m.prefill(a.clone(), b)[0] for a, b in parts]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(6):
+        for s, (a, b), want in zip(streams, parts, alone):
+            with torch.cuda.stream(s):
+                outs.append((m.prefill(a.clone(), b)[0], want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, want) for got, want in outs)
