@@ -68,12 +68,14 @@ static cudaError_t launch_rows(const GgRowsArgs& r, int parts, bool sums, cudaSt
   return launch_pdl(kernel, dim3(unsigned(r.rows)), dim3(kGgRowThreads), smem, st, r);
 }
 
-// f16 parts of a row and f16 terms of a Q6_K integer by the types: two terms where the output keeps float32
+// f16 parts of a row and f16 terms of a Q6_K integer by the output's type. float32 and f16 outputs take everything the operands hold (the
+// integers' second term: in one, rounded to 11 bits, an f16 result was off by 2.6e-4 where its own rounding is 2.1e-4). bf16 keeps 8
+// bits: one term and one part (2^-12 each) in front of it leave 1.7e-3, the error of its rounding, as it is.
 template <bool Q6, int NT>
 static cudaError_t launch_by_type(int out_ty, int nx, const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
   constexpr int NA = Q6 ? 2 : 1;
   if (out_ty == DARASK_GGML_F32) return nx == 2 ? launch_products<Q6, NT, 2, NA, float>(m, a, st) : launch_products<Q6, NT, 1, NA, float>(m, a, st);
-  if (out_ty == DARASK_GGML_F16) return nx == 2 ? launch_products<Q6, NT, 2, 1, __half>(m, a, st) : launch_products<Q6, NT, 1, 1, __half>(m, a, st);
+  if (out_ty == DARASK_GGML_F16) return nx == 2 ? launch_products<Q6, NT, 2, NA, __half>(m, a, st) : launch_products<Q6, NT, 1, NA, __half>(m, a, st);
   return launch_products<Q6, NT, 1, 1, __nv_bfloat16>(m, a, st);
 }
 
