@@ -43,14 +43,14 @@ static GroupedWs carve(void* base, long long rows, int k, int parts) {
   return w;
 }
 
-template <bool Q6, int NT, int NX, int NA, typename OUT>
+template <bool Q6, int NT, int NX, typename OUT>
 static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
-  using S = GgShape<Q6, NT, NX, NA>;
+  using S = GgShape<Q6, NT, NX>;
   static_assert(S::kSmem + 3 * 1024 <= kSmemBudget, "rings and 3 KB of barriers and scales must fit one block");
   static bool configured[64] = {};      // the opt-in is per device and per kernel
   const int dev = current_device_slot();
   if (dev < 0) return cudaErrorInvalidDevice;
-  auto kernel = ggml_grouped_kernel<Q6, NT, NX, NA, OUT>;
+  auto kernel = ggml_grouped_kernel<Q6, NT, NX, OUT>;
   if (!configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
@@ -61,22 +61,27 @@ static cudaError_t launch_products(const CUtensorMap (&m)[6], const GgArgs& a, c
 
 template <int KIND>
 static cudaError_t launch_rows(const GgRowsArgs& r, int parts, bool sums, cudaStream_t st) {
-  auto kernel = sums ? ggml_rows_kernel<KIND, false, true> : ggml_rows_kernel<KIND, false, false>;
-  if constexpr (KIND != 2 && KIND != 3)                  // plain 16-bit rows have one part
-    if (parts == 2) kernel = sums ? ggml_rows_kernel<KIND, true, true> : ggml_rows_kernel<KIND, true, false>;
+  constexpr bool kOne = KIND == 2 || KIND == 3;          // plain 16-bit rows have one part, float32 and SwiGLU rows two
+  auto kernel = sums ? ggml_rows_kernel<KIND, !kOne, true> : ggml_rows_kernel<KIND, !kOne, false>;
+  if constexpr (KIND == 0)
+    if (parts == 1) kernel = sums ? ggml_rows_kernel<KIND, false, true> : ggml_rows_kernel<KIND, false, false>;
   const size_t smem = size_t(r.src.k < kGgRowHeld ? r.src.k : kGgRowHeld) * sizeof(float);
   return launch_pdl(kernel, dim3(unsigned(r.rows)), dim3(kGgRowThreads), smem, st, r);
 }
 
-// f16 parts of a row and f16 terms of a Q6_K integer by the output's type. float32 and f16 outputs take everything the operands hold (the
-// integers' second term: in one, rounded to 11 bits, an f16 result was off by 2.6e-4 where its own rounding is 2.1e-4). bf16 keeps 8
-// bits: one term and one part (2^-12 each) in front of it leave 1.7e-3, the error of its rounding, as it is.
+// Every output type takes all that the operands hold. With one part of two-part rows (11 bits of 22) and one term of Q6_K's integers in front
+// of bf16 and f16, bf16 results were off by up to 1.73e-3 and f16 ones by 2.6e-4, where their own roundings are 1.66e-3 and 2.07e-4; the
+// second part and the second term cost bf16 results 12 to 30 % of the time (32768 rows, 128 groups of 2048 x 768 Q6_K: 286 -> 314 us for bf16
+// rows, 288 -> 347 us for float32 rows).
+template <bool Q6, int NT, typename OUT>
+static cudaError_t launch_by_parts(int parts, const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
+  return parts == 2 ? launch_products<Q6, NT, 2, OUT>(m, a, st) : launch_products<Q6, NT, 1, OUT>(m, a, st);
+}
 template <bool Q6, int NT>
-static cudaError_t launch_by_type(int out_ty, int nx, const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
-  constexpr int NA = Q6 ? 2 : 1;
-  if (out_ty == DARASK_GGML_F32) return nx == 2 ? launch_products<Q6, NT, 2, NA, float>(m, a, st) : launch_products<Q6, NT, 1, NA, float>(m, a, st);
-  if (out_ty == DARASK_GGML_F16) return nx == 2 ? launch_products<Q6, NT, 2, NA, __half>(m, a, st) : launch_products<Q6, NT, 1, NA, __half>(m, a, st);
-  return launch_products<Q6, NT, 1, 1, __nv_bfloat16>(m, a, st);
+static cudaError_t launch_by_type(int out_ty, int parts, const CUtensorMap (&m)[6], const GgArgs& a, cudaStream_t st) {
+  if (out_ty == DARASK_GGML_F32) return launch_by_parts<Q6, NT, float>(parts, m, a, st);
+  if (out_ty == DARASK_GGML_F16) return launch_by_parts<Q6, NT, __half>(parts, m, a, st);
+  return launch_by_parts<Q6, NT, __nv_bfloat16>(parts, m, a, st);
 }
 
 }  // namespace dmoe
@@ -117,8 +122,6 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   if (e) return e;
   const bool q6 = d->w_ty == DARASK_GGML_Q6_K;
   const int parts = row_parts(d->x_ty, d->swiglu), row_bytes = ggml_row_bytes(d->w_ty, d->k), nblk = d->k / 256;
-  // a bf16 result keeps 8 bits: one f16 part (11 bits) of float32 rows is enough in front of it
-  const int nx = d->out_ty == DARASK_GGML_BF16 ? 1 : parts;
   const GroupedWs ws = carve(d->workspace, d->rows, d->k, parts);
   GgRowsArgs r = {};
   r.src = RowSource{d->x, d->ldx, d->x_ty, d->k, d->swiglu, row_source_vec(d->x, d->x_ty, d->ldx, d->k, d->swiglu)};
@@ -129,8 +132,8 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   CUtensorMap m[6];                     // weights (two matrices), rows of x by 32 and by 128, their sums by 32 and by 128
   if (!byte_map(m + 0, d->w, wrows, wcols, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
       !byte_map(m + 1, d->w_up ? d->w_up : d->w, wrows, wcols, row_bytes, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-      !byte_map(m + 2, ws.planes, (unsigned long long)nx * d->rows, d->k * 2ull, d->k * 2ull, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !byte_map(m + 3, ws.planes, (unsigned long long)nx * d->rows, d->k * 2ull, d->k * 2ull, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !byte_map(m + 2, ws.planes, (unsigned long long)parts * d->rows, d->k * 2ull, d->k * 2ull, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !byte_map(m + 3, ws.planes, (unsigned long long)parts * d->rows, d->k * 2ull, d->k * 2ull, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !byte_map(m + 4, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !byte_map(m + 5, ws.sum, d->rows, nblk * 32ull, nblk * 32ull, 128, 32, CU_TENSOR_MAP_SWIZZLE_32B))
     return cudaErrorInvalidValue;
@@ -138,13 +141,13 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   const bool whole = r.src.vec >= (d->x_ty == DARASK_GGML_F32 ? 1 : 2) && d->ldx % (d->x_ty == DARASK_GGML_F32 ? 4 : 8) == 0;
   const int kind = !whole ? 0 : (d->x_ty == DARASK_GGML_F32 ? 1 : d->x_ty == DARASK_GGML_F16 ? 2 : 3) + (d->swiglu ? 3 : 0);
   switch (kind) {
-    case 0: e = launch_rows<0>(r, nx, !q6, st); break;
-    case 1: e = launch_rows<1>(r, nx, !q6, st); break;
-    case 2: e = launch_rows<2>(r, nx, !q6, st); break;
-    case 3: e = launch_rows<3>(r, nx, !q6, st); break;
-    case 4: e = launch_rows<4>(r, nx, !q6, st); break;
-    case 5: e = launch_rows<5>(r, nx, !q6, st); break;
-    default: e = launch_rows<6>(r, nx, !q6, st);
+    case 0: e = launch_rows<0>(r, parts, !q6, st); break;
+    case 1: e = launch_rows<1>(r, parts, !q6, st); break;
+    case 2: e = launch_rows<2>(r, parts, !q6, st); break;
+    case 3: e = launch_rows<3>(r, parts, !q6, st); break;
+    case 4: e = launch_rows<4>(r, parts, !q6, st); break;
+    case 5: e = launch_rows<5>(r, parts, !q6, st); break;
+    default: e = launch_rows<6>(r, parts, !q6, st);
   }
   if (e) return e;
   GgArgs a = {};
@@ -155,8 +158,8 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
   a.aligned = reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->ldo * ob % 16 == 0 && (!d->w_up || d->n * ob % 16 == 0);
   a.status = status;
   const bool narrow = grouped_narrow(d);
-  if (q6) return narrow ? launch_by_type<true, 32>(d->out_ty, nx, m, a, st) : launch_by_type<true, 128>(d->out_ty, nx, m, a, st);
-  return narrow ? launch_by_type<false, 32>(d->out_ty, nx, m, a, st) : launch_by_type<false, 128>(d->out_ty, nx, m, a, st);
+  if (q6) return narrow ? launch_by_type<true, 32>(d->out_ty, parts, m, a, st) : launch_by_type<true, 128>(d->out_ty, parts, m, a, st);
+  return narrow ? launch_by_type<false, 32>(d->out_ty, parts, m, a, st) : launch_by_type<false, 128>(d->out_ty, parts, m, a, st);
 }
 
 extern "C" int darask_ggml_grouped_status(unsigned* host_status, cudaStream_t st) {

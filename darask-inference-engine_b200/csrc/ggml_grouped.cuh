@@ -2,8 +2,8 @@
 //   out[i][j] = x[row(i)] . W_g[j]      for the dispatch rows i of every group g
 // A block of 256 weights is d times integers, sc_b q (Q4_K, at most 945) or sc_b (q - 32) (Q6_K, at most 4096), less dmin
 // times integers m_b that multiply the sums of x over 32 columns (Q4_K). The tensor cores multiply these integers: f16 holds
-// Q4_K's exactly (11 significant bits) and Q6_K's to 2^-12 (a second f16 term holds the rest where the output is float32), so
-// a weight is never rounded and has no range to lose. d and dmin are applied in float32 once per 256 columns, when the partial
+// Q4_K's exactly (11 significant bits) and Q6_K's to 2^-12 (a second f16 term holds the rest), so a weight is never rounded and
+// has no range to lose, whatever the type of the output. d and dmin are applied in float32 once per 256 columns, when the partial
 // product leaves TMEM. A row of x is divided by a power of two (largest value into [2^9, 2^10)) and split into one or two f16
 // parts (float32: 22 bits); the power of two comes back in the store.
 //
@@ -41,14 +41,14 @@ struct GgArgs {
   unsigned* status;
 };
 
-// NT: rows of x per tile, NX: f16 parts of a row of x, NA: f16 terms of a Q6_K integer. A step is 128 columns of k.
-template <bool Q6, int NT, int NX, int NA>
+// NT: rows of x per tile, NX: f16 parts of a row of x. A step is 128 columns of k.
+template <bool Q6, int NT, int NX>
 struct GgShape {
   // TMEM holds the weights of kSets steps, and a set of four expander warps belongs to each slot. Few rows leave room for four slots,
   // whose sets hide their latencies from each other; 128 rows leave two (there, sets that fill each step together took 439 us where
   // these take 423, and four promotion warps instead of eight 466: 32768 rows, 128 groups of 2 x 768 x 2048).
   static constexpr bool kWide = NT > 32;
-  static constexpr int kSets = kWide ? 2 : NA == 2 ? 3 : 4;
+  static constexpr int kSets = kWide ? 2 : Q6 ? 3 : 4;
   static constexpr int kPromote = kWide ? 8 : 4;         // warps that promote and store: two per quarter of the weight rows, half of x each
   static constexpr int kThreads = 128 * (1 + kSets) + 32 * kPromote;
   // wide: registers of the roles, the expanders and the promotion; their sum is what the block is launched with (640 x 96)
@@ -86,7 +86,7 @@ struct GgShape {
   // TMEM columns: two main buffers, one or two of min products, the weights, their second terms
   static constexpr int kMinBufs = Q6 ? 0 : kWide ? 1 : 2;
   static constexpr uint32_t kColMin = 2 * NT, kColA = kColMin + kMinBufs * NT, kColA2 = kColA + 64 * kSets;
-  static_assert(kRawStages >= 3 && kColA2 + (NA == 2 ? 64 * kSets : 0) <= 512, "rings must fit");
+  static_assert(kRawStages >= 3 && kColA2 + (Q6 ? 64 * kSets : 0) <= 512, "rings must fit");
 };
 
 // ---- rows of x -> f16 parts --------------------------------------------------------------------------------------------
@@ -288,12 +288,12 @@ template <> DEVI float from_float<float>(float v) { return v; }
 template <> DEVI __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> DEVI __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <bool Q6, int NT, int NX, int NA, typename OUT>
-__global__ void __launch_bounds__((GgShape<Q6, NT, NX, NA>::kThreads), 1)
+template <bool Q6, int NT, int NX, typename OUT>
+__global__ void __launch_bounds__((GgShape<Q6, NT, NX>::kThreads), 1)
 ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x4, const __grid_constant__ CUtensorMap map_sum,
                     const __grid_constant__ CUtensorMap map_sum4, const GgArgs a) {
-  using S = GgShape<Q6, NT, NX, NA>;
+  using S = GgShape<Q6, NT, NX>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float2* dring = reinterpret_cast<float2*>(smem + S::kOffD);               // [4][128] {d, dmin} of the rows
@@ -493,8 +493,8 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             const uint32_t first = S::kSteps == 2 || step == 0 ? 0u : 1u;
             const uint64_t dx1 = dx + (S::kBox >> 4), dl = dx + (S::kPart >> 4), dl1 = dl + (S::kBox >> 4);
             if (NX == 2) umma_f16_ts_step(d, at, dl, dl1, idesc, first, go);
-            if (NA == 2) umma_f16_ts_step(d, a2, dx, dx1, idesc, NX == 2 ? 1u : first, go);
-            umma_f16_ts_step(d, at, dx, dx1, idesc, NX == 2 || NA == 2 ? 1u : first, go);
+            if (Q6) umma_f16_ts_step(d, a2, dx, dx1, idesc, NX == 2 ? 1u : first, go);
+            umma_f16_ts_step(d, at, dx, dx1, idesc, NX == 2 || Q6 ? 1u : first, go);
             if (!Q6 && step == 1)                            // sums times mins
               umma_f16_ss(tmem_min + (S::kMinBufs == 2 ? buf * NT : 0u), dmin + (S::kMins == 2 ? buf * (4096u >> 4) : 0u), dsum0 + (x0 + step) * uint32_t(S::kXStage >> 4), idesc, 0u, go);
             umma_commit_if(empty + x0 + step, go);
@@ -593,11 +593,11 @@ ggml_grouped_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
                                             __float2half2_rn(1056.f));                    // q - 32
                   const __half2 p = __hmul2(z, sc);
                   v[2 * q + o] = as_word(p);
-                  if (NA == 2) r[2 * q + o] = as_word(__hfma2(z, sc, __hneg2(p)));
+                  r[2 * q + o] = as_word(__hfma2(z, sc, __hneg2(p)));
                 }
               }
               tmem_st16(tmem_a + dst + part * 16, v);
-              if (NA == 2) tmem_st16(tmem_a2 + dst + part * 16, r);
+              tmem_st16(tmem_a2 + dst + part * 16, r);
             }
           }
           }
