@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .formats import GGML_Q4_K, GGML_Q6_K, ggml_tensor_bytes, q6k_r16_row_bytes
+from .formats import GGML_BF16, GGML_F16, GGML_F32, GGML_Q4_K, GGML_Q6_K, ggml_tensor_bytes, q6k_r16_row_bytes
 
 TENSORS = ("ffn_gate_inp.weight", "ffn_gate_exps.weight", "ffn_up_exps.weight", "ffn_down_exps.weight",
            "ffn_gate_shexp.weight", "ffn_up_shexp.weight", "ffn_down_shexp.weight", "ffn_gate_inp_shexp.weight")
@@ -92,13 +92,28 @@ def grouped_status(device="cuda") -> int:
     return s.value
 
 
+def _marking(method):
+    def call(self, *args, **kw):
+        self.changed = True
+        return method(self, *args, **kw)
+    return call
+
+
+class _Tensors(dict):
+    """A layer's tensors by name. Remembers that one was put in or taken out, so that the layer looks them over before its next call
+    and not in front of every one (a `Weight` is replaced, not edited)."""
+    changed = True
+    __setitem__, __delitem__, __ior__ = _marking(dict.__setitem__), _marking(dict.__delitem__), _marking(dict.__ior__)
+    update, setdefault, pop, popitem, clear = (_marking(m) for m in (dict.update, dict.setdefault, dict.pop, dict.popitem, dict.clear))
+
+
 class KogarashiMoeLayer:
     """One layer's MoE FFN: weights resident on one GPU, buffers sized for `max_tokens`."""
 
     def __init__(self, hidden: int, inter: int, experts: int, topk: int, max_tokens: int = 1, device="cuda"):
         self.hidden, self.inter, self.experts, self.topk, self.max_tokens = hidden, inter, experts, topk, max_tokens
         self.device = torch.device(device)
-        self.weights: dict[str, Weight] = {}
+        self.weights: dict[str, Weight] = _Tensors()
         self.router_bias = None   # optional float32 [experts] logit offset (not in the reference model)
         lib = _lib.lib()
         nbytes = lib.kogarashi_moe_workspace_bytes(hidden, inter, experts, topk, max_tokens)
@@ -129,6 +144,39 @@ class KogarashiMoeLayer:
             raw = packed
         self.weights[name] = Weight(raw, ty, k, rows, ne)
 
+    def _check_weights(self) -> None:
+        """The kernels take addresses and decode what is there by the layer's sizes and by one type each for gate and up, down, and the
+        router; the shared expert has no sizes or types of its own. So every tensor must have just these."""
+        h, f, e, t = self.hidden, self.inter, self.experts, self.weights
+        exps = {"gate": (h, f), "up": (h, f), "down": (f, h)}
+        shapes = {"ffn_gate_inp.weight": (h, e), "ffn_gate_inp_shexp.weight": (h,)}
+        for name, ne in exps.items():
+            shapes[f"ffn_{name}_exps.weight"], shapes[f"ffn_{name}_shexp.weight"] = ne + (e,), ne
+
+        def strip(ne):                   # trailing dimensions of one say nothing
+            ne = tuple(ne)
+            while len(ne) > 1 and ne[-1] == 1:
+                ne = ne[:-1]
+            return ne
+        for name, ne in shapes.items():
+            w = t.get(name)
+            if w is None:
+                continue
+            if strip(w.ne) != strip(ne):
+                raise ValueError(f"{name}: shape {list(w.ne)}, the layer needs {list(ne)}")
+            if w.ty not in ((GGML_F32, GGML_F16, GGML_BF16) if "inp" in name else (GGML_Q4_K, GGML_Q6_K)):
+                raise ValueError(f"{name}: GGML type {w.ty} is not supported here")
+            rows = ggml_tensor_bytes(w.ty, ne) // ggml_tensor_bytes(w.ty, ne[:1])
+            nbytes = rows * q6k_r16_row_bytes(ne[0]) if w.ty == GGML_Q6_K else ggml_tensor_bytes(w.ty, ne)
+            if w.data.dtype is not torch.uint8 or not w.data.is_contiguous() or w.data.numel() != nbytes or \
+                    w.data.get_device() != self.workspace.get_device():
+                raise ValueError(f"{name}: data must be {nbytes} contiguous bytes on the layer's device")
+        for name, like in (("ffn_up_exps", "ffn_gate_exps"), ("ffn_gate_shexp", "ffn_gate_exps"), ("ffn_up_shexp", "ffn_gate_exps"),
+                           ("ffn_down_shexp", "ffn_down_exps"), ("ffn_gate_inp_shexp", "ffn_gate_inp")):
+            a, b = t.get(name + ".weight"), t.get(like + ".weight")
+            if a is not None and b is not None and a.ty != b.ty:
+                raise ValueError(f"{name}.weight: GGML type {a.ty}, must be that of {like}.weight, {b.ty}")
+
     def _w(self, name):
         w = self.weights.get(name)
         return (w.data.data_ptr(), w.ty) if w is not None else (None, 0)
@@ -151,6 +199,10 @@ class KogarashiMoeLayer:
 
     def _descriptor(self, x, n, attn_out, norm_w, eps):
         """The call's descriptor but for its routes and its workspace."""
+        if getattr(self.weights, "changed", True):
+            self._check_weights()
+            if isinstance(self.weights, _Tensors):
+                self.weights.changed = False
         d = _lib.KogarashiMoe()
         d.hidden, d.inter, d.experts, d.topk, d.tokens = self.hidden, self.inter, self.experts, self.topk, n.shape[0]
         d.router_w, d.router_ty = self._w("ffn_gate_inp.weight")
