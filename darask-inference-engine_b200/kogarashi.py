@@ -216,8 +216,9 @@ class KogarashiMoeLayer:
         d.sh_inp_w = self._w("ffn_gate_inp_shexp.weight")[0]
         d.n, d.x = n.data_ptr(), x.data_ptr()
         if norm_w is not None:
-            if norm_w.dtype != torch.float32 or norm_w.numel() != self.hidden or (attn_out is not None and (attn_out.shape != x.shape or attn_out.dtype != torch.float32)):
-                raise ValueError("norm_w / attn_out")
+            if norm_w.dtype != torch.float32 or norm_w.numel() != self.hidden or not norm_w.is_contiguous() or \
+                    (attn_out is not None and (attn_out.shape != x.shape or attn_out.dtype != torch.float32 or not attn_out.is_contiguous())):
+                raise ValueError("norm_w and attn_out must be contiguous float32 [H] and [T, H]")
             d.norm_w, d.norm_eps = norm_w.data_ptr(), eps
             d.attn_out = attn_out.data_ptr() if attn_out is not None else None
         elif attn_out is not None:

@@ -71,3 +71,14 @@ def test_tensors_replaced_later_are_looked_at_again():
             descriptor(m)
     m.weights.update({"ffn_down_shexp.weight": w})
     descriptor(m)
+
+
+def test_strided_inputs_of_the_layer_entry_are_refused():
+    """The entry kernel reads attn_out and norm_w as packed rows: views with strides gave other numbers."""
+    m = layer()
+    x, norm = torch.zeros(2, H), torch.ones(H)
+    for attn_out, norm_w in ((torch.zeros(2, 2 * H)[:, :H], norm), (torch.zeros(H, 2).t(), norm), (x.clone(), torch.ones(2 * H)[::2]), (None, torch.ones(2 * H)[::2])):
+        with pytest.raises(ValueError, match="norm_w"):
+            m._descriptor(x, x.clone(), attn_out, norm_w, 1e-6)
+    d = m._descriptor(x, x.clone(), x, norm, 1e-6)
+    assert d.attn_out == x.data_ptr() and d.norm_w == norm.data_ptr()
