@@ -71,6 +71,7 @@ class DaraskFp8Linear(ctypes.Structure):
         ("x", c_void_p), ("x_ty", c_int), ("ldx", c_longlong), ("x_scales", c_void_p), ("ld_xs", c_longlong), ("swiglu", c_int),
         ("w", c_void_p), ("ldw", c_longlong), ("w_scales", c_void_p), ("ld_ws", c_longlong),
         ("out", c_void_p), ("out_ty", c_int), ("ldo", c_longlong), ("add", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("status", c_void_p),
     ]
 
 
@@ -82,10 +83,12 @@ class DaraskGgmlGrouped(ctypes.Structure):
         ("assignments", c_void_p), ("topk", c_int), ("swiglu", c_int),
         ("w", c_void_p), ("w_up", c_void_p), ("w_ty", c_int),
         ("out", c_void_p), ("out_ty", c_int), ("ldo", c_longlong), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("status", c_void_p),
     ]
 
 
 _SIGNATURES = {
+    "darask_status_take": (c_int, [c_void_p, ctypes.POINTER(c_uint), c_void_p]),
     "darask_fp8_linear_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "darask_fp8_linear": (c_int, [ctypes.POINTER(DaraskFp8Linear), c_void_p]),
     "darask_fp8_linear_status": (c_int, [ctypes.POINTER(c_uint), c_void_p]),
@@ -219,6 +222,25 @@ def current_stream(device_index: int) -> int:
         return torch._C._cuda_getCurrentRawStream(device_index)      # what torch.cuda.current_stream(...).cuda_stream holds, without the object
     except AttributeError:
         return torch.cuda.current_stream(device_index).cuda_stream
+
+
+def status_pointer(status, device_index: int):
+    """Address of a caller's status word (int32 tensor of one element), None without one."""
+    if status is None:
+        return None
+    import torch
+    if status.dtype is not torch.int32 or status.numel() != 1 or status.get_device() != device_index:
+        raise ValueError("status must be one int32 on the device of the call")
+    return status.data_ptr()
+
+
+def take_status(word) -> int:
+    """Bits of a status word (int32 tensor of one element on a GPU); clears it and synchronizes the current stream of its device."""
+    import torch
+    s = c_uint(0)
+    with torch.cuda.device(word.device):
+        check(lib().darask_status_take(word.data_ptr(), ctypes.byref(s), current_stream(word.get_device())), "darask_status_take")
+    return s.value
 
 
 def row_stride(t) -> int:

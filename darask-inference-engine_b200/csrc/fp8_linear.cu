@@ -6,23 +6,14 @@
 #include <cuda_fp8.h>
 #include "fp8_linear_stream.cuh"
 #include "fp8_linear_tile.cuh"
+#include "status.cuh"
 
 namespace dmoe {
 
 static __device__ unsigned g_fp8_linear_status;
-// its address, looked up once per device
 static cudaError_t status_word(unsigned** p) {
   static unsigned* known[64] = {};
-  const int dev = current_device_slot();
-  if (dev < 0) return cudaErrorInvalidDevice;
-  if (!known[dev]) {
-    void* q = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&q, g_fp8_linear_status);
-    if (e != cudaSuccess) return e;
-    known[dev] = static_cast<unsigned*>(q);
-  }
-  *p = known[dev];
-  return cudaSuccess;
+  return device_word(g_fp8_linear_status, known, p);
 }
 
 // One warp per row and 128 columns, four columns per lane: scale = absmax / 448 (1 for zeros), code = e4m3(x * (1 / scale)),
@@ -140,6 +131,7 @@ static bool linear_ok(const DaraskFp8Linear* d) {
   if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->m > (1 << 24) || d->n > (1 << 24) || d->k > (1 << 20)) return false;
   if (!d->w || !d->w_scales || reinterpret_cast<uintptr_t>(d->w_scales) % 4 || reinterpret_cast<uintptr_t>(d->w) % 16 || d->ldw % 16 || d->ldw < d->k) return false;
   const long long kb = (d->k + 127) / 128;
+  if (reinterpret_cast<uintptr_t>(d->status) % 4) return false;
   if (d->ld_ws < kb || !row_type_bytes(d->out_ty) || d->ldo < d->n || (d->add && d->out_ty != DARASK_GGML_F32)) return false;
   if (d->m == 0) return true;
   if (!d->x || !d->out || reinterpret_cast<uintptr_t>(d->out) % row_type_bytes(d->out_ty)) return false;
@@ -156,9 +148,9 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
   if (!linear_ok(d)) return cudaErrorInvalidValue;
   if (d->m == 0) return cudaSuccess;
   const int kb = (d->k + 127) / 128;
-  unsigned* status = nullptr;
-  cudaError_t e = status_word(&status);
-  if (e != cudaSuccess) return e;
+  unsigned* status = d->status;
+  cudaError_t e = cudaSuccess;
+  if (!status && (e = status_word(&status))) return e;
   const bool codes = d->x_ty == DARASK_E4M3;
   const LinearPlan p = linear_plan(d->m, d->n, kb, codes);
   FsArgs a = {};
@@ -198,8 +190,6 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
 extern "C" int darask_fp8_linear_status(unsigned* host_status, cudaStream_t st) {
   if (!host_status) return cudaErrorInvalidValue;
   unsigned* p = nullptr;
-  cudaError_t e = status_word(&p);
-  if (!e) e = cudaMemcpyAsync(host_status, p, 4, cudaMemcpyDeviceToHost, st);
-  if (!e) e = cudaMemsetAsync(p, 0, 4, st);
-  return e ? e : cudaStreamSynchronize(st);
+  const cudaError_t e = status_word(&p);
+  return e ? e : darask_status_take(p, host_status, st);
 }

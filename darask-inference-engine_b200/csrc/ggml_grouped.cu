@@ -4,23 +4,14 @@
 // of 256 columns (kogarashi kernels/native.cu:21-41).
 #include "../../include/darask_moe_b200.h"
 #include "ggml_grouped.cuh"
+#include "status.cuh"
 
 namespace dmoe {
 
 static __device__ unsigned g_ggml_grouped_status;
-// its address, looked up once per device
 static cudaError_t status_word(unsigned** p) {
   static unsigned* known[64] = {};
-  const int dev = current_device_slot();
-  if (dev < 0) return cudaErrorInvalidDevice;
-  if (!known[dev]) {
-    void* q = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&q, g_ggml_grouped_status);
-    if (e != cudaSuccess) return e;
-    known[dev] = static_cast<unsigned*>(q);
-  }
-  *p = known[dev];
-  return cudaSuccess;
+  return device_word(g_ggml_grouped_status, known, p);
 }
 
 static int ggml_row_bytes(int ty, int k) {
@@ -105,6 +96,7 @@ static bool grouped_ok(const DaraskGgmlGrouped* d) {
   if (!d->w || reinterpret_cast<uintptr_t>(d->w) % 16 || reinterpret_cast<uintptr_t>(d->w_up) % 16 || !ggml_row_bytes(d->w_ty, d->k)) return false;
   const size_t eb = row_type_bytes(d->x_ty), ob = row_type_bytes(d->out_ty);
   if (!eb || !ob || d->ldx < (d->swiglu ? 2ll : 1ll) * d->k || d->ldo < (d->w_up ? 2ll : 1ll) * d->n) return false;
+  if (reinterpret_cast<uintptr_t>(d->status) % 4) return false;
   if (d->assignments && (d->topk < 1 || reinterpret_cast<uintptr_t>(d->assignments) % 4)) return false;
   if (grouped_tile_cap(d) >= 1ll << 30) return false;      // tiles are counted in 32 bits, two counts added
   if (d->rows == 0) return true;
@@ -117,9 +109,9 @@ static bool grouped_ok(const DaraskGgmlGrouped* d) {
 extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t st) {
   if (!grouped_ok(d)) return cudaErrorInvalidValue;
   if (d->rows == 0) return cudaSuccess;
-  unsigned* status = nullptr;
-  cudaError_t e = status_word(&status);
-  if (e) return e;
+  unsigned* status = d->status;
+  cudaError_t e = cudaSuccess;
+  if (!status && (e = status_word(&status))) return e;
   const bool q6 = d->w_ty == DARASK_GGML_Q6_K;
   const int parts = row_parts(d->x_ty, d->swiglu), row_bytes = ggml_row_bytes(d->w_ty, d->k), nblk = d->k / 256;
   const GroupedWs ws = carve(d->workspace, d->rows, d->k, parts);
@@ -165,8 +157,6 @@ extern "C" int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* d, cudaStream_t
 extern "C" int darask_ggml_grouped_status(unsigned* host_status, cudaStream_t st) {
   if (!host_status) return cudaErrorInvalidValue;
   unsigned* p = nullptr;
-  cudaError_t e = status_word(&p);
-  if (!e) e = cudaMemcpyAsync(host_status, p, 4, cudaMemcpyDeviceToHost, st);
-  if (!e) e = cudaMemsetAsync(p, 0, 4, st);
-  return e ? e : cudaStreamSynchronize(st);
+  const cudaError_t e = status_word(&p);
+  return e ? e : darask_status_take(p, host_status, st);
 }

@@ -39,14 +39,15 @@ def grouped_gemm(a_codes, a_scales, ranges, w0, sw0, w1=None, sw1=None, quantize
     return (out, scales) if mode == 2 else out
 
 
-def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None, add=False):
+def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None, add=False, status=None):
     """Dense product in block-scaled FP8, x [m, k] -> [m, n].  w uint8 (e4m3 codes) [n, k], w_scales float32 [ceil(n/128), >= ceil(k/128)]
     (``quantize.fp8_block``).  x float32, float16 or bfloat16 is quantized by the call with one scale per row and 128 columns; with
     `swiglu` its rows hold gate | up ([m, 2k]) and silu(gate) * up is quantized.  x uint8 holds e4m3 codes, with x_scales float32
     [m, >= ceil(k/128)] (``quantize.fp8_act``).  Sums are float32; `out_dtype` (float32, float16, bfloat16) defaults to x's type, or
     bfloat16 for codes.  With `add` the product is added to what a float32 `out` holds.  `out` must not overlap an input.  Rows
     may be strided; rows of w and of codes start on 16-byte boundaries.  Any m, including 0; k as w has it.
-    Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
+    `status`: one int32 on the device to which the call's status bits are added (OR); without it they go to the device's shared word,
+    which `linear_status` reads.  Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
     if w.dim() != 2 or w.dtype is not torch.uint8 or w_scales.dim() != 2 or w_scales.dtype is not torch.float32:
         raise ValueError("w must be uint8 [n, k] and w_scales float32 [n blocks, k blocks]")
     n, k = w.shape
@@ -80,22 +81,24 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
     xp, wp = x.data_ptr(), w.data_ptr()
     if wp % 16 or ldw % 16 or (codes and m and (xp % 16 or ldx % 16)):
         raise ValueError("rows of w and of codes must start on 16-byte boundaries")
+    word = None if status is None else _lib.status_pointer(status, dev)
     if m == 0:
         return out
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return linear(x, w, w_scales, x_scales, swiglu, None, out, add)
+            return linear(x, w, w_scales, x_scales, swiglu, None, out, add, status)
     lib = _lib.lib()
     nbytes = lib.darask_fp8_linear_workspace_bytes(m, n, k, ty)
     scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     d = _lib.DaraskFp8Linear(m, n, k, xp, ty, ldx, x_scales.data_ptr() if codes else None, ldxs, 1 if swiglu else 0, wp, ldw,
-                             w_scales.data_ptr(), ldws, out.data_ptr(), out_ty, ldo, 1 if add else 0, scratch.data_ptr() if nbytes else None, nbytes)
+                             w_scales.data_ptr(), ldws, out.data_ptr(), out_ty, ldo, 1 if add else 0, scratch.data_ptr() if nbytes else None, nbytes,
+                             word)
     _lib.check(lib.darask_fp8_linear(ctypes.byref(d), _lib.current_stream(dev)), "darask_fp8_linear")
     return out
 
 
 def linear_status(device="cuda") -> int:
-    """Status bits that `linear` calls on this device have set since the last look; clears them and synchronizes the current stream."""
+    """Status bits that `linear` calls without a `status` of their own have set on this device since the last look; clears them and synchronizes the current stream."""
     s = ctypes.c_uint(0)
     device = torch.device(device)
     with torch.cuda.device(device):

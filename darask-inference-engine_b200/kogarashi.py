@@ -28,14 +28,15 @@ class Weight:
     ne: tuple
 
 
-def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=False, out_dtype=None, out=None):
+def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=False, out_dtype=None, out=None, status=None):
     """Product grouped by expert over GGUF weights: out[i] = x[row(i)] . W_g^T for the rows i of every group g.
     weight: a Q4_K or Q6_K `Weight` of GGML order [k, n, groups] as ``KogarashiMoeLayer.load`` keeps it (Q6_K regrouped);
     with `up`, a second one of the same shape, out holds both products side by side ([rows, 2n]).  ranges int32 [groups, 2] =
     {rows, offset}.  x float32, float16 or bfloat16 [*, k]; dispatch row i reads x row assignments[i] // topk (int32, on the
     device), or row i without assignments.  With `swiglu` the rows of x hold gate | up ([*, 2k]) and silu(gate) * up is multiplied.
     Sums are float32; `out_dtype` defaults to x's type.  Ranges do not overlap, `out` overlaps no input.  Rows outside every range
-    are left as they were (uninitialised when `out` is not given).  Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
+    are left as they were (uninitialised when `out` is not given).  `status`: one int32 on the device to which the call's status bits are added
+    (OR); without it they go to the device's shared word, which `grouped_status` reads.  Runs on the current stream of x's device and does not synchronize; the scratch belongs to the call."""
     k, n, groups = weight.k, weight.rows, weight.ne[2] if len(weight.ne) > 2 else 1
     if weight.ty not in (GGML_Q4_K, GGML_Q6_K) or k < 256 or k % 256 or n < 1 or not 1 <= groups <= 1024:
         raise ValueError("weight must be Q4_K or Q6_K [k % 256 == 0, n, groups <= 1024]")
@@ -67,24 +68,25 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
             any(t.get_device() != dev for t in data) or (assignments is not None and assignments.get_device() != dev):
         raise ValueError("tensors must share one CUDA device, x and out have unit column stride and rows that do not overlap; "
                          "out must be float32, float16 or bfloat16")
+    word = _lib.status_pointer(status, dev)
     if rows == 0:
         return out
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return grouped_gemm(x, ranges, weight, up, assignments, topk, swiglu, None, out)
+            return grouped_gemm(x, ranges, weight, up, assignments, topk, swiglu, None, out, status)
     lib = _lib.lib()
     nbytes = lib.darask_ggml_grouped_workspace_bytes(rows, k, ty, 1 if swiglu else 0)
     scratch = x.new_empty(nbytes, dtype=torch.uint8)
     d = _lib.DaraskGgmlGrouped(groups, n, k, rows, ranges.data_ptr(), x.data_ptr(), ty, ldx, x.shape[0],
                                assignments.data_ptr() if assignments is not None else None, topk, 1 if swiglu else 0,
                                data[0].data_ptr(), data[1].data_ptr() if up is not None else None, weight.ty,
-                               out.data_ptr(), out_ty, ldo, scratch.data_ptr(), nbytes)
+                               out.data_ptr(), out_ty, ldo, scratch.data_ptr(), nbytes, word)
     _lib.check(lib.darask_ggml_grouped_gemm(ctypes.byref(d), _lib.current_stream(dev)), "darask_ggml_grouped_gemm")
     return out
 
 
 def grouped_status(device="cuda") -> int:
-    """Status bits that `grouped_gemm` calls on this device have set since the last look; clears them and synchronizes the current stream."""
+    """Status bits that `grouped_gemm` calls without a `status` of their own have set on this device since the last look; clears them and synchronizes the current stream."""
     s = ctypes.c_uint(0)
     device = torch.device(device)
     with torch.cuda.device(device):

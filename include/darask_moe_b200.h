@@ -401,8 +401,11 @@ int darask_fp8_ep_sum(float* out, const float* zr, int ranks, int tokens, int tc
  *   ld*      row strides in elements.  out must not overlap an input.
  *   workspace  darask_fp8_linear_workspace_bytes(m, n, k, x_ty) bytes, 256-byte aligned (0 bytes: may be NULL), not shared by
  *            calls that can overlap; nothing has to be initialised and nothing is kept between calls.
- * darask_fp8_linear_status copies the device's status word (DARASK_STATUS_WAIT_TIMEOUT) to *host_status and clears it; it
- * synchronizes the stream. */
+ *   status   a device word of the caller's to which the call's status bits (DARASK_STATUS_WAIT_TIMEOUT) are added; NULL: the word that all
+ *            such calls on the device share, which darask_fp8_linear_status takes.
+ * darask_status_take copies a status word to *host_status and clears it, in one step as far as running kernels can tell, and
+ * synchronizes the stream; the *_linear_status and *_grouped_status calls do so with the device's shared word. */
+int darask_status_take(unsigned* word, unsigned* host_status /* host */, darask_stream_t stream);
 enum { DARASK_E4M3 = 100 };
 typedef struct {
   int m, n, k;
@@ -413,6 +416,7 @@ typedef struct {
   const float* w_scales; long long ld_ws;
   void* out; int out_ty; long long ldo; int add;
   void* workspace; size_t workspace_bytes;
+  unsigned* status;
 } DaraskFp8Linear;
 size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_ty);
 int darask_fp8_linear(const DaraskFp8Linear* desc /* host */, darask_stream_t stream);
@@ -431,7 +435,8 @@ int darask_fp8_linear_status(unsigned* host_status /* host */, darask_stream_t s
  * parts (22 bits), f16 and bf16 rows as they are, with one power of two per row taken out first.  An infinity or a NaN in a row
  * makes the row's outputs NaN.  A range that leaves [0, rows) is cut, a row(i) >= x_rows reads as zeros, and of overlapping ranges
  * that hold many times `rows` the last ones may be left out; each sets
- * DARASK_STATUS_BAD_ROUTE in the device's status word (darask_ggml_grouped_status, as darask_fp8_linear_status).
+ * DARASK_STATUS_BAD_ROUTE in `status`, or without one in the device's shared word (darask_ggml_grouped_status, as for
+ * darask_fp8_linear).
  * workspace: darask_ggml_grouped_workspace_bytes(rows, k, x_ty, swiglu) bytes, 256-byte aligned, as for darask_fp8_linear. */
 typedef struct {
   int groups, n, k;
@@ -443,6 +448,7 @@ typedef struct {
   const void* w; const void* w_up; int w_ty;
   void* out; int out_ty; long long ldo;
   void* workspace; size_t workspace_bytes;
+  unsigned* status;
 } DaraskGgmlGrouped;
 size_t darask_ggml_grouped_workspace_bytes(long long rows, int k, int x_ty, int swiglu);
 int darask_ggml_grouped_gemm(const DaraskGgmlGrouped* desc /* host */, darask_stream_t stream);
