@@ -172,6 +172,7 @@ _SIGNATURES = {
     "kogarashi_moe_layer": (c_int, [ctypes.POINTER(KogarashiMoe), c_void_p]),
     "kogarashi_moe_prefill_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "kogarashi_moe_prefill": (c_int, [ctypes.POINTER(KogarashiMoe), c_int, c_void_p]),
+    "kogarashi_moe_prefill_checked": (c_int, [ctypes.POINTER(KogarashiMoe), c_int, c_void_p, c_void_p]),
     "kogarashi_moe_set_single_launch": (c_int, [c_int]),
     "kogarashi_moe_static_scratch_bytes": (c_size_t, []),
     "kogarashi_moe_layer_static": (c_int, [ctypes.POINTER(KogarashiMoe), c_void_p]),

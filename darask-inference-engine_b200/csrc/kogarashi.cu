@@ -300,11 +300,16 @@ __global__ void __launch_bounds__(256) prefill_position_kernel(const unsigned* a
 // A thread has COLS columns, so that a route's row is read with few and independent loads.
 template <int COLS>
 __global__ void __launch_bounds__(128) prefill_combine_kernel(float* x, const float* y, const float* ysh, const float* prob, const unsigned* position,
-                                                              const float* sg, int hidden, int topk, unsigned rows) {
+                                                              const float* sg, int hidden, int topk, unsigned rows, const unsigned* status,
+                                                              unsigned* status_sum) {
   __shared__ unsigned at[32];
   __shared__ float p[32];
   pdl_wait();
   pdl_launch();
+  if (status_sum && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    const unsigned bits = __ldcg(status);                // of all launches in front
+    if (bits) atomicOr(status_sum, bits);
+  }
   const int i = (blockIdx.y * 128 + threadIdx.x) * COLS, t = blockIdx.x;
   if (threadIdx.x < topk) {
     at[threadIdx.x] = __ldcg(position + size_t(t) * topk + threadIdx.x);
@@ -497,6 +502,11 @@ extern "C" size_t kogarashi_moe_prefill_workspace_bytes(int hidden, int inter, i
 }
 
 extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cudaStream_t st) {
+  return kogarashi_moe_prefill_checked(d, logits_given, nullptr, st);
+}
+
+extern "C" int kogarashi_moe_prefill_checked(const KogarashiMoe* d, int logits_given, unsigned* status_sum, cudaStream_t st) {
+  if (reinterpret_cast<uintptr_t>(status_sum) % 4) return cudaErrorInvalidValue;
   if (!descriptor_ok(d) || !d->workspace || reinterpret_cast<uintptr_t>(d->workspace) % 256) return cudaErrorInvalidValue;
   const int H = d->hidden, F = d->inter, E = d->experts, K = d->topk, T = d->tokens;
   if ((long long)T * K > (1ll << 27) || d->workspace_bytes < kogarashi_moe_prefill_workspace_bytes(H, F, E, K, T)) return cudaErrorInvalidValue;
@@ -540,6 +550,7 @@ extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cu
     g.x = d->n; g.x_ty = DARASK_GGML_F32; g.ldx = H; g.x_rows = T; g.assignments = assignments; g.topk = K;
     g.w = gate; g.w_up = up; g.w_ty = d->gate_ty;
     g.out = w.gu; g.out_ty = DARASK_GGML_F32; g.ldo = 2ll * F; g.workspace = w.products; g.workspace_bytes = w.products_bytes;
+    g.status = w.status;
     const int r = darask_ggml_grouped_gemm(&g, st);
     if (r) return (cudaError_t)r;
     g.n = H; g.k = F; g.x = w.gu; g.ldx = 2ll * F; g.x_rows = count; g.assignments = nullptr; g.swiglu = 1;
@@ -552,7 +563,7 @@ extern "C" int kogarashi_moe_prefill(const KogarashiMoe* d, int logits_given, cu
   const bool four = reinterpret_cast<uintptr_t>(d->x) % 16 == 0;
   return launch_pdl(four ? prefill_combine_kernel<4> : prefill_combine_kernel<1>, dim3(T, (H + (four ? 511 : 127)) / (four ? 512 : 128)), dim3(128), 0, st, d->x,
                     (const float*)w.y, shared ? (const float*)w.ysh : (const float*)nullptr, (const float*)d->prob, (const unsigned*)w.position,
-                    (const float*)w.sg, H, K, unsigned(routes));
+                    (const float*)w.sg, H, K, unsigned(routes), (const unsigned*)w.status, status_sum);
 }
 
 // ---- stand-alone pieces (also used by the parity tests) ------------------------------------------

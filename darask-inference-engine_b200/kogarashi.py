@@ -124,6 +124,7 @@ class KogarashiMoeLayer:
         self.logits = torch.empty(max_tokens, experts, dtype=torch.float32, device=self.device)
         self.ids = torch.empty(max_tokens, topk, dtype=torch.int32, device=self.device)
         self.prob = torch.empty(max_tokens, topk, dtype=torch.float32, device=self.device)
+        self._prefill_status = torch.zeros(1, dtype=torch.int32, device=self.device)      # of `prefill` calls, whose scratch does not last
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -252,7 +253,8 @@ class KogarashiMoeLayer:
         scratch = x.new_empty(nbytes, dtype=torch.uint8)
         d.workspace, d.workspace_bytes = scratch.data_ptr(), nbytes
         with torch.cuda.device(self.device):
-            _lib.check(lib.kogarashi_moe_prefill(ctypes.byref(d), 1 if given else 0, self._stream()), "kogarashi_moe_prefill")
+            _lib.check(lib.kogarashi_moe_prefill_checked(ctypes.byref(d), 1 if given else 0, self._prefill_status.data_ptr(), self._stream()),
+                       "kogarashi_moe_prefill")
         return x, ids, prob
 
     def forward_host(self, x_host: torch.Tensor, n_host: torch.Tensor, out_host: torch.Tensor | None = None) -> torch.Tensor:
@@ -302,6 +304,7 @@ class KogarashiMoeLayer:
         return plan["pin_out"]
 
     def status(self) -> int:
+        """Status bits of the last `forward` and of every `prefill` since the last look; synchronizes the current stream."""
         out = ctypes.c_uint(0)
         _lib.check(_lib.lib().kogarashi_moe_status(self.workspace.data_ptr(), ctypes.byref(out), self._stream()), "status")
-        return out.value
+        return out.value | _lib.take_status(self._prefill_status)

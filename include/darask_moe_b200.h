@@ -131,10 +131,13 @@ int kogarashi_moe_layer(const KogarashiMoe* desc /* host */, darask_stream_t str
 /* The same layer for prompts and large batches: the same descriptor and results (routing from the same logits, sums in another
  * order), the expert products through darask_ggml_grouped_gemm instead of passes of eight tokens.  `workspace` holds
  * kogarashi_moe_prefill_workspace_bytes(...) bytes, 256-byte aligned, needs no initialisation and belongs to the call (never the
- * one that kogarashi_moe_layer runs in, which keeps words between calls); kogarashi_moe_status reads its status word.  logits_given != 0: desc->logits holds the logits (router_bias included) and the
+ * one that kogarashi_moe_layer runs in, which keeps words between calls); kogarashi_moe_status reads its status word, which holds the
+ * bits of everything that the call launched, its products among them.  kogarashi_moe_prefill_checked adds (ORs) these bits to
+ * *status_sum as well, a device word of the caller's that lasts longer than the workspace (darask_status_take).  logits_given != 0: desc->logits holds the logits (router_bias included) and the
  * router projection is left out; the shared expert's gate is projected all the same. */
 size_t kogarashi_moe_prefill_workspace_bytes(int hidden, int inter, int experts, int topk, int tokens);
 int kogarashi_moe_prefill(const KogarashiMoe* desc /* host */, int logits_given, darask_stream_t stream);
+int kogarashi_moe_prefill_checked(const KogarashiMoe* desc /* host */, int logits_given, unsigned* status_sum, darask_stream_t stream);
 /* One token with an F32 router and Q4_K gate/up runs as ONE persistent launch (router rows, top-k in every CTA,
  * gate/up, down and combine; the CTAs hand logits, products and rows to each other as tagged words with bounded
  * polling, the weight stream running through); other shapes take four launches.  enabled = 0 makes the calling host thread take the four launches for one token as well

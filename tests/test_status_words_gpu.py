@@ -106,3 +106,75 @@ def test_two_readers_at_once():
         for t in threads:
             t.join(20)
         assert sorted(got) == [0, 0, 0, 5]
+
+
+def test_the_status_of_a_prompt_outlives_its_scratch():
+    """Bits in a call's workspace reach the caller's word. The bits come from the test, written to the workspace's status word from another
+    stream while the call runs (its own launches have no way to set one for a valid call)."""
+    import darask_inference_engine_b200 as D
+    from tests.test_kogarashi_gpu import run_layer
+    lib = D._lib.lib()
+    tokens = 900
+    layer, acts = W.kogarashi_layer(26, hidden=512, inter=256, experts=16, topk=4, tokens=tokens, shared=True, pool=8)
+    m, _ = run_layer(layer, {**acts, "x": acts["x"][:1], "n": acts["n"][:1]})
+    x, n = torch.from_numpy(acts["x"].copy()).cuda(), torch.from_numpy(acts["n"].copy()).cuda()
+    d = m._descriptor(x, n, None, None, 1e-6)
+    logits, ids, prob = torch.empty(tokens, 16, device="cuda"), torch.empty(tokens, 4, dtype=torch.int32, device="cuda"), torch.empty(tokens, 4, device="cuda")
+    d.logits, d.ids, d.prob = logits.data_ptr(), ids.data_ptr(), prob.data_ptr()
+    nbytes = lib.kogarashi_moe_prefill_workspace_bytes(512, 256, 16, 4, tokens)
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device="cuda")
+    d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
+    total = torch.zeros(1, dtype=torch.int32, device="cuda")
+    host = ctypes.c_uint(0)
+    # where the workspace keeps its status word: the one that kogarashi_moe_status reads
+    for at in range(0, 4096, 256):
+        ws.zero_()
+        ws[at:at + 4].view(torch.int32).fill_(1 << 20)
+        D._lib.check(lib.kogarashi_moe_status(ws.data_ptr(), ctypes.byref(host), D._lib.current_stream(0)), "status")
+        if host.value == 1 << 20:
+            break
+    else:
+        raise AssertionError("no status word found")
+    word = ws[at:at + 4].view(torch.int32)
+
+    def call():
+        D._lib.check(lib.kogarashi_moe_prefill_checked(ctypes.byref(d), 0, total.data_ptr(), D._lib.current_stream(0)), "prefill")
+    call()                                               # alone: the bit of before is cleared, none is set
+    assert D._lib.take_status(total) == 0
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        for _ in range(400):
+            word.fill_(1 << 21)
+    with torch.cuda.stream(side):
+        graph.replay()
+    for _ in range(4):
+        call()
+    torch.cuda.synchronize()
+    assert D._lib.take_status(total) == 1 << 21
+    # and the layer's own calls report to the layer
+    m.prefill(x, n)
+    assert m.status() == 0
+    m._prefill_status.fill_(1)
+    assert m.status() == 1 and m.status() == 0
+
+
+def test_prompts_hand_the_layers_word_to_the_library(monkeypatch):
+    import darask_inference_engine_b200 as D
+    from tests.test_kogarashi_gpu import run_layer
+    layer, acts = W.kogarashi_layer(27, hidden=256, inter=256, experts=4, topk=2, tokens=3, shared=False, pool=4)
+    m, _ = run_layer(layer, acts)
+    real, words = D._lib.lib(), []
+
+    class Recorder:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def kogarashi_moe_prefill_checked(self, d, given, word, stream):
+            words.append(word)
+            return real.kogarashi_moe_prefill_checked(d, given, word, stream)
+    monkeypatch.setattr(D._lib, "lib", Recorder)
+    x, n = torch.from_numpy(acts["x"].copy()).cuda(), torch.from_numpy(acts["n"].copy()).cuda()
+    m.prefill(x, n)
+    assert words == [m._prefill_status.data_ptr()]
+    assert m.status() == 0
