@@ -116,6 +116,7 @@ class Fp8MoeLayer:
         self.prob = torch.empty(max_tokens, topk, dtype=torch.float32, device=self.device)
         self.w = {}
         self.shared = None
+        self._shared_status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -158,10 +159,12 @@ class Fp8MoeLayer:
         _lib.check(_lib.lib().darask_fp8_moe_layer(ctypes.byref(d), self._stream()), "darask_fp8_moe_layer")
         if self.shared is not None:
             gu_w, gu_s, down_w, down_s = self.shared
-            linear(linear(x, gu_w, gu_s, out_dtype=torch.float32), down_w, down_s, swiglu=True, out=out, add=True)
+            rows = linear(x, gu_w, gu_s, out_dtype=torch.float32, status=self._shared_status)
+            linear(rows, down_w, down_s, swiglu=True, out=out, add=True, status=self._shared_status)
         return out
 
     def status(self) -> int:
+        """Status bits of the last call's routed experts and of the shared expert's products since the last look; synchronizes."""
         s = ctypes.c_uint(0)
         _lib.check(_lib.lib().darask_fp8_moe_status(self.workspace.data_ptr(), ctypes.byref(s), self._stream()), "darask_fp8_moe_status")
-        return s.value
+        return s.value | _lib.take_status(self._shared_status)

@@ -178,3 +178,29 @@ def test_prompts_hand_the_layers_word_to_the_library(monkeypatch):
     m.prefill(x, n)
     assert words == [m._prefill_status.data_ptr()]
     assert m.status() == 0
+
+
+def test_the_fp8_layer_reports_its_shared_expert(monkeypatch):
+    import darask_inference_engine_b200 as D
+    hidden, inter, tokens = 256, 128, 5
+    layer, acts = W.fp8_layer(3, hidden, inter, 8, 2, tokens)
+    m = D.Fp8MoeLayer(hidden, inter, 8, 2, tokens)
+    for name in ("gate", "up", "down"):
+        mats = getattr(layer, name)
+        m.load(name, torch.from_numpy(np.stack([p for p, _ in mats])), torch.from_numpy(np.stack([s for _, s in mats])))
+    rng = W.rng_for(17)
+    m.load_shared(*[tuple(torch.from_numpy(a) for a in F.fp8_block_quantize(W.normal(rng, s, s[1] ** -0.5))) for s in ((128, hidden), (128, hidden), (hidden, 128))])
+    x, logits = torch.from_numpy(acts["x"]).bfloat16().cuda(), torch.from_numpy(acts["logits"]).cuda()
+    want = m.forward(x, logits).clone()
+    assert m.status() == 0
+    real, words = D.fp8.linear, []
+
+    def linear(*args, status=None, **kw):
+        words.append(status)
+        out = real(*args, status=status, **kw)
+        status.bitwise_or_(len(words))                   # as a wait that runs out in the first or the second product would
+        return out
+    monkeypatch.setattr(D.fp8, "linear", linear)
+    assert torch.equal(m.forward(x, logits), want)
+    assert len(words) == 2 and m.status() == 3 and m.status() == 0
+    assert D.fp8.linear_status() == 0
