@@ -91,6 +91,7 @@ _SIGNATURES = {
     "darask_status_take": (c_int, [c_void_p, ctypes.POINTER(c_uint), c_void_p]),
     "darask_fp8_linear_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "darask_fp8_linear": (c_int, [ctypes.POINTER(DaraskFp8Linear), c_void_p]),
+    "darask_fp8_linear_plan": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]),
     "darask_fp8_linear_status": (c_int, [ctypes.POINTER(c_uint), c_void_p]),
     "darask_ggml_grouped_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int, c_int]),
     "darask_ggml_grouped_gemm": (c_int, [ctypes.POINTER(DaraskGgmlGrouped), c_void_p]),

@@ -37,8 +37,8 @@ __global__ void __launch_bounds__(256) fp8_linear_quant_kernel(const RowSource s
 struct LinearPlan { int nt, splits; bool fused, tile; };
 static bool linear_small(int m, int kb) { return m <= 8 && kb <= 8 * kFsResident; }
 // Rows of x per tile, blocks per cluster and kind of kernel by the time they are expected to take, in ns. The weights are fitted to a
-// sweep over 17 to 1024 rows of matrices from 1024 x 1536 to 8192 x 4096: a 128-column block of k takes 310, 390, 510 or 780 ns with
-// 16, 32, 64 or 128 rows (1.3 times as long where two blocks share an SM), joining S parts 450 S (1 + NT / 64), a 256 x 256 tile of the
+// sweep over 17 to 1024 rows of matrices from 1024 x 1536 to 8192 x 4096: a 128-column block of k takes 310, 390 or 780 ns with
+// 16, 32 or 128 rows (64 rows took 510, which 32 or 128 always beat, so there are no such tiles; 1.3 times as long where two blocks share an SM), joining S parts 450 S (1 + NT / 64), a 256 x 256 tile of the
 // pair kernel 550 ns per block of k and 900 more to start. (4096 x 4096, 256 rows: 128 rows in two parts 18.7 us, 32 rows undivided
 // 19.6, pairs 22.0; 512 rows: pairs 23.2, 128 rows 30.5.)
 static LinearPlan linear_plan(int m, int n, int kb, bool codes) {
@@ -53,8 +53,9 @@ static LinearPlan linear_plan(int m, int n, int kb, bool codes) {
     return p;
   }
   long long best = -1;
-  for (int nt = 16, unit = 0; nt <= 128; nt *= 2, ++unit) {
-    static const int kUnit[4] = {310, 390, 510, 780};
+  for (int unit = 0; unit < 3; ++unit) {
+    static const int kRows[3] = {16, 32, 128}, kUnit[3] = {310, 390, 780};
+    const int nt = kRows[unit];
     if (nt > 16 && nt / 2 >= m) break;                 // no wider than the rows need
     const long long tiles = tiles_n * ((m + nt - 1) / nt);
     for (int splits = 1; splits <= 8 && splits <= kb; splits *= 2) {
@@ -182,9 +183,17 @@ extern "C" int darask_fp8_linear(const DaraskFp8Linear* d, cudaStream_t st) {
   switch (p.nt) {
     case 16: return launch_stream<16, false>(mw, mx, a, int(tiles), p.splits, st);
     case 32: return launch_stream<32, false>(mw, mx, a, int(tiles), p.splits, st);
-    case 64: return launch_stream<64, false>(mw, mx, a, int(tiles), p.splits, st);
     default: return launch_stream<128, false>(mw, mx, a, int(tiles), p.splits, st);
   }
+}
+
+extern "C" int darask_fp8_linear_plan(int m, int n, int k, int x_ty, int* plan) {
+  if (!plan || m < 1 || n < 1 || k < 1 || m > (1 << 24) || n > (1 << 24) || k > (1 << 20) || (x_ty != DARASK_E4M3 && !row_type_bytes(x_ty))) return cudaErrorInvalidValue;
+  const LinearPlan p = linear_plan(m, n, (k + 127) / 128, x_ty == DARASK_E4M3);
+  plan[0] = p.tile ? 256 : p.nt;
+  plan[1] = p.tile ? 1 : p.splits;
+  plan[2] = p.fused;
+  return cudaSuccess;
 }
 
 extern "C" int darask_fp8_linear_status(unsigned* host_status, cudaStream_t st) {

@@ -42,7 +42,7 @@ struct FsArgs {
 
 template <int NT>
 struct FsShape {
-  static constexpr int kStages = NT <= 32 ? 5 : NT == 64 ? 8 : 6;
+  static constexpr int kStages = NT <= 32 ? 5 : 6;
   static constexpr int kStageBytes = 128 * 128 + NT * 128;
   static constexpr int kFactorFloats = 2 * kFsGroup * NT;
   static constexpr int kRingBytes = kStages * kStageBytes;

@@ -423,6 +423,9 @@ typedef struct {
 } DaraskFp8Linear;
 size_t darask_fp8_linear_workspace_bytes(int m, int n, int k, int x_ty);
 int darask_fp8_linear(const DaraskFp8Linear* desc /* host */, darask_stream_t stream);
+/* What a call of these sizes runs on the current device: plan[0] rows of x per tile (16, 32 or 128; 256: tiles of block pairs),
+ * plan[1] parts that k is divided into, plan[2] 1 where the rows are quantized in the product's launch. */
+int darask_fp8_linear_plan(int m, int n, int k, int x_ty, int* plan /* host, 3 words */);
 int darask_fp8_linear_status(unsigned* host_status /* host */, darask_stream_t stream);
 
 /* ---- product grouped by expert over GGUF weights ------------------------------------------------------------------
