@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(float* x, const fl
   using V = typename std::conditional<COLS == 4, float4, float>::type;
   union Row { V v; float f[COLS]; };
   Row sum = {}, own;
-  own.v = *reinterpret_cast<const V*>(x + size_t(t) * hidden + i);
+  own.v = __ldcg(reinterpret_cast<const V*>(x + size_t(t) * hidden + i));
 #pragma unroll 8
   for (int s = 0; s < topk; ++s) {
     if (at[s] >= rows) continue;

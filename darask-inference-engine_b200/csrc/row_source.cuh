@@ -68,14 +68,9 @@ DEVI void row_source_load4(const RowSource& s, long long row, int c, float (&v)[
   }
 }
 
-DEVI float read_elem(const void* p, int ty, size_t i) {          // of an output that is added to
-  if (ty == DARASK_GGML_F32) return static_cast<const float*>(p)[i];
-  if (ty == DARASK_GGML_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
 // one result in the output's type, rounded once from float32; `add`: on top of what is there
 DEVI void store_elem(void* out, int ty, size_t i, float v, int add = 0) {
-  if (add) v += read_elem(out, ty, i);
+  if (add) v += load_elem(out, ty, i);
   if (ty == DARASK_GGML_F32) static_cast<float*>(out)[i] = v;
   else if (ty == DARASK_GGML_F16) static_cast<__half*>(out)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
