@@ -32,8 +32,10 @@ __global__ void __launch_bounds__(256) fp8_linear_quant_kernel(const RowSource s
   reinterpret_cast<uint32_t*>(codes)[w * 32 + lane] = out;
 }
 
-// What a call runs. `fused` (rows quantized in the product's launch) depends on m and k alone, as the workspace does: one launch less
-// (4.9 against 5.0 us on the device for 6 rows of 2048 x 2048, 9.2 against 7.8 for 8 of 4096 x 4096, and 4 us less on the host).
+// What a call runs. `fused` (rows quantized in the product's launch) depends on m and k alone, as the workspace does. It saves a launch, 4 us
+// on the host, which is what bounds such calls when they are made one by one (9.8 us a call for 8 rows of 4096 x 4096 bf16); in a
+// captured graph it gains nothing for small matrices (4.9 against 5.0 us for 6 rows of 2048 x 2048) and loses for large ones, where
+// every block quantizes its part of k again (9.2 against 7.8 us for 8 rows of 4096 x 4096).
 struct LinearPlan { int nt, splits; bool fused, tile; };
 static bool linear_small(int m, int kb) { return m <= 8 && kb <= 8 * kFsResident; }
 // Rows of x per tile, blocks per cluster and kind of kernel by the time they are expected to take, in ns. The weights are fitted to a

@@ -9,9 +9,10 @@
 //   warps 4-7   tcgen05.ld of the block's partial tile (thread = one weight row), times the factors, added in registers
 // FUSED: x comes as float rows; before the loop all warps but 0 quantize this block's part of x straight into the
 // swizzled operand tiles, which stay in shared memory (one tile of 16 for up to 8 rows, at most kFsResident blocks of k): one launch.
-// Bound: a single row by the latency of one pass (4096 x 4096: 6.1 us on the device, 2.75 TB/s, 2.6 us at the rate of a copy; start,
-// quantizer, four dependent ring rounds and the join are the rest), more rows by the promotion, which costs a block of k 310 ns with 16
-// rows and 780 with 128 (256 rows of 4096 x 2048: 13.4 us). Rows as the N operand: as M they would cost a 128-row tile for one token.
+// Bound: a single row by the latency of one pass (4096 x 4096 in a graph of calls: 6.3 us with other weights in every call, 2.65 TB/s, 5.9 with
+// the same ones, which L2 holds; 2.6 us at the rate of a copy; start, quantizer, four dependent ring rounds and the join are the rest),
+// more rows by the promotion, which costs a block of k 310 ns with 16 rows and 780 with 128 (256 rows of 4096 x 2048: 14.6 us with the
+// quantizer in front, in tiles of 32 rows). Rows as the N operand: as M they would cost a 128-row tile for one token.
 #pragma once
 #include <cuda_fp8.h>
 #include "row_source.cuh"

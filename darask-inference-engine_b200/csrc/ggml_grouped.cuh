@@ -61,10 +61,6 @@ struct GgShape {
   static constexpr int kSums = Q6 ? 0 : NT * 32;         // NT rows x 16 f16: the sums of eight groups of 32 columns, high and low parts
   static constexpr int kXStage = NX * kPart + kSums;     // Q4_K: the sums travel with the second step of a block
   static constexpr int kXStages = kWide && NX == 2 ? 2 : 4;
-  // Partial products per block. The tensor core cuts the sum of every 16 columns to the accumulator's 24 bits, toward zero, so that the
-  // error grows with the number of sums and does not average out. Integers times bf16 or f16 hardly have bits to lose (3e-7 of the result
-  // over 256 columns); two parts do: multiplied into one accumulator in turn they lost 1.5e-6 (Q4_K; Q6_K 8e-7). So there the small
-  // products come first and every step has an accumulator of its own (PREC).
   // Partial products per block of 256 columns. The tensor core cuts the sum of every 16 columns to the accumulator's 24 bits, toward
   // zero, so that the error grows with the number of sums and does not average out; products of two parts have bits to lose. In turn in
   // one accumulator they lost 1.5e-6 of the result (Q4_K, whose codes have no sign and largely cancel against the mins) and 8e-7 (Q6_K).
