@@ -98,7 +98,8 @@ def linear(x, w, w_scales, x_scales=None, swiglu=False, out_dtype=None, out=None
 
 
 def linear_status(device="cuda") -> int:
-    """Status bits that `linear` calls without a `status` of their own have set on this device since the last look; clears them and synchronizes the current stream."""
+    """Status bits that `linear` calls without a `status` of their own have set on this device since the last look; clears them and
+    synchronizes the current stream."""
     s = ctypes.c_uint(0)
     device = torch.device(device)
     with torch.cuda.device(device):

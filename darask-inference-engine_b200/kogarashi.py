@@ -86,7 +86,8 @@ def grouped_gemm(x, ranges, weight, up=None, assignments=None, topk=1, swiglu=Fa
 
 
 def grouped_status(device="cuda") -> int:
-    """Status bits that `grouped_gemm` calls without a `status` of their own have set on this device since the last look; clears them and synchronizes the current stream."""
+    """Status bits that `grouped_gemm` calls without a `status` of their own have set on this device since the last look; clears them and
+    synchronizes the current stream."""
     s = ctypes.c_uint(0)
     device = torch.device(device)
     with torch.cuda.device(device):

@@ -2,8 +2,8 @@
  *
  * Conventions, the same as the reference engine's kernel launchers
  * (engines/hayate/crates/kernels/src/cuda.rs:29-36): every call only enqueues work on the
- * given stream, never allocates and never synchronizes (the two *_status calls, which copy one
- * word back, are the exception); device pointers must stay valid until the stream has passed
+ * given stream, never allocates and never synchronizes (the *_status calls and darask_status_take,
+ * which copy one word back, are the exception); device pointers must stay valid until the stream has passed
  * the launch; the return value is a cudaError_t as int, cudaErrorInvalidValue (1) for
  * arguments that fail validation.  All pointers are device pointers unless a comment says
  * "host".  `stream` is a cudaStream_t / CUstream.
@@ -105,8 +105,8 @@ typedef struct {
   const void* gate_w; int gate_ty;                     /* ffn_gate_exps       [hidden, inter, E]    */
   const void* up_w; int up_ty;                         /* ffn_up_exps                               */
   const void* down_w; int down_ty;                     /* ffn_down_exps       [inter, hidden, E]    */
-  const void* sh_gate_w; const void* sh_up_w;          /* ffn_{gate,up}_shexp, same types; NULL: no shared expert */
-  const void* sh_down_w;                               /* ffn_down_shexp                            */
+  const void* sh_gate_w; const void* sh_up_w;          /* ffn_{gate,up}_shexp, same types and width; NULL: no shared expert */
+  const void* sh_down_w;                               /* ffn_down_shexp, type down_ty              */
   const void* sh_inp_w;                                /* ffn_gate_inp_shexp  [hidden], type router_ty */
   float* n;                                            /* [tokens][hidden] normalised input (buffer "n"); written when norm_w is set */
   float* x;                                            /* [tokens][hidden] residual stream, updated in place ("x") */
@@ -437,8 +437,10 @@ int darask_fp8_linear_status(unsigned* host_status /* host */, darask_stream_t s
  *   swiglu   rows of x hold gate | up (2k columns) and silu(gate) * up is multiplied (the down product).
  *   out      [rows][ldo], overlapping no input; rows outside every range are left as they were, ranges do not overlap (a row in
  *            two of them holds either product).
- * Sums in float32; weights enter as exact integers (Q4_K, Q6_K: block scale times an integer), float32 rows as two f16
- * parts (22 bits), f16 and bf16 rows as they are, with one power of two per row taken out first.  An infinity or a NaN in a row
+ * Sums in float32, rounded once to out's type; weights enter as exact integers (Q4_K, Q6_K: block scale times an integer), float32 rows and
+ * SwiGLU products as two f16 parts (22 bits), f16 and bf16 rows as they are, with one power of two per row taken out first (what lies
+ * below 2^-34 of the row's largest value is lost).  The tensor core cuts the sum of every 16 columns to 24 bits: float32 results are off by
+ * 3e-7 to 6e-7 of their size.  An infinity or a NaN in a row
  * makes the row's outputs NaN.  A range that leaves [0, rows) is cut, a row(i) >= x_rows reads as zeros, and of overlapping ranges
  * that hold many times `rows` the last ones may be left out; each sets
  * DARASK_STATUS_BAD_ROUTE in `status`, or without one in the device's shared word (darask_ggml_grouped_status, as for
